@@ -389,6 +389,35 @@ int lev_qkv_norm_rope_append_split(lev_ctx* ctx, float* q, float* k, float* v, i
                                    const int32_t* pos, const lev_kv_layout* layout, void* k_pool,
                                    void* v_pool, const int32_t* block_table, const int32_t* slot);
 
+/* ---- attention of many rows per sequence (prompts, prompt pieces, drafted tokens) ------
+ * Element types of activations that these and the scoring entry points take. */
+enum { LEV_ELEM_F32 = 0, LEV_ELEM_F16 = 1, LEV_ELEM_BF16 = 2 };
+/* lev_attn_chunk: a chunk of new tokens per sequence over the paged cache that already holds their K and V rows
+ * (lev_kv_append or lev_qkv_norm_rope_append first): the prompt side of lev_attn_decode.  Rows start[c] ... start[c+1]-1
+ * of q and out belong to chunk c, whose first row is at position pos[c] of sequence slot[c]; the row at position p attends to
+ * (p - window, p] (window 0: [0, p]), weights softmax(scale * q.k), query head h reads KV head h / (q_heads / kv_heads).
+ * Replaces one attn_decode per token of the reference's prefill (rust/crates/lev-model/src/gpu.rs:1346).
+ *   start int32 [n_chunks + 1], slot and pos int32 [n_chunks] on the device; a chunk may be empty; rows outside
+ *   [start[0], start[n_chunks]) are not written.  n_rows: rows that q and out hold.
+ *   q f32 (rounded to f16: magnitudes above 65504 are not served) or f16, out f16 or bf16 (what lev_gemm_prefill reads);
+ *   rows q_ld and out_ld elements apart (whole 16-byte steps, 16-byte aligned), heads contiguous: q may be the leading part of
+ *   each row of a fused projection output.  out must not overlap q.  f32 caches are rounded to f16 in the same way.
+ *   head_dim 128 or 256; up to 16 query heads per KV head; any page size (powers of two from 8 on are fastest).
+ * A slot or position outside the layout, or a table entry outside the pool, is not followed: rows of that chunk are NaN; start entries
+ * that are no range leave their chunk out; both are reported by the next status read.  Cached values that a row does not attend to may
+ * be anything, NaN included.  No work buffers: captured graphs and streams share nothing.  Repeat runs give the same bits. */
+int lev_attn_chunk(lev_ctx* ctx, const lev_kv_layout* layout, const void* k_pool, const void* v_pool,
+                   const int32_t* block_table, int n_chunks, const int32_t* start, const int32_t* slot,
+                   const int32_t* pos, int64_t n_rows, int q_heads, const void* q, int q_type,
+                   int64_t q_ld, int window, float scale, void* out, int out_type, int64_t out_ld);
+/* lev_attn_prompt: whole prompts packed behind one another, no cache: row i of sequence s attends to rows
+ * (i - window, i] of the same sequence.  q, k, v and out of one type (f16 or bf16), rows *_ld elements apart, heads contiguous (k and
+ * v may be parts of the rows of a fused projection output); everything else as lev_attn_chunk. */
+int lev_attn_prompt(lev_ctx* ctx, int n_seqs, const int32_t* start, int64_t n_rows, int q_heads,
+                    int kv_heads, int head_dim, int type, const void* q, int64_t q_ld, const void* k,
+                    int64_t k_ld, const void* v, int64_t v_ld, int window, float scale, void* out,
+                    int64_t out_ld);
+
 /* ---- routed MoE composite ----------------------------------------------
  * Expert weights are the fused gate_up tensor [experts][2*inter][hidden] and
  * the down tensor [experts][hidden][inter], both Q4_0

@@ -70,6 +70,8 @@ class KVLayout(C.Structure):
 
 
 KV_F32, KV_F16 = 0, 1
+ELEM_F32, ELEM_F16, ELEM_BF16 = 0, 1, 2
+NO_TOKEN = -1
 
 # name -> (restype, argtypes); every symbol the header declares
 _P, _I, _L, _Z, _U = C.c_void_p, C.c_int, C.c_int64, C.c_size_t, C.c_uint
@@ -112,6 +114,8 @@ SIGNATURES = {
     "lev_kv_append": (_I, [_P, C.POINTER(KVLayout), _P, _P, _P, _P, _P, _I, _P, _P]),
     "lev_attn_decode": (_I, [_P, C.POINTER(KVLayout), _P, _P, _P, _P, _P, _I, _I, _P, _I, C.c_float, _P]),
     "lev_attn_decode_ld": (_I, [_P, C.POINTER(KVLayout), _P, _P, _P, _P, _P, _I, _I, _P, _L, _I, C.c_float, _P]),
+    "lev_attn_chunk": (_I, [_P, C.POINTER(KVLayout), _P, _P, _P, _I, _P, _P, _P, _L, _I, _P, _I, _L, _I, C.c_float, _P, _I, _L]),
+    "lev_attn_prompt": (_I, [_P, _I, _P, _L, _I, _I, _I, _I, _P, _L, _P, _L, _P, _L, _I, C.c_float, _P, _L]),
     "lev_gemm_prefill": (_I, [_P, _P, _P, _L, _P, _U]),
     "lev_act_bf16": (_I, [_P, _P, _L, _P]),
     "lev_moe_weights_upload": (_I, [_P, _P, _P, _Z, _P, _Z, _I, _I, _I, _I, _I, _I, C.POINTER(_P)]),
@@ -182,7 +186,7 @@ class _CtypesHost:
 
     def __init__(self, lib: C.CDLL):
         self._lib = lib
-        for name in ("matvec", "rmsnorm", "axpy", "act_bf16", "gemm_prefill", "moe_layer", "moe_layer_residual"):
+        for name in ("matvec", "rmsnorm", "axpy", "act_bf16", "gemm_prefill", "moe_layer", "moe_layer_residual", "attn_prompt"):
             setattr(self, name, getattr(lib, "lev_" + name))
 
     def matvec_fused(self, ctx, w, row0, rows, x, x_count, n_cols, prologue, norm_weight, eps, residual, alpha, y, cap):
@@ -194,6 +198,9 @@ class _CtypesHost:
 
     def kv_append(self, ctx, layout, *args):
         return self._lib.lev_kv_append(ctx, C.cast(layout, C.POINTER(KVLayout)), *args)
+
+    def attn_chunk(self, ctx, layout, *args):
+        return self._lib.lev_attn_chunk(ctx, C.cast(layout, C.POINTER(KVLayout)), *args)
 
     def attn_decode(self, ctx, layout, *args):
         return self._lib.lev_attn_decode(ctx, C.cast(layout, C.POINTER(KVLayout)), *args)

@@ -40,6 +40,39 @@ def _ptr(a):
     return a.ctypes.data
 
 
+_ELEM = {}
+
+
+def _elem(t, what: str, allowed: str) -> int:
+    """LEV_ELEM_* of a CUDA tensor's type, one of `allowed` (names separated by spaces)."""
+    if not _ELEM:
+        import torch
+
+        _ELEM.update({torch.float32: (L.ELEM_F32, "float32"), torch.float16: (L.ELEM_F16, "float16"), torch.bfloat16: (L.ELEM_BF16, "bfloat16")})
+    code, name = _ELEM.get(t.dtype, (None, str(t.dtype)))
+    if name not in allowed:
+        raise TypeError(f"{what} is {name}: {allowed.replace(' ', ' or ')} is wanted")
+    return code
+
+
+def _head_rows(t, what: str):
+    """[rows][heads][head_dim] with heads and dims contiguous, as the parts of a fused projection output lie: its row stride."""
+    if t.ndim != 3 or t.stride(2) != 1 or t.stride(1) != t.shape[2]:
+        raise ValueError(f"{what}: [rows][heads][head_dim] with contiguous heads is wanted, got shape {tuple(t.shape)}, strides {t.stride()}")
+    return t.stride(0)
+
+
+def _i32(t, n: int, what: str):
+    if t.numel() != n or str(t.dtype) != "torch.int32" or not t.is_contiguous():
+        raise ValueError(f"{what}: {n} contiguous int32 values are wanted, got {t.numel()} of {t.dtype}")
+
+
+def _on(device: int, *tensors):
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device.index != device):
+            raise ValueError(f"a tensor lies on {t.device}, the context on cuda:{device}")
+
+
 def _raw_stream(device: int) -> int:
     """torch's current stream of a device as a cudaStream_t value."""
     global _raw_stream
@@ -447,6 +480,51 @@ class Context:
                                                 _ptr(out)))
         return out
 
+    # -- attention of many rows per sequence (torch CUDA tensors only) --
+    def attn_chunk(self, cache: "PagedKV", start, slot, pos, q, window: int = 0, scale: float = 1.0, out=None, dtype=None):
+        """lev_attn_chunk: rows start[c] ... start[c + 1] - 1 of q [rows][q_heads][head_dim] (f32 or f16; rows may be a stride apart)
+        are new tokens of sequence slot[c] from position pos[c] on, whose K and V rows are in the cache already -> out of q's
+        shape in bf16 (or `dtype` float16); start, slot and pos are int32 device tensors."""
+        import torch
+
+        n = slot.numel()
+        if out is None:
+            out = torch.empty(q.shape, dtype=dtype or torch.bfloat16, device=q.device)
+        _on(self.device, q, out, start, slot, pos, cache.k)
+        q_ld, out_ld = _head_rows(q, "q"), _head_rows(out, "out")
+        if out.shape != q.shape or q.shape[2] != cache.layout.head_dim:
+            raise ValueError(f"q {tuple(q.shape)}, out {tuple(out.shape)}, head dimension {cache.layout.head_dim} of the cache")
+        _i32(start, n + 1, "start")
+        _i32(slot, n, "slot")
+        _i32(pos, n, "pos")
+        qt, ot = _elem(q, "q", "float32 float16"), _elem(out, "out", "float16 bfloat16")
+        self._flags(False, False)
+        self._check(self.host.attn_chunk(self._h, C.addressof(cache.layout), _ptr(cache.k), _ptr(cache.v), _ptr(cache.table), n, _ptr(start),
+                                         _ptr(slot), _ptr(pos), q.shape[0], q.shape[1], _ptr(q), qt, q_ld, window, scale, _ptr(out), ot, out_ld))
+        return out
+
+    def attn_prompt(self, q, k, v, start, window: int = 0, scale: float = 1.0, out=None):
+        """lev_attn_prompt: causal attention of whole prompts packed behind one another; q [rows][q_heads][head_dim], k and v
+        [rows][kv_heads][head_dim] of one 16-bit type, rows may be a stride apart (views of a fused projection output);
+        start int32 [sequences + 1] on the device."""
+        import torch
+
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _on(self.device, q, k, v, out, start)
+        n = start.numel() - 1
+        q_ld, k_ld, v_ld, out_ld = _head_rows(q, "q"), _head_rows(k, "k"), _head_rows(v, "v"), _head_rows(out, "out")
+        if out.shape != q.shape or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+            raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, out {tuple(out.shape)}")
+        _i32(start, n + 1, "start")
+        ty = _elem(q, "q", "float16 bfloat16")
+        if not (q.dtype == k.dtype == v.dtype == out.dtype):
+            raise TypeError(f"q, k, v and out are of one type: got {q.dtype}, {k.dtype}, {v.dtype}, {out.dtype}")
+        self._flags(False, False)
+        self._check(self.host.attn_prompt(self._h, n, _ptr(start), q.shape[0], q.shape[1], k.shape[1], q.shape[2], ty, _ptr(q), q_ld, _ptr(k), k_ld,
+                                          _ptr(v), v_ld, window, scale, _ptr(out), out_ld))
+        return out
+
     def _matvec_host(self, fn, blocks, out_dim, in_dim, x):
         blocks = np.ascontiguousarray(blocks, np.uint8)
         x = np.ascontiguousarray(x, np.float32)
@@ -668,6 +746,27 @@ class PagedKV:
         self.free = list(range(blocks - 1, 0, -1))
         self.owned = [[] for _ in range(slots)]
         self.page, self.max_blocks = page, max_blocks
+
+    @classmethod
+    def over(cls, k, v, table) -> "PagedKV":
+        """A cache handle over pools [blocks][page][kv_heads][head_dim] and an int32 block table [slots][max_blocks] that the caller
+        keeps and fills (`ensure` and `release` are not for such a handle: the caller hands out the blocks)."""
+        import torch
+
+        if k.shape != v.shape or k.dtype != v.dtype or k.ndim != 4 or not k.is_contiguous() or not v.is_contiguous():
+            raise ValueError(f"pools {tuple(k.shape)} of {k.dtype} and {tuple(v.shape)} of {v.dtype}: two contiguous ones of one shape are wanted")
+        if table.ndim != 2 or table.dtype is not torch.int32 or not table.is_contiguous():
+            raise ValueError(f"block table {tuple(table.shape)} of {table.dtype}: int32 [slots][max_blocks] is wanted")
+        kind = {torch.float16: L.KV_F16, torch.float32: L.KV_F32}.get(k.dtype)
+        if kind is None:
+            raise TypeError(f"cache pools of {k.dtype}: float16 or float32 is wanted")
+        self = cls.__new__(cls)
+        blocks, page, kv_heads, head_dim = k.shape
+        self.layout = L.KVLayout(kind, page, kv_heads, head_dim, blocks, table.shape[1], table.shape[0])
+        self.k, self.v, self.table = k, v, table
+        self.page, self.max_blocks = page, table.shape[1]
+        self.table_host, self.free, self.owned = None, [], None
+        return self
 
     def ensure(self, slot: int, pos: int) -> int:
         """Make sequence `slot` own the block of `pos`; returns the flat pool position."""

@@ -824,9 +824,7 @@ __global__ void k_kv_append(AttnArgs A, void* k_pool, void* v_pool, const float*
 
 }  // namespace
 
-namespace {
-
-int check_layout(lev_ctx* ctx, const lev_kv_layout* L) {
+int lev_check_kv_layout(lev_ctx* ctx, const lev_kv_layout* L) {
     if (!L) return LEV_BAD_ARGUMENT;
     if (L->kv_type != LEV_KV_F16 && L->kv_type != LEV_KV_F32) return lev_fail(ctx, LEV_BAD_ARGUMENT, "cache element type %d", L->kv_type);
     if (L->head_dim != 128 && L->head_dim != 256) return lev_fail(ctx, LEV_UNSUPPORTED, "head dimension %d (128 or 256)", L->head_dim);
@@ -836,6 +834,8 @@ int check_layout(lev_ctx* ctx, const lev_kv_layout* L) {
                         (long long)L->blocks, L->max_blocks, L->slots);
     return LEV_OK;
 }
+
+namespace {
 
 AttnArgs base_args(lev_ctx* ctx, const lev_kv_layout* L, const int32_t* table, const int32_t* slot, const int32_t* pos) {
     AttnArgs A = {};
@@ -908,7 +908,7 @@ cudaError_t launch_split_g(int group, dim3 grid, size_t smem, cudaStream_t strea
 extern "C" int lev_kv_append(lev_ctx* ctx, const lev_kv_layout* L, void* k_pool, void* v_pool, const int32_t* block_table,
                              const int32_t* slot, const int32_t* pos, int n_cols, const float* k, const float* v) {
     if (!ctx || !k_pool || !v_pool || !block_table || !slot || !pos || !k || !v) return LEV_BAD_ARGUMENT;
-    LEV_TRY(check_layout(ctx, L));
+    LEV_TRY(lev_check_kv_layout(ctx, L));
     if (n_cols < 1 || n_cols > 65535) return lev_fail(ctx, LEV_BAD_DIMENSIONS, "columns %d", n_cols);
     LEV_CUDA(ctx, cudaSetDevice(ctx->device));
     AttnArgs A = base_args(ctx, L, block_table, slot, pos);
@@ -935,7 +935,7 @@ extern "C" int lev_attn_decode_ld(lev_ctx* ctx, const lev_kv_layout* L, const vo
                                   const int32_t* slot, const int32_t* pos, int n_cols, int q_heads, const float* q, int64_t q_ld, int window,
                                   float scale, float* out) {
     if (!ctx || !k_pool || !v_pool || !block_table || !slot || !pos || !q || !out) return LEV_BAD_ARGUMENT;
-    LEV_TRY(check_layout(ctx, L));
+    LEV_TRY(lev_check_kv_layout(ctx, L));
     if (q_ld < (int64_t)q_heads * L->head_dim || q_ld % 2 != 0 || ((uintptr_t)q & 7) != 0)
         return lev_fail(ctx, LEV_BAD_ARGUMENT, "query rows %lld elements apart (at least %lld, even, 8-byte aligned)", (long long)q_ld,
                         (long long)q_heads * L->head_dim);

@@ -1,0 +1,1013 @@
+// Causal attention of many query rows per sequence on the fifth-generation tensor cores (tcgen05 + TMEM + TMA), sm_100a:
+// a chunk of new tokens over the paged KV cache (lev_attn_chunk) and whole prompts packed behind one another
+// (lev_attn_prompt).
+//
+//   out[i][h] = sum_j softmax_j(scale * q[i][h] . K[j][h / group]) V[j][h / group],   j in (p_i - window, p_i]
+//
+// (the single-query form is lev_attn.cu; g4_attn, Sources/LeviathanCore/Gemma4.swift:4412-4457, one row of this.)
+//
+// A tile is 128 MMA rows: the `group` query heads of one KV head for as many consecutive tokens as fit, so K and V are
+// read once for all heads that share them.  Positions are walked in steps of 128 with the running maximum and sum of
+// the softmax:
+//   S = Q K^T      both operands in shared memory (K-major, 128-byte swizzle), 128 columns of tensor memory
+//   P = 2^(S' - m) by one warpgroup per tile, a thread per row; P goes back to tensor memory in 16 bits over S
+//   O += P V       P from tensor memory, V from shared memory as it lies in the cache ([position][dim]: N-major)
+// The reference m of a row follows its running maximum only when that has moved by more than 2^8 (the weights stay
+// below 256, exact in 16 bits to the same relative error), so that O is rescaled in a handful of steps and not in every
+// one.  Sums of weights are f32, O is f32 in tensor memory.  Rounded to 16 bits: q where it comes as f32 (the cache is
+// f16, and both operands of an MMA have one type), P (11 bits for f16, 8 for bf16 prompts), the output.
+//
+// Roles of a CTA: one (two) softmax warpgroup(s), one warp that issues MMAs, one that issues TMA boxes; where the cache
+// cannot be boxed (f32 pools, page sizes that neither divide 128 nor are multiples of it) the last three warps of the
+// CTA copy and convert rows instead.  Every wait is bounded (about a second, then LEV_TIMEOUT).
+//
+// Places that a row does not attend to may hold anything, NaN included.  Scores there are replaced, but 0 * NaN is NaN
+// in the product with V: a row whose sums come out non-finite is computed once more, position by position, over the
+// places that it does attend to (tc_row_again; never taken where all values are finite).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "lev_stream.h"
+#include "lev_umma.cuh"
+
+namespace {
+
+constexpr int TC_KV = 128;                 // positions per step
+constexpr unsigned TC_STAGE = 32768;       // 128 rows x 128 columns of 16 bits: two slabs of 64 columns
+constexpr int TC_MAX_STAGES = 6;
+constexpr int TC_LOAD_WARPS = 3;           // copying warps where TMA boxes do not apply
+constexpr float TC_LAZY = 8.0f;            // how far (log2) the maximum may run ahead of a row's reference
+enum { TC_F32 = LEV_ELEM_F32, TC_F16 = LEV_ELEM_F16, TC_BF16 = LEV_ELEM_BF16 };
+
+struct TcArgs {
+    const void* q;
+    int64_t q_ld;
+    int q_type, mma_type, out_type, kv_type;   // LEV_ELEM_*; mma_type: what the tensor core multiplies
+    void* out;
+    int64_t out_ld;
+    const int32_t *start, *slot, *pos, *table; // table NULL: packed prompts, positions count from start[]
+    const void *k, *v;
+    int64_t k_ld, v_ld;                        // packed: elements between rows
+    int64_t rows, blocks;
+    int seqs, q_heads, kv_heads, group, tpt;   // tpt: tokens of a 128-row tile
+    int page, max_blocks, slots;
+    int box_k, box_v;                          // rows of a TMA box; 0: rows are copied by warps
+    int window, splits, negate;
+    float sl;                                  // |scale| * log2(e)
+    int* status;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ unsigned pack16(float lo, float hi, int type) {
+    unsigned r;
+    if (type == TC_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 two(float lo, float hi) {
+    f32x2 v;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+__device__ __forceinline__ void both(f32x2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma_2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+__device__ __forceinline__ f32x2 add_2(f32x2 a, f32x2 b) {
+    f32x2 v;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ void tmem_st32(unsigned a, const unsigned* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n" ::"r"(a),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
+        "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]),
+        "r"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void wg_sync(int id) { asm volatile("bar.sync %0, 128;\n" ::"r"(id) : "memory"); }
+
+// O[128 x N] += P[128 x 128] V[128 x N]: P from tensor memory (64 columns of packed pairs), V N-major in shared memory
+// (slabs of 64 dims, 128-byte rows of one position each).  Eight MMAs of 16 positions: P steps by 8 columns, V by 2 KB.
+// Descriptor low word: address, distance between slabs; high word: 8 positions = 1024 bytes, version, 128-byte swizzle.
+template <int CG>
+__device__ __forceinline__ void tc_pv(unsigned d, unsigned p, unsigned b_lo, unsigned idesc, unsigned acc, unsigned elected) {
+    constexpr unsigned kDescHi = (unsigned)((1024 >> 4) | (1u << 14) | (2u << 29));
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+#define LEV_PV(GROUP)                                                                                          \
+    asm volatile(                                                                                              \
+        "{\n .reg .pred p, q;\n .reg .b64 db;\n setp.ne.b32 p, %5, 0;\n setp.ne.b32 q, %6, 0;\n"               \
+        " mov.b64 db, {%2, %4};\n"                                                                             \
+        " @q tcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d),                 \
+        "r"(p + 8u * i), "r"(b_lo + 128u * i), "r"(idesc), "r"(kDescHi), "r"(i ? 1u : acc), "r"(elected)       \
+        : "memory")
+        if (CG == 2) LEV_PV("2");
+        else LEV_PV("1");
+#undef LEV_PV
+    }
+}
+// one box of a cache page (column, head, row of the page, block) or of packed rows (column, head, row)
+template <int CG, int DIMS>
+__device__ __forceinline__ void tc_box(unsigned dst, const CUtensorMap* map, int x, int h, int r, int b, unsigned bar, unsigned elected) {
+#define LEV_BOX(GROUP)                                                                                                       \
+    if (DIMS == 4)                                                                                                           \
+        asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %7, 0;\n"                                                           \
+                     " @q cp.async.bulk.tensor.4d" GROUP ".shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n}\n" \
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(h), "r"(r), "r"(b), "r"(bar), "r"(elected) \
+                     : "memory");                                                                                            \
+    else                                                                                                                     \
+        asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %6, 0;\n"                                                           \
+                     " @q cp.async.bulk.tensor.3d" GROUP ".shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n}\n" \
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(h), "r"(r), "r"(bar), "r"(elected)         \
+                     : "memory")
+    if (CG == 2) {
+        LEV_BOX(".cta_group::2");
+    } else {
+        LEV_BOX("");
+    }
+#undef LEV_BOX
+}
+
+// what a unit (a CTA, a pair, or the CTAs of a split) works on
+struct TcUnit {
+    int seq, t0, len;   // sequence, first token of the unit, tokens of the sequence
+    int row0;           // first row of the sequence
+    int pos0;           // position of its first token
+    int slot;
+    int ok;             // slot and positions inside the layout
+};
+
+// unit u of all sequences' units (each sequence has ceil(tokens / per), the last tokens first: they attend to most).
+// One warp; false when there are fewer units.  A pair of start[] entries that is no range counts as an empty sequence.
+__device__ bool tc_find(const TcArgs& A, int u, int per, int lane, TcUnit* U) {
+    int before = 0;
+    bool found = false;
+    for (int s0 = 0; s0 < A.seqs && (!found || u == 0); s0 += 32) {   // the first unit looks all of start[] over
+        const int s = s0 + lane;
+        int a = 0, n = 0;
+        if (s < A.seqs) {
+            a = A.start[s];
+            const int b = A.start[s + 1];
+            if (a < 0 || b < a || (int64_t)b > A.rows) {
+                if (u == 0) atomicOr(A.status, LEV_DEV_BAD_INDEX);
+            } else {
+                n = b - a;
+            }
+        }
+        const int units = (n + per - 1) / per;
+        int scan = units;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, scan, o);
+            if (lane >= o) scan += x;
+        }
+        const unsigned has = __ballot_sync(0xffffffffu, before + scan > u);
+        if (has && !found) {
+            const int l = __ffs(has) - 1;
+            const int mine = u - before - (scan - units);   // of lane l: the unit's number inside its sequence
+            U->seq = s0 + l;
+            U->t0 = __shfl_sync(0xffffffffu, (units - 1 - mine) * per, l);
+            U->len = __shfl_sync(0xffffffffu, n, l);
+            U->row0 = __shfl_sync(0xffffffffu, a, l);
+            found = true;
+        }
+        before += __shfl_sync(0xffffffffu, scan, 31);
+    }
+    return found;
+}
+
+// element address of position p of this unit's KV head; NULL for a table entry outside the pool
+__device__ __forceinline__ const unsigned char* tc_row(const TcArgs& A, const TcUnit& U, int kvh, int hd, int p, bool is_v) {
+    const int size = A.kv_type == TC_F32 ? 4 : 2;
+    const unsigned char* base = static_cast<const unsigned char*>(is_v ? A.v : A.k);
+    if (!A.table) return base + ((int64_t)(U.row0 + p) * (is_v ? A.v_ld : A.k_ld) + (int64_t)kvh * hd) * size;
+    const int pg = p / A.page, e = A.table[(int64_t)U.slot * A.max_blocks + pg];
+    if (e < 0 || e >= A.blocks) return nullptr;
+    return base + LEV_KV_ROW(e, p - pg * A.page, kvh, A.page, A.kv_heads) * (int64_t)hd * size;
+}
+__device__ __forceinline__ float tc_value(const unsigned char* row, int i, int kv_type) {
+    if (kv_type == TC_F32) return __half2float(__float2half_rn(reinterpret_cast<const float*>(row)[i]));
+    if (kv_type == TC_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row)[i]);
+    return __half2float(reinterpret_cast<const __half*>(row)[i]);
+}
+// query element as the tensor core sees it
+__device__ __forceinline__ float tc_query(const TcArgs& A, int64_t at) {
+    float x;
+    if (A.q_type == TC_F32) x = __half2float(__float2half_rn(static_cast<const float*>(A.q)[at]));
+    else if (A.q_type == TC_BF16) x = __bfloat162float(static_cast<const __nv_bfloat16*>(A.q)[at]);
+    else x = __half2float(static_cast<const __half*>(A.q)[at]);
+    return A.negate ? -x : x;
+}
+__device__ __forceinline__ void tc_store16(const TcArgs& A, int64_t at, float x) {
+    if (A.out_type == TC_BF16) static_cast<__nv_bfloat16*>(A.out)[at] = __float2bfloat16_rn(x);
+    else static_cast<__half*>(A.out)[at] = __float2half_rn(x);
+}
+
+// One row again, position by position over [lo, hi): for rows whose sums met a non-finite value where they do not attend.
+// 128 threads of the tile's warpgroup; scratch: HD + 128 floats.  Returns thread t's dims t (and t + 128) unnormalised.
+template <int HD>
+__device__ void tc_row_again(const TcArgs& A, const TcUnit& U, int kvh, int64_t q_at, int lo, int hi, int t, int bar, float* scratch,
+                             float* o, float* m_out, float* l_out) {
+    float *qs = scratch, *ws = scratch + HD;
+    wg_sync(bar);
+    for (int i = t; i < HD; i += 128) qs[i] = tc_query(A, q_at + i);
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < HD / 128; i++) o[i] = 0.f;
+    for (int b = lo; b < hi; b += 128) {
+        wg_sync(bar);   // qs is written; the weights of the step before are read
+        float s = -INFINITY;
+        if (b + t < hi) {
+            const unsigned char* row = tc_row(A, U, kvh, HD, b + t, false);
+            s = row ? 0.f : NAN;
+            if (row)
+                for (int i = 0; i < HD; i++) s = fmaf(qs[i], tc_value(row, i, A.kv_type), s);
+        }
+        ws[t] = s;
+        wg_sync(bar);
+        const int n = hi - b < 128 ? hi - b : 128;
+        float m_new = m;
+        for (int j = 0; j < n; j++) m_new = fmaxf(m_new, ws[j]);
+        const float ref = m_new == -INFINITY ? 0.f : m_new, corr = ex2((m - ref) * A.sl);
+        m = m_new;
+        l *= corr;
+#pragma unroll
+        for (int i = 0; i < HD / 128; i++) o[i] *= corr;
+        for (int j = 0; j < n; j++) {
+            const float w = ex2((ws[j] - ref) * A.sl);
+            l += w;
+            const unsigned char* row = tc_row(A, U, kvh, HD, b + j, true);
+#pragma unroll
+            for (int i = 0; i < HD / 128; i++) o[i] = fmaf(w, row ? tc_value(row, t + 128 * i, A.kv_type) : NAN, o[i]);
+        }
+    }
+    *m_out = m;
+    *l_out = l;
+}
+
+template <int HD, int TILES>
+struct TcDims {
+    static constexpr int kWarps = 4 * TILES + 4;
+    static constexpr int kMma = 4 * TILES, kTma = 4 * TILES + 1;   // warps kTma .. kTma + 2 copy rows without boxes
+    static constexpr unsigned kQTile = 128u * HD * 2;
+    static constexpr int kStages = (int)((227u * 1024 - 2048 - TILES * kQTile) / TC_STAGE) < TC_MAX_STAGES
+                                       ? (int)((227u * 1024 - 2048 - TILES * kQTile) / TC_STAGE)
+                                       : TC_MAX_STAGES;
+    static constexpr size_t kSmem = 1024 + TILES * kQTile + (size_t)kStages * TC_STAGE;
+};
+
+// HD: head dimension.  TILES: 128-row tiles of a CTA, each with a softmax warpgroup; one tile has two S buffers, two
+// tiles have one each.  CG = 2: a pair of CTAs (cta_group::2) with one tile each that share K and V.  splits > 1: the
+// CTAs of a cluster take parts of the positions and merge through distributed shared memory.
+template <int HD, int TILES, int CG>
+__global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
+    k_attn_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ TcArgs A) {
+    using D = TcDims<HD, TILES>;
+    constexpr int NS = D::kStages;
+    constexpr int KV_STAGES = CG == 2 ? 1 : HD / 128;   // stages of a K (or V) tile of this CTA
+    constexpr int O_COL = 256;                          // tensor memory: S slots at 0 and 128, then O
+    extern __shared__ unsigned char smem_dyn[];
+    __shared__ __align__(8) unsigned long long full[NS], empty[NS], s_full[2], p_full[2], pv_done[2], q_full;
+    __shared__ unsigned tmem_base_s;
+    __shared__ int abort_s, bad_s;
+    __shared__ __align__(16) float merge_ml[128][2];   // splits: a row's reference and sum
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned rank = CG == 2 ? cluster_rank() : 0u;
+    const int kvh = blockIdx.y;
+    const int split = CG == 2 ? 0 : (int)blockIdx.x % A.splits;
+    const int unit = (int)blockIdx.x / (CG == 2 ? 2 : A.splits);
+    const int per = A.tpt * TILES * CG;
+    pdl_wait();
+    pdl_launch_dependents();
+    TcUnit U;
+    if (!tc_find(A, unit, per, lane, &U)) return;   // the same answer in every CTA of the unit
+    U.ok = 1;
+    U.pos0 = 0;
+    U.slot = 0;
+    if (A.table) {
+        U.slot = A.slot[U.seq];
+        U.pos0 = A.pos[U.seq];
+        U.ok = U.slot >= 0 && U.slot < A.slots && U.pos0 >= 0 && (int64_t)U.pos0 + U.len <= (int64_t)A.max_blocks * A.page;
+    }
+    const int tokens = U.len - U.t0 < per ? U.len - U.t0 : per;   // of the unit
+    if (!U.ok) {   // nothing is followed: the rows are NaN
+        if (threadIdx.x == 0 && rank == 0 && split == 0) atomicOr(A.status, LEV_DEV_BAD_INDEX);
+        if (rank == 0 && split == 0)
+            for (int i = threadIdx.x; i < tokens * A.group * HD; i += blockDim.x) {
+                const int r = i / HD, tok = r / A.group;
+                tc_store16(A, (int64_t)(U.row0 + U.t0 + tok) * A.out_ld + (int64_t)(kvh * A.group + r - tok * A.group) * HD + (i - r * HD), NAN);
+            }
+        return;
+    }
+    // positions of the unit: its first row's lowest to its last row's own
+    const int p_first = U.pos0 + U.t0, p_last = p_first + tokens - 1;
+    const int lo_unit = A.window > 0 && p_first + 1 > A.window ? p_first + 1 - A.window : 0;
+    const int j_all = lo_unit / TC_KV, n_all = p_last / TC_KV - j_all + 1;
+    const int jb = j_all + (int)((int64_t)n_all * split / A.splits), je = j_all + (int)((int64_t)n_all * (split + 1) / A.splits);
+    const int n = je - jb;
+
+    const unsigned smem = (smem_u32(smem_dyn) + 1023u) & ~1023u;
+    const unsigned ring = smem + TILES * D::kQTile;
+    const int tma = A.box_k > 0;
+    if (threadIdx.x == 0) {
+        abort_s = 0;
+        bad_s = 0;
+        for (int s = 0; s < NS; s++) {
+            mbar_init(smem_u32(&full[s]), tma ? 1 : TC_LOAD_WARPS);
+            mbar_init(smem_u32(&empty[s]), 1);
+        }
+        for (int s = 0; s < 2; s++) {
+            mbar_init(smem_u32(&s_full[s]), 1);
+            mbar_init(smem_u32(&p_full[s]), 4 * CG);
+            mbar_init(smem_u32(&pv_done[s]), 1);
+        }
+        mbar_init(smem_u32(&q_full), 4 * TILES * CG);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+    }
+    if (warp == D::kMma) {
+        if (CG == 2) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_base_s)), "r"(512) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_base_s)), "r"(512) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+        }
+    }
+    tc_before();
+    __syncthreads();
+    if (CG == 2) cluster_sync_all();
+    tc_after();
+    const unsigned tmem = tmem_base_s;
+    volatile int* abort_flag = &abort_s;
+
+    if (warp < 4 * TILES) {
+        // ---- softmax: thread = row of the tile ----
+        const int tile = warp >> 2, w4 = warp & 3, t = threadIdx.x & 127;
+        const int tile_tok = (int)(rank * TILES + tile) * A.tpt;   // first token of the tile inside the unit
+        const int tok = t / A.group, head = kvh * A.group + t - tok * A.group;
+        const bool live = tok < A.tpt && tile_tok + tok < tokens;
+        {   // the tile's queries, rounded to 16 bits, in the swizzled K-major layout
+            const unsigned qs = smem + (unsigned)tile * D::kQTile;
+            constexpr int kPieces = HD / 8, kRows = 32 / kPieces < 1 ? 1 : 32 / kPieces;   // 16-byte pieces of a row; rows of a warp's step
+            const int piece = lane % kPieces, sub = lane / kPieces;
+#pragma unroll 4
+            for (int r0 = w4 * 32; r0 < w4 * 32 + 32; r0 += kRows) {
+                const int r = r0 + sub, rt = r / A.group;
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (rt < A.tpt && tile_tok + rt < tokens) {
+                    const int64_t at = (int64_t)(U.row0 + U.t0 + tile_tok + rt) * A.q_ld + (int64_t)(kvh * A.group + r - rt * A.group) * HD + piece * 8;
+                    if (A.q_type == TC_F32) {
+                        const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(A.q) + at);
+                        const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(A.q) + at + 4);
+                        v = make_uint4(pack16(a.x, a.y, TC_F16), pack16(a.z, a.w, TC_F16), pack16(b.x, b.y, TC_F16), pack16(b.z, b.w, TC_F16));
+                    } else {
+                        v = *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(A.q) + at);
+                    }
+                    if (A.negate) v = make_uint4(v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
+                }
+                const unsigned dst = qs + (unsigned)(piece >> 3) * 16384u + (unsigned)r * 128u + (unsigned)(((piece & 7) ^ (r & 7)) << 4);
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                if (CG == 2) mbar_arrive_cluster(map_to_rank(smem_u32(&q_full), 0));
+                else mbar_arrive(smem_u32(&q_full));
+            }
+        }
+        const int p = p_first + tile_tok + tok;                     // this row's position
+        const int row_lo = A.window > 0 ? p + 1 - A.window : 0;     // and its first one (may be negative)
+        const int p_tile0 = p_first + tile_tok, p_tile1 = p_tile0 + A.tpt - 1;   // positions of the tile's rows
+        const unsigned lane_base = tmem + ((unsigned)(w4 * 32) << 16);
+        const unsigned o_addr = lane_base + O_COL + (TILES == 2 ? tile * 128 : 0);
+        float m = -INFINITY;   // reference of the row's weights, in units of S
+        f32x2 sum = two(0.f, 0.f);
+        const f32x2 sl2 = two(A.sl, A.sl);
+        for (int i = 0; i < n; i++) {
+            const int slot_i = TILES == 2 ? tile : i & 1, par = TILES == 2 ? i & 1 : (i >> 1) & 1;
+            const unsigned s_addr = lane_base + (unsigned)slot_i * 128u;
+            pk_wait(smem_u32(&s_full[slot_i]), par, abort_flag);
+            __syncwarp();
+            tc_after();
+            unsigned s[128];
+#pragma unroll
+            for (int c = 0; c < 4; c++) tmem_ld32(s_addr + 32u * c, s + 32 * c);
+            asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+            const int c0 = (jb + i) * TC_KV;
+            if (c0 + TC_KV - 1 > p_tile0 || (A.window > 0 && c0 <= p_tile1 - A.window)) {   // some row does not attend to all of it
+                const int hi = p - c0, lo = row_lo - c0;
+#pragma unroll
+                for (int c = 0; c < 128; c++)
+                    if (c > hi || c < lo) s[c] = 0xFF800000u;
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < 128; c += 8)
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                    mx[q] = fmaxf(mx[q], fmaxf(__uint_as_float(s[c + 2 * q]), __uint_as_float(s[c + 2 * q + 1])));
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            // the reference follows when the maximum has run away from it
+            float corr = 1.f;
+            if (top > m && (i == 0 || m == -INFINITY || (top - m) * A.sl > TC_LAZY)) {
+                corr = ex2((m - top) * A.sl);   // 0 where there was no reference
+                m = top;
+            }
+            if (i > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+                const int prev = TILES == 2 ? tile : (i - 1) & 1, ppar = TILES == 2 ? (i - 1) & 1 : ((i - 1) >> 1) & 1;
+                pk_wait(smem_u32(&pv_done[prev]), ppar, abort_flag);
+                __syncwarp();
+                tc_after();
+                sum = fma_2(sum, two(corr, corr), two(0.f, 0.f));
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 16) {
+                    unsigned o[16];
+                    tmem_ld16(o_addr + c, o);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+#pragma unroll
+                    for (int q = 0; q < 16; q++) o[q] = __float_as_uint(__uint_as_float(o[q]) * corr);
+                    asm volatile(
+                        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n" ::"r"(
+                            o_addr + c),
+                        "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]), "r"(o[8]), "r"(o[9]), "r"(o[10]),
+                        "r"(o[11]), "r"(o[12]), "r"(o[13]), "r"(o[14]), "r"(o[15])
+                        : "memory");
+                }
+            }
+            const float neg = m == -INFINITY ? 0.f : -m * A.sl;
+            const f32x2 neg2 = two(neg, neg);
+            f32x2 part = two(0.f, 0.f);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                unsigned pk[32];
+#pragma unroll
+                for (int c = 0; c < 32; c++) {
+                    float a, b;
+                    both(fma_2(two(__uint_as_float(s[64 * h + 2 * c]), __uint_as_float(s[64 * h + 2 * c + 1])), sl2, neg2), a, b);
+                    a = ex2(a);
+                    b = ex2(b);
+                    const f32x2 e = two(a, b);
+                    if (c & 1) part = add_2(part, e);
+                    else sum = add_2(sum, e);
+                    pk[c] = pack16(a, b, A.mma_type);
+                }
+                tmem_st32(s_addr + 32u * h, pk);
+            }
+            sum = add_2(sum, part);
+            asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+            tc_before();
+            __syncwarp();
+            if (lane == 0) {
+                const unsigned bar = smem_u32(&p_full[slot_i]);
+                if (CG == 2) mbar_arrive_cluster(map_to_rank(bar, 0));
+                else mbar_arrive(bar);
+            }
+        }
+        if (n > 0) {
+            const int last = TILES == 2 ? tile : (n - 1) & 1, lpar = TILES == 2 ? (n - 1) & 1 : ((n - 1) >> 1) & 1;
+            pk_wait(smem_u32(&pv_done[last]), lpar, abort_flag);
+            __syncwarp();
+            tc_after();
+        }
+        float l0, l1;
+        both(sum, l0, l1);
+        float l = l0 + l1;
+        const bool bad = bad_s != 0;   // a table entry outside the pool: the rows are NaN
+        const int64_t out_at = (int64_t)(U.row0 + U.t0 + tile_tok + tok) * A.out_ld + (int64_t)head * HD;
+        const float inv = bad ? NAN : 1.f / l;
+        float probe = 0.f;   // NaN when a sum is not finite
+        float* part_o = reinterpret_cast<float*>(smem_dyn + (smem - smem_u32(smem_dyn)));   // splits: [row][HD], 16-byte pieces swizzled
+        if (n > 0) {
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+                unsigned o[32];
+                tmem_ld32(o_addr + c, o);
+                asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+#pragma unroll
+                for (int q = 0; q < 32; q++) probe = fmaf(__uint_as_float(o[q]), 0.f, probe);
+                if (A.splits > 1) {
+#pragma unroll
+                    for (int q = 0; q < 32; q += 4)
+                        *reinterpret_cast<uint4*>(part_o + t * HD + (((c + q) >> 2 ^ (t & 7)) << 2)) = make_uint4(o[q], o[q + 1], o[q + 2], o[q + 3]);
+                } else if (live) {
+                    unsigned v[16];
+#pragma unroll
+                    for (int q = 0; q < 16; q++) v[q] = pack16(__uint_as_float(o[2 * q]) * inv, __uint_as_float(o[2 * q + 1]) * inv, A.out_type);
+                    uint4* dst = reinterpret_cast<uint4*>(static_cast<unsigned short*>(A.out) + out_at + c);
+#pragma unroll
+                    for (int q = 0; q < 4; q++) dst[q] = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                }
+            }
+        }
+        tc_before();
+        // rows that met a non-finite value where they do not attend (or where they do: the answer is then the same)
+        const unsigned again_warp = __ballot_sync(0xffffffffu, live && n > 0 && !bad && probe != 0.f);
+        unsigned* again_s = reinterpret_cast<unsigned*>(&merge_ml[0][0]) + 4 * tile;   // the statistics are stored behind this
+        if (lane == 0) again_s[w4] = again_warp;
+        wg_sync(1 + tile);
+        unsigned again[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) again[q] = again_s[q];
+        wg_sync(1 + tile);
+        if (again[0] | again[1] | again[2] | again[3]) {
+            float* scratch = reinterpret_cast<float*>(smem_dyn + (smem - smem_u32(smem_dyn)) + (A.splits > 1 ? 128 * HD * 4 : tile * (int)D::kQTile));
+#pragma unroll 1
+            for (int r = 0; r < 128; r++) {
+                if (!((again[r >> 5] >> (r & 31)) & 1u)) continue;
+                const int rt = r / A.group, rp = p_first + tile_tok + rt;
+                const int64_t row = U.row0 + U.t0 + tile_tok + rt, rh = kvh * A.group + r - rt * A.group;
+                int lo = A.window > 0 && rp + 1 > A.window ? rp + 1 - A.window : 0, hi = rp + 1;
+                lo = lo > jb * TC_KV ? lo : jb * TC_KV;
+                hi = hi < je * TC_KV ? hi : je * TC_KV;
+                float o[HD / 128], m2, l2;
+                tc_row_again<HD>(A, U, kvh, row * A.q_ld + rh * HD, lo, hi, t, 1 + tile, scratch, o, &m2, &l2);
+#pragma unroll
+                for (int q = 0; q < HD / 128; q++) {
+                    const int d = t + 128 * q;
+                    if (A.splits > 1) part_o[r * HD + ((((d >> 2) ^ (r & 7)) << 2) | (d & 3))] = o[q];
+                    else tc_store16(A, row * A.out_ld + rh * HD + d, o[q] / l2);
+                }
+                if (t == r) {
+                    m = m2;
+                    l = l2;
+                }
+            }
+        }
+        if (A.splits > 1) {
+            merge_ml[t][0] = bad ? 0.f : m;
+            merge_ml[t][1] = bad ? NAN : l;
+        }
+    } else if (warp == D::kMma) {
+        // ---- MMA issue (of a pair: the leader): the whole warp walks the loop, one elected lane issues ----
+        if (rank == 0) {
+            const unsigned elected = elect_lane();
+            const unsigned fmt = A.mma_type == TC_BF16 ? (1u << 7) | (1u << 10) : 0u;
+            const unsigned m_field = (unsigned)((128 * CG) >> 4) << 24;
+            const unsigned id_qk = (1u << 4) | fmt | ((128u >> 3) << 17) | m_field;
+            const unsigned id_pv = (1u << 4) | fmt | (1u << 16) | ((unsigned)((CG == 2 ? HD : 128) >> 3) << 17) | m_field;   // B is N-major
+            constexpr unsigned kKSlab = 128u / CG * 128u;   // bytes of 64 columns of this CTA's rows of K
+            Ring kr(NS), vr(NS);   // stages of the next K and of the next V tile
+            auto qk = [&](int tile, int slot_i, bool release) {   // S[slot] = Q[tile] K^T
+                Ring st = kr;
+#pragma unroll
+                for (int h = 0; h < KV_STAGES; h++) {
+                    pk_wait(smem_u32(&full[st.s]), st.ph, abort_flag);
+                    tc_after();
+                    const unsigned kb = ring + (unsigned)st.s * TC_STAGE;
+                    constexpr int kSlabs = HD / 64 / KV_STAGES;
+#pragma unroll
+                    for (int b = 0; b < kSlabs; b++)
+                        pk_mma4<CG>(tmem + (unsigned)slot_i * 128u, pk_desc_lo(smem + (unsigned)tile * D::kQTile + (unsigned)(h * kSlabs + b) * 16384u),
+                                    pk_desc_lo(kb + (unsigned)b * kKSlab), id_qk, (h | b) ? 1u : 0u, elected);
+                    if (release) pk_commit<CG>(smem_u32(&empty[st.s]), elected);
+                    st.step(1);
+                }
+                pk_commit<CG>(smem_u32(&s_full[slot_i]), elected);
+            };
+            auto pv = [&](int tile, int slot_i, bool first, bool release) {   // O[tile] += P[slot] V
+                Ring st = vr;
+#pragma unroll
+                for (int h = 0; h < KV_STAGES; h++) {
+                    pk_wait(smem_u32(&full[st.s]), st.ph, abort_flag);
+                    tc_after();
+                    const unsigned vb = ring + (unsigned)st.s * TC_STAGE;
+                    const unsigned b_lo = ((vb >> 4) & 0x3FFFu) | ((16384u >> 4) << 16);
+                    tc_pv<CG>(tmem + O_COL + (TILES == 2 ? tile * 128u : h * 128u), tmem + (unsigned)slot_i * 128u, b_lo, id_pv, first ? 0u : 1u, elected);
+                    if (release) pk_commit<CG>(smem_u32(&empty[st.s]), elected);
+                    st.step(1);
+                }
+                pk_commit<CG>(smem_u32(&pv_done[slot_i]), elected);
+            };
+            pk_wait(smem_u32(&q_full), 0, abort_flag);
+            tc_after();
+            if (TILES == 2) {
+                // stages: K0 V0 K1 V1 ...
+                vr.step(1);
+                if (n > 0) {
+                    qk(0, 0, false);
+                    qk(1, 1, true);
+                    kr.step(2);
+                }
+                for (int i = 0; i < n; i++) {
+#pragma unroll
+                    for (int tile = 0; tile < 2; tile++) {
+                        pk_wait(smem_u32(&p_full[tile]), i & 1, abort_flag);
+                        tc_after();
+                        pv(tile, tile, i == 0, tile == 1);
+                        if (i + 1 < n) qk(tile, tile, tile == 1);
+                    }
+                    kr.step(2);
+                    vr.step(2);
+                }
+            } else {
+                // stages: K0 K1 V0 K2 V1 ... (each KV_STAGES long)
+                Ring st(NS);
+                if (n > 0) {
+                    kr = st;
+                    qk(0, 0, true);
+                    st.step(KV_STAGES);
+                }
+                for (int i = 0; i < n; i++) {
+                    if (i + 1 < n) {
+                        kr = st;
+                        qk(0, (i + 1) & 1, true);
+                        st.step(KV_STAGES);
+                    }
+                    pk_wait(smem_u32(&p_full[i & 1]), (i >> 1) & 1, abort_flag);
+                    tc_after();
+                    vr = st;
+                    pv(0, i & 1, i == 0, true);
+                    st.step(KV_STAGES);
+                }
+            }
+        }
+    } else if (tma) {
+        // ---- TMA boxes, in the order in which the MMA warp takes the stages ----
+        if (warp == D::kTma) {
+            const unsigned elected = elect_lane();
+            const unsigned full_c = CG == 2 ? map_to_rank(smem_u32(&full[0]), 0) : smem_u32(&full[0]);
+            const int32_t* trow = A.table ? A.table + (int64_t)U.slot * A.max_blocks : nullptr;
+            const int page_lo = A.table ? lo_unit / A.page : 0, page_hi = A.table ? p_last / A.page : 0;
+            Ring st(NS);
+            auto load = [&](int i, bool is_v) {
+                const CUtensorMap* map = is_v ? &vmap : &kmap;
+                const int c0 = (jb + i) * TC_KV;
+                const int r_first = CG == 2 && !is_v ? (int)rank * 64 : 0, r_n = CG == 2 && !is_v ? 64 : 128;   // rows of this CTA
+                const unsigned slab = (unsigned)r_n * 128u;
+                constexpr int kSlabsV = 2, kSlabsK = CG == 2 ? HD / 64 : 2;
+                int entry = 0;
+                const int box = is_v ? A.box_v : A.box_k;
+                if (trow) {   // lane l: the table entry of box l; pages that no row attends to are filled with zeros, not read
+                    const int pg = (c0 + r_first + lane * box) / A.page;
+                    entry = (int)A.blocks;
+                    if (lane * box < r_n && pg >= page_lo && pg <= page_hi) {
+                        entry = trow[pg];
+                        if (entry < 0 || entry >= A.blocks) {
+                            atomicOr(A.status, LEV_DEV_BAD_INDEX);
+                            bad_s = 1;
+                            entry = (int)A.blocks;
+                        }
+                    }
+                    __syncwarp();
+                }
+#pragma unroll
+                for (int h = 0; h < KV_STAGES; h++) {
+                    pk_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
+                    const unsigned bar = full_c + 8u * (unsigned)st.s, dst = ring + (unsigned)st.s * TC_STAGE;
+                    if (rank == 0) pk_expect(smem_u32(&full[st.s]), TC_STAGE * CG, elected);
+                    const int x0 = CG == 2 ? (is_v ? (int)rank * 128 : 0) : h * 128;
+                    for (int r = 0; r < r_n; r += box) {
+                        const int e = trow ? __shfl_sync(0xffffffffu, entry, r / box) : 0;
+                        const int at = c0 + r_first + r;
+#pragma unroll
+                        for (int b = 0; b < (is_v ? kSlabsV : kSlabsK); b++) {
+                            const unsigned to = dst + (unsigned)b * slab + (unsigned)r * 128u;
+                            if (trow) tc_box<CG, 4>(to, map, x0 + 64 * b, kvh, at % A.page, e, bar, elected);
+                            else tc_box<CG, 3>(to, map, x0 + 64 * b, kvh, U.row0 + at, 0, bar, elected);
+                        }
+                    }
+                    st.step(1);
+                }
+            };
+            if (TILES == 2) {
+                for (int i = 0; i < n; i++) {
+                    load(i, false);
+                    load(i, true);
+                }
+            } else {
+                for (int i = 0; i <= n; i++) {
+                    if (i < n) load(i, false);
+                    if (i > 0) load(i - 1, true);
+                }
+            }
+            for (int s = 0; s < NS; s++) {   // the tensor core's last releases have arrived
+                pk_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
+                st.step(1);
+            }
+        }
+    } else {
+        // ---- rows copied (and converted) by warps: pages of any size, f32 pools ----
+        const int w = warp - D::kTma;
+        Ring st(NS);
+        auto load = [&](int i, bool is_v) {
+            const int c0 = (jb + i) * TC_KV;
+            for (int h = 0; h < KV_STAGES; h++) {
+                pk_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
+                const unsigned dst = ring + (unsigned)st.s * TC_STAGE;
+                // two rows of 16 pieces (8 values each) per step of a warp
+                const int piece = lane & 15, sub = lane >> 4;
+                for (int r0 = 2 * w; r0 < 128; r0 += 2 * TC_LOAD_WARPS * 4) {
+                    uint4 v[4];
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const int r = r0 + q * 2 * TC_LOAD_WARPS + sub, at = c0 + r;
+                        v[q] = make_uint4(0u, 0u, 0u, 0u);
+                        if (r < 128 && at >= lo_unit && at <= p_last) {
+                            const unsigned char* src = tc_row(A, U, kvh, HD, at, is_v);
+                            if (!src) {
+                                atomicOr(A.status, LEV_DEV_BAD_INDEX);
+                                bad_s = 1;
+                            } else if (A.kv_type == TC_F32) {
+                                const float4* f = reinterpret_cast<const float4*>(src) + (h * 16 + piece) * 2;
+                                const float4 a = f[0], b = f[1];
+                                v[q] = make_uint4(pack16(a.x, a.y, TC_F16), pack16(a.z, a.w, TC_F16), pack16(b.x, b.y, TC_F16), pack16(b.z, b.w, TC_F16));
+                            } else {
+                                v[q] = *(reinterpret_cast<const uint4*>(src) + h * 16 + piece);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const int r = r0 + q * 2 * TC_LOAD_WARPS + sub;
+                        if (r < 128)
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst + (unsigned)(piece >> 3) * 16384u + (unsigned)r * 128u +
+                                                                                            (unsigned)(((piece & 7) ^ (r & 7)) << 4)),
+                                         "r"(v[q].x), "r"(v[q].y), "r"(v[q].z), "r"(v[q].w)
+                                         : "memory");
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&full[st.s]));
+                st.step(1);
+            }
+        };
+        if (TILES == 2) {
+            for (int i = 0; i < n; i++) {
+                load(i, false);
+                load(i, true);
+            }
+        } else {
+            for (int i = 0; i <= n; i++) {
+                if (i < n) load(i, false);
+                if (i > 0) load(i - 1, true);
+            }
+        }
+        for (int s = 0; s < NS; s++) {
+            pk_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
+            st.step(1);
+        }
+    }
+    pk_finish(abort_flag, A.status, LEV_DEV_TIMEOUT);
+    if (CG == 1 && A.splits > 1) {
+        // ---- merge: CTA z of the cluster adds its share of the rows, the parts in order ----
+        cluster_sync_all();
+        const int used = tokens * A.group, Z = A.splits;
+        const int ra = used * split / Z, rb = used * (split + 1) / Z;
+        const unsigned ml = smem_u32(&merge_ml[0][0]);
+        constexpr int kQuads = HD / 4;
+        for (int item = ra * kQuads + threadIdx.x; item < rb * kQuads; item += blockDim.x) {
+            const int r = item / kQuads, qd = item - r * kQuads;
+            float mm = -INFINITY;
+            for (int z = 0; z < Z; z++) {
+                float mz;
+                asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(mz) : "r"(map_to_rank(ml + 8u * r, z)) : "memory");
+                mm = fmaxf(mm, mz);
+            }
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+            float l = 0.f;
+            for (int z = 0; z < Z; z++) {
+                float mz, lz;
+                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];\n" : "=f"(mz), "=f"(lz) : "r"(map_to_rank(ml + 8u * r, z)) : "memory");
+                if (mz == -INFINITY && lz == 0.f) continue;   // this part attends to nothing
+                const float w = ex2((mz - mm) * A.sl);
+                float4 o;
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n"
+                             : "=f"(o.x), "=f"(o.y), "=f"(o.z), "=f"(o.w)
+                             : "r"(map_to_rank(smem + (unsigned)(r * HD + ((qd ^ (r & 7)) << 2)) * 4u, z))
+                             : "memory");
+                l = fmaf(lz, w, l);
+                a.x = fmaf(o.x, w, a.x);
+                a.y = fmaf(o.y, w, a.y);
+                a.z = fmaf(o.z, w, a.z);
+                a.w = fmaf(o.w, w, a.w);
+            }
+            const float inv = 1.f / l;
+            const int tok = r / A.group;
+            unsigned short* dst = static_cast<unsigned short*>(A.out) + (int64_t)(U.row0 + U.t0 + tok) * A.out_ld + (int64_t)(kvh * A.group + r - tok * A.group) * HD + 4 * qd;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack16(a.x * inv, a.y * inv, A.out_type), pack16(a.z * inv, a.w * inv, A.out_type));
+        }
+        cluster_sync_all();   // a CTA's shared memory stays until its peers have read it
+    }
+    if (CG == 2) cluster_sync_all();
+    tc_after();
+    if (warp == D::kMma) {
+        if (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// ---- host side ----
+
+struct TcPlan {
+    int tiles, cg, splits;
+    int64_t units;
+};
+
+// What a call's launch looks like, from what the host knows: rows and sequences (the lengths are on the device) and the
+// most positions that a row can attend to.
+TcPlan tc_plan(const lev_ctx* ctx, int64_t rows, int seqs, int kv_heads, int tpt, int hd, int64_t span, bool boxes) {
+    TcPlan P = {1, 1, 1, 0};
+    const int64_t mean = (rows + seqs - 1) / seqs, sms = ctx->prop.multiProcessorCount;
+    const int64_t tiles = (mean + tpt - 1) / tpt * seqs * kv_heads;   // 128-row tiles, about
+    if (2 * tiles <= sms) {
+        // few tiles: the CTAs of a cluster share the positions of one
+        while (P.splits < 16 && 2 * P.splits * tiles <= sms && 2 * P.splits * TC_KV <= span) P.splits *= 2;
+    } else if (mean > tpt) {
+        if (hd == 128) P.tiles = 2;
+        else if (boxes) P.cg = 2;
+    }
+    const int64_t per = (int64_t)tpt * P.tiles * P.cg;
+    P.units = rows / per + seqs < rows ? rows / per + seqs : rows;
+    return P;
+}
+
+template <int HD, int TILES, int CG>
+int tc_launch(lev_ctx* ctx, const CUtensorMap& kmap, const CUtensorMap& vmap, const TcArgs& A, int64_t units) {
+    using D = TcDims<HD, TILES>;
+    static bool configured[16] = {};
+    if (!configured[ctx->device & 15]) {
+        LEV_CUDA(ctx, cudaFuncSetAttribute(k_attn_tc<HD, TILES, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)D::kSmem));
+        if (TILES == 1 && CG == 1) LEV_CUDA(ctx, cudaFuncSetAttribute(k_attn_tc<HD, TILES, CG>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        configured[ctx->device & 15] = true;
+    }
+    const int cluster = CG == 2 ? 2 : A.splits;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(units * cluster), (unsigned)A.kv_heads);
+    cfg.blockDim = dim3(D::kWarps * 32);
+    cfg.dynamicSmemBytes = D::kSmem;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    LEV_CUDA(ctx, cudaLaunchKernelEx(&cfg, k_attn_tc<HD, TILES, CG>, kmap, vmap, A));
+    ctx->launches++;
+    return lev_cuda_check(ctx, cudaGetLastError(), "k_attn_tc");
+}
+
+int tc_run(lev_ctx* ctx, const CUtensorMap& kmap, const CUtensorMap& vmap, const TcArgs& A, const TcPlan& P, int hd) {
+    if (hd == 256) return P.cg == 2 ? tc_launch<256, 1, 2>(ctx, kmap, vmap, A, P.units) : tc_launch<256, 1, 1>(ctx, kmap, vmap, A, P.units);
+    return P.tiles == 2 ? tc_launch<128, 2, 1>(ctx, kmap, vmap, A, P.units) : tc_launch<128, 1, 1>(ctx, kmap, vmap, A, P.units);
+}
+
+bool ranges_meet(const void* a, int64_t an, const void* b, int64_t bn) {
+    return (const char*)a < (const char*)b + bn && (const char*)b < (const char*)a + an;
+}
+
+// what both entry points check
+int tc_check(lev_ctx* ctx, int n_seqs, int64_t n_rows, int q_heads, int kv_heads, int head_dim, const void* q, int q_type, int64_t q_ld,
+             const void* out, int64_t out_ld, int window, float scale) {
+    if (head_dim != 128 && head_dim != 256) return lev_fail(ctx, LEV_UNSUPPORTED, "head dimension %d (128 or 256)", head_dim);
+    if (n_seqs < 1 || n_seqs > 65535 || n_rows < 1 || n_rows > (1 << 30))
+        return lev_fail(ctx, LEV_BAD_DIMENSIONS, "%lld rows of %d sequences", (long long)n_rows, n_seqs);
+    if (kv_heads < 1 || kv_heads > 1024 || q_heads < 1 || q_heads % kv_heads != 0)
+        return lev_fail(ctx, LEV_BAD_DIMENSIONS, "%d query heads over %d KV heads", q_heads, kv_heads);
+    if (q_heads / kv_heads > 16) return lev_fail(ctx, LEV_UNSUPPORTED, "%d query heads per KV head (at most 16)", q_heads / kv_heads);
+    if (window < 0 || !isfinite(scale)) return lev_fail(ctx, LEV_BAD_ARGUMENT, "window %d, scale %g", window, (double)scale);
+    const int64_t least = (int64_t)q_heads * head_dim;
+    const int q_size = q_type == LEV_ELEM_F32 ? 4 : 2;
+    if (q_ld < least || out_ld < least || q_ld * q_size % 16 != 0 || out_ld % 8 != 0 || q_ld > (int64_t)1 << 31 || out_ld > (int64_t)1 << 31)
+        return lev_fail(ctx, LEV_BAD_ARGUMENT, "query rows %lld and output rows %lld elements apart (at least %lld, whole 16-byte steps)", (long long)q_ld,
+                        (long long)out_ld, (long long)least);
+    if ((((uintptr_t)q | (uintptr_t)out) & 15) != 0) return lev_fail(ctx, LEV_BAD_ARGUMENT, "queries or output are not 16-byte aligned");
+    if (ranges_meet(q, ((n_rows - 1) * q_ld + least) * q_size, out, ((n_rows - 1) * out_ld + least) * 2))
+        return lev_fail(ctx, LEV_BAD_ARGUMENT, "the output overlaps the queries");
+    return LEV_OK;
+}
+
+TcArgs tc_args(lev_ctx* ctx, int n_seqs, const int32_t* start, int64_t n_rows, int q_heads, int kv_heads, const void* q, int q_type, int64_t q_ld,
+               int window, float scale, void* out, int out_type, int64_t out_ld) {
+    TcArgs A = {};
+    A.q = q;
+    A.q_type = q_type;
+    A.q_ld = q_ld;
+    A.out = out;
+    A.out_type = out_type;
+    A.out_ld = out_ld;
+    A.start = start;
+    A.rows = n_rows;
+    A.seqs = n_seqs;
+    A.q_heads = q_heads;
+    A.kv_heads = kv_heads;
+    A.group = q_heads / kv_heads;
+    A.tpt = 128 / A.group;
+    A.window = window;
+    A.negate = scale < 0.f;   // maxima are taken of S: a negative scale goes into the queries
+    A.sl = (scale == 0.f ? 1e-30f : fabsf(scale)) * 1.4426950408889634f;   // a scale of zero: the same weights, and a replaced score stays -inf
+    A.status = ctx->d_status;
+    return A;
+}
+
+}  // namespace
+
+extern "C" int lev_attn_chunk(lev_ctx* ctx, const lev_kv_layout* L, const void* k_pool, const void* v_pool, const int32_t* block_table, int n_chunks,
+                              const int32_t* start, const int32_t* slot, const int32_t* pos, int64_t n_rows, int q_heads, const void* q, int q_type,
+                              int64_t q_ld, int window, float scale, void* out, int out_type, int64_t out_ld) {
+    if (!ctx || !k_pool || !v_pool || !block_table || !start || !slot || !pos || !q || !out) return LEV_BAD_ARGUMENT;
+    LEV_TRY(lev_check_kv_layout(ctx, L));
+    if (q_type != LEV_ELEM_F32 && q_type != LEV_ELEM_F16) return lev_fail(ctx, LEV_UNSUPPORTED, "query element type %d (f32 or f16)", q_type);
+    if (out_type != LEV_ELEM_F16 && out_type != LEV_ELEM_BF16) return lev_fail(ctx, LEV_UNSUPPORTED, "output element type %d (f16 or bf16)", out_type);
+    LEV_TRY(tc_check(ctx, n_chunks, n_rows, q_heads, L->kv_heads, L->head_dim, q, q_type, q_ld, out, out_ld, window, scale));
+    if ((((uintptr_t)k_pool | (uintptr_t)v_pool) & 15) != 0) return lev_fail(ctx, LEV_BAD_ARGUMENT, "cache pools are not 16-byte aligned");
+    EncodeTiledFn enc = encode_tiled();
+    if (!enc) return lev_fail(ctx, LEV_UNSUPPORTED, "cuTensorMapEncodeTiled is not available");
+    LEV_CUDA(ctx, cudaSetDevice(ctx->device));
+    TcArgs A = tc_args(ctx, n_chunks, start, n_rows, q_heads, L->kv_heads, q, q_type, q_ld, window, scale, out, out_type, out_ld);
+    const int hd = L->head_dim;
+    A.mma_type = TC_F16;
+    A.kv_type = L->kv_type == LEV_KV_F32 ? TC_F32 : TC_F16;
+    A.slot = slot;
+    A.pos = pos;
+    A.table = block_table;
+    A.k = k_pool;
+    A.v = v_pool;
+    A.blocks = L->blocks;
+    A.page = L->page;
+    A.max_blocks = L->max_blocks;
+    A.slots = L->slots;
+    // pages that make up whole steps of 128 positions out of whole swizzle atoms go by TMA, others are copied by warps
+    const bool boxes = A.kv_type == TC_F16 && L->page % 8 == 0 && (TC_KV % L->page == 0 || L->page % TC_KV == 0) && L->blocks < (1ll << 31);
+    const int64_t cap = (int64_t)L->max_blocks * L->page, span = window > 0 && window < cap ? window : cap;
+    const TcPlan P = tc_plan(ctx, n_rows, n_chunks, L->kv_heads, A.tpt, hd, span, boxes);
+    A.splits = P.splits;
+    CUtensorMap kmap = {}, vmap = {};
+    if (boxes) {
+        const int box_v = L->page < TC_KV ? L->page : TC_KV, box_k = box_v > TC_KV / P.cg ? TC_KV / P.cg : box_v;
+        const cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)L->kv_heads, (cuuint64_t)L->page, (cuuint64_t)L->blocks};
+        const cuuint64_t strides[3] = {(cuuint64_t)(LEV_KV_ROW(0, 0, 1, L->page, L->kv_heads) * hd * 2), (cuuint64_t)(LEV_KV_ROW(0, 1, 0, L->page, L->kv_heads) * hd * 2),
+                                       (cuuint64_t)L->kv_heads * L->page * hd * 2};
+        const cuuint32_t one[4] = {1, 1, 1, 1};
+        for (int i = 0; i < 2; i++) {
+            const cuuint32_t box[4] = {64, 1, (cuuint32_t)(i ? box_v : box_k), 1};
+            const CUresult cr = enc(i ? &vmap : &kmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(i ? v_pool : k_pool), dims, strides, box, one,
+                                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+            if (cr != CUDA_SUCCESS) return lev_fail(ctx, LEV_KERNEL_FAILED, "cuTensorMapEncodeTiled failed (%d)", (int)cr);
+        }
+        A.box_k = box_k;
+        A.box_v = box_v;
+    }
+    return tc_run(ctx, kmap, vmap, A, P, hd);
+}
+
+extern "C" int lev_attn_prompt(lev_ctx* ctx, int n_seqs, const int32_t* start, int64_t n_rows, int q_heads, int kv_heads, int head_dim, int type,
+                               const void* q, int64_t q_ld, const void* k, int64_t k_ld, const void* v, int64_t v_ld, int window, float scale,
+                               void* out, int64_t out_ld) {
+    if (!ctx || !start || !q || !k || !v || !out) return LEV_BAD_ARGUMENT;
+    if (type != LEV_ELEM_F16 && type != LEV_ELEM_BF16) return lev_fail(ctx, LEV_UNSUPPORTED, "element type %d (f16 or bf16)", type);
+    LEV_TRY(tc_check(ctx, n_seqs, n_rows, q_heads, kv_heads, head_dim, q, type, q_ld, out, out_ld, window, scale));
+    const int64_t least = (int64_t)kv_heads * head_dim;
+    if (k_ld < least || v_ld < least || k_ld % 8 != 0 || v_ld % 8 != 0 || k_ld > (int64_t)1 << 31 || v_ld > (int64_t)1 << 31 ||
+        (((uintptr_t)k | (uintptr_t)v) & 15) != 0)
+        return lev_fail(ctx, LEV_BAD_ARGUMENT, "key rows %lld and value rows %lld elements apart (at least %lld, whole 16-byte steps, 16-byte aligned)",
+                        (long long)k_ld, (long long)v_ld, (long long)least);
+    const int64_t out_bytes = ((n_rows - 1) * out_ld + (int64_t)q_heads * head_dim) * 2;
+    if (ranges_meet(k, ((n_rows - 1) * k_ld + least) * 2, out, out_bytes) || ranges_meet(v, ((n_rows - 1) * v_ld + least) * 2, out, out_bytes))
+        return lev_fail(ctx, LEV_BAD_ARGUMENT, "the output overlaps the keys or values");
+    EncodeTiledFn enc = encode_tiled();
+    if (!enc) return lev_fail(ctx, LEV_UNSUPPORTED, "cuTensorMapEncodeTiled is not available");
+    LEV_CUDA(ctx, cudaSetDevice(ctx->device));
+    TcArgs A = tc_args(ctx, n_seqs, start, n_rows, q_heads, kv_heads, q, type, q_ld, window, scale, out, type, out_ld);
+    A.mma_type = A.kv_type = type;
+    A.k = k;
+    A.v = v;
+    A.k_ld = k_ld;
+    A.v_ld = v_ld;
+    const int64_t span = window > 0 && window < n_rows ? window : n_rows;
+    const TcPlan P = tc_plan(ctx, n_rows, n_seqs, kv_heads, A.tpt, head_dim, span, true);
+    A.splits = P.splits;
+    A.box_v = TC_KV;
+    A.box_k = TC_KV / P.cg;
+    CUtensorMap kmap, vmap;
+    const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)kv_heads, (cuuint64_t)n_rows};
+    const cuuint32_t one[3] = {1, 1, 1};
+    for (int i = 0; i < 2; i++) {
+        const cuuint64_t strides[2] = {(cuuint64_t)head_dim * 2, (cuuint64_t)(i ? v_ld : k_ld) * 2};
+        const cuuint32_t box[3] = {64, 1, (cuuint32_t)(i ? A.box_v : A.box_k)};
+        const CUresult cr = enc(i ? &vmap : &kmap, type == LEV_ELEM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                                const_cast<void*>(i ? v : k), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (cr != CUDA_SUCCESS) return lev_fail(ctx, LEV_KERNEL_FAILED, "cuTensorMapEncodeTiled failed (%d)", (int)cr);
+    }
+    return tc_run(ctx, kmap, vmap, A, P, head_dim);
+}

@@ -138,6 +138,7 @@ int lev_read_status(lev_ctx* ctx, int* bits);
     } while (0)
 
 // ---- launchers implemented in the kernel translation units ----
+int lev_check_kv_layout(lev_ctx* ctx, const lev_kv_layout* L);   // lev_attn.cu
 int lev_launch_scale_check(lev_ctx* ctx, const lev_weights* w);
 int lev_launch_finite_check(lev_ctx* ctx, const float* v, int64_t n, int bit);
 int lev_launch_dequantize(lev_ctx* ctx, const lev_weights* w, int64_t row0, int64_t rows, float* out);

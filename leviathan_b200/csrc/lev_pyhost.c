@@ -64,10 +64,20 @@ HOST_FN(kv_append, 10, lev_ctx* c = P(a[0]); lev_kv_layout* l = P(a[1]); void* k
 HOST_FN(attn_decode, 13, lev_ctx* c = P(a[0]); lev_kv_layout* l = P(a[1]); void* kp = P(a[2]); void* vp = P(a[3]); int32_t* tb = P(a[4]);
         int32_t* s = P(a[5]); int32_t* p = P(a[6]); long long nc = I(a[7]); long long qh = I(a[8]); float* q = P(a[9]); long long win = I(a[10]);
         float sc = F(a[11]); float* y = P(a[12]), lev_attn_decode(c, l, kp, vp, tb, s, p, (int)nc, (int)qh, q, (int)win, sc, y))
+HOST_FN(attn_chunk, 19, lev_ctx* c = P(a[0]); lev_kv_layout* l = P(a[1]); void* kp = P(a[2]); void* vp = P(a[3]); int32_t* tb = P(a[4]);
+        long long nc = I(a[5]); int32_t* st0 = P(a[6]); int32_t* s = P(a[7]); int32_t* p = P(a[8]); long long rows = I(a[9]); long long qh = I(a[10]);
+        void* q = P(a[11]); long long qt = I(a[12]); long long ql = I(a[13]); long long win = I(a[14]); float sc = F(a[15]); void* y = P(a[16]);
+        long long yt = I(a[17]); long long yl = I(a[18]),
+        lev_attn_chunk(c, l, kp, vp, tb, (int)nc, st0, s, p, rows, (int)qh, q, (int)qt, ql, (int)win, sc, y, (int)yt, yl))
+HOST_FN(attn_prompt, 18, lev_ctx* c = P(a[0]); long long nc = I(a[1]); int32_t* st0 = P(a[2]); long long rows = I(a[3]); long long qh = I(a[4]);
+        long long kh = I(a[5]); long long hd = I(a[6]); long long ty = I(a[7]); void* q = P(a[8]); long long ql = I(a[9]); void* k = P(a[10]);
+        long long kl = I(a[11]); void* v = P(a[12]); long long vl = I(a[13]); long long win = I(a[14]); float sc = F(a[15]); void* y = P(a[16]);
+        long long yl = I(a[17]),
+        lev_attn_prompt(c, (int)nc, st0, rows, (int)qh, (int)kh, (int)hd, (int)ty, q, ql, k, kl, v, vl, (int)win, sc, y, yl))
 
 #define ENTRY(NAME) {#NAME, (PyCFunction)(void (*)(void))NAME, METH_FASTCALL, NULL}
 static PyMethodDef methods[] = {ENTRY(matvec), ENTRY(matvec_fused), ENTRY(matvec_chain), ENTRY(rmsnorm), ENTRY(axpy),
                                 ENTRY(act_bf16), ENTRY(gemm_prefill), ENTRY(moe_layer), ENTRY(moe_layer_residual), ENTRY(kv_append),
-                                ENTRY(attn_decode), {NULL, NULL, 0, NULL}};
+                                ENTRY(attn_decode), ENTRY(attn_chunk), ENTRY(attn_prompt), {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pyhost", NULL, -1, methods, NULL, NULL, NULL, NULL};
 PyMODINIT_FUNC PyInit__pyhost(void) { return PyModule_Create(&module); }

@@ -100,12 +100,35 @@ __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::befor
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void wg_sync(int id) { asm volatile("bar.sync %0, 128;\n" ::"r"(id) : "memory"); }
 
-// O[128 x N] += P[128 x 128] V[128 x N]: P from tensor memory (64 columns of packed pairs), V N-major in shared memory
-// (slabs of 64 dims, 128-byte rows of one position each).  Eight MMAs of 16 positions: P steps by 8 columns, V by 2 KB.
-// Descriptor low word: address, distance between slabs; high word: 8 positions = 1024 bytes, version, 128-byte swizzle.
+// How the 16-bit rows of a stage lie in shared memory: eight rows of 64 columns make a 1024-byte swizzle atom; `group` bytes
+// lie between atoms of consecutive rows and `slab` bytes between atoms of consecutive columns.
+struct TcLayout {
+    unsigned group, slab;
+    __device__ __forceinline__ unsigned hi() const { return (group >> 4) | (1u << 14) | (2u << 29); }   // stride, version, swizzle
+};
+// S[128 x 128] (+)= Q[128 x 64] K[128 x 64]^T, both K-major: four MMAs of 16 columns (32 bytes)
 template <int CG>
-__device__ __forceinline__ void tc_pv(unsigned d, unsigned p, unsigned b_lo, unsigned idesc, unsigned acc, unsigned elected) {
-    constexpr unsigned kDescHi = (unsigned)((1024 >> 4) | (1u << 14) | (2u << 29));
+__device__ __forceinline__ void tc_qk(unsigned d, unsigned a_lo, unsigned b_lo, unsigned b_hi, unsigned idesc, unsigned acc, unsigned elected) {
+    constexpr unsigned kQHi = (unsigned)((1024 >> 4) | (1u << 14) | (2u << 29));
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+#define LEV_QK(GROUP)                                                                                          \
+    asm volatile(                                                                                              \
+        "{\n .reg .pred p, q;\n .reg .b64 da, db;\n setp.ne.b32 p, %6, 0;\n setp.ne.b32 q, %7, 0;\n"           \
+        " mov.b64 da, {%1, %3};\n mov.b64 db, {%2, %4};\n"                                                     \
+        " @q tcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], da, db, %5, p;\n}\n" ::"r"(d),                   \
+        "r"(a_lo + 2u * i), "r"(b_lo + 2u * i), "r"(kQHi), "r"(b_hi), "r"(idesc), "r"(i ? 1u : acc), "r"(elected) \
+        : "memory")
+        if (CG == 2) LEV_QK("2");
+        else LEV_QK("1");
+#undef LEV_QK
+    }
+}
+// O[128 x N] += P[128 x 128] V[128 x N]: P from tensor memory (64 columns of packed pairs), V N-major in shared memory.
+// Eight MMAs of 16 positions: P steps by 8 columns, V by two atoms of rows.  The descriptor's low word holds the address
+// and the distance between slabs.
+template <int CG>
+__device__ __forceinline__ void tc_pv(unsigned d, unsigned p, unsigned b_lo, unsigned b_hi, unsigned step, unsigned idesc, unsigned acc, unsigned elected) {
 #pragma unroll
     for (int i = 0; i < 8; i++) {
 #define LEV_PV(GROUP)                                                                                          \
@@ -113,32 +136,36 @@ __device__ __forceinline__ void tc_pv(unsigned d, unsigned p, unsigned b_lo, uns
         "{\n .reg .pred p, q;\n .reg .b64 db;\n setp.ne.b32 p, %5, 0;\n setp.ne.b32 q, %6, 0;\n"               \
         " mov.b64 db, {%2, %4};\n"                                                                             \
         " @q tcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d),                 \
-        "r"(p + 8u * i), "r"(b_lo + 128u * i), "r"(idesc), "r"(kDescHi), "r"(i ? 1u : acc), "r"(elected)       \
+        "r"(p + 8u * i), "r"(b_lo + step * i), "r"(idesc), "r"(b_hi), "r"(i ? 1u : acc), "r"(elected)          \
         : "memory")
         if (CG == 2) LEV_PV("2");
         else LEV_PV("1");
 #undef LEV_PV
     }
 }
-// one box of a cache page (column, head, row of the page, block) or of packed rows (column, head, row)
-template <int CG, int DIMS>
-__device__ __forceinline__ void tc_box(unsigned dst, const CUtensorMap* map, int x, int h, int r, int b, unsigned bar, unsigned elected) {
+// Packed rows: one box of 64 columns (column, head, row).  Cache pages: one box of whole atoms, all columns that the stage
+// wants at once (column 0 of an atom, its row 0, slab, group of eight rows, block), so that a page is one or two boxes:
+// with a box per page and slab, boxes of 2 KB, the issuing warp bounded the kernel (512 rows at 8192 positions 454 us).
+template <int CG>
+__device__ __forceinline__ void tc_box_rows(unsigned dst, const CUtensorMap* map, int x, int h, int r, unsigned bar, unsigned elected) {
 #define LEV_BOX(GROUP)                                                                                                       \
-    if (DIMS == 4)                                                                                                           \
-        asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %7, 0;\n"                                                           \
-                     " @q cp.async.bulk.tensor.4d" GROUP ".shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n}\n" \
-                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(h), "r"(r), "r"(b), "r"(bar), "r"(elected) \
-                     : "memory");                                                                                            \
-    else                                                                                                                     \
-        asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %6, 0;\n"                                                           \
-                     " @q cp.async.bulk.tensor.3d" GROUP ".shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n}\n" \
-                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(h), "r"(r), "r"(bar), "r"(elected)         \
-                     : "memory")
-    if (CG == 2) {
-        LEV_BOX(".cta_group::2");
-    } else {
-        LEV_BOX("");
-    }
+    asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %6, 0;\n"                                                               \
+                 " @q cp.async.bulk.tensor.3d" GROUP ".shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n}\n" \
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(h), "r"(r), "r"(bar), "r"(elected)             \
+                 : "memory")
+    if (CG == 2) LEV_BOX(".cta_group::2");
+    else LEV_BOX("");
+#undef LEV_BOX
+}
+template <int CG>
+__device__ __forceinline__ void tc_box_page(unsigned dst, const CUtensorMap* map, int slab, int group, int block, unsigned bar, unsigned elected) {
+#define LEV_BOX(GROUP)                                                                                                       \
+    asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %6, 0;\n"                                                               \
+                 " @q cp.async.bulk.tensor.5d" GROUP ".shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%7, %7, %2, %3, %4}], [%5];\n}\n" \
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(slab), "r"(group), "r"(block), "r"(bar), "r"(elected), "r"(0) \
+                 : "memory")
+    if (CG == 2) LEV_BOX(".cta_group::2");
+    else LEV_BOX("");
 #undef LEV_BOX
 }
 
@@ -188,6 +215,14 @@ __device__ bool tc_find(const TcArgs& A, int u, int per, int lane, TcUnit* U) {
         before += __shfl_sync(0xffffffffu, scan, 31);
     }
     return found;
+}
+
+// layout of a stage of `rows` x `cols`: boxes of pages are whole rows of atoms, boxes of packed rows and copied rows slabs
+__device__ __forceinline__ TcLayout tc_layout(const TcArgs& A, int rows, int cols) {
+    TcLayout L;
+    L.group = A.box_k > 0 && A.table ? (unsigned)cols * 16u : 1024u;
+    L.slab = A.box_k > 0 && A.table ? 1024u : (unsigned)rows * 128u;
+    return L;
 }
 
 // element address of position p of this unit's KV head; NULL for a table entry outside the pool
@@ -560,7 +595,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
             const unsigned m_field = (unsigned)((128 * CG) >> 4) << 24;
             const unsigned id_qk = (1u << 4) | fmt | ((128u >> 3) << 17) | m_field;
             const unsigned id_pv = (1u << 4) | fmt | (1u << 16) | ((unsigned)((CG == 2 ? HD : 128) >> 3) << 17) | m_field;   // B is N-major
-            constexpr unsigned kKSlab = 128u / CG * 128u;   // bytes of 64 columns of this CTA's rows of K
+            const TcLayout kl = tc_layout(A, 128 / CG, HD / KV_STAGES), vl = tc_layout(A, 128, 128);
             Ring kr(NS), vr(NS);   // stages of the next K and of the next V tile
             auto qk = [&](int tile, int slot_i, bool release) {   // S[slot] = Q[tile] K^T
                 Ring st = kr;
@@ -572,8 +607,8 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                     constexpr int kSlabs = HD / 64 / KV_STAGES;
 #pragma unroll
                     for (int b = 0; b < kSlabs; b++)
-                        pk_mma4<CG>(tmem + (unsigned)slot_i * 128u, pk_desc_lo(smem + (unsigned)tile * D::kQTile + (unsigned)(h * kSlabs + b) * 16384u),
-                                    pk_desc_lo(kb + (unsigned)b * kKSlab), id_qk, (h | b) ? 1u : 0u, elected);
+                        tc_qk<CG>(tmem + (unsigned)slot_i * 128u, pk_desc_lo(smem + (unsigned)tile * D::kQTile + (unsigned)(h * kSlabs + b) * 16384u),
+                                  pk_desc_lo(kb + (unsigned)b * kl.slab), kl.hi(), id_qk, (h | b) ? 1u : 0u, elected);
                     if (release) pk_commit<CG>(smem_u32(&empty[st.s]), elected);
                     st.step(1);
                 }
@@ -586,8 +621,9 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                     pk_wait(smem_u32(&full[st.s]), st.ph, abort_flag);
                     tc_after();
                     const unsigned vb = ring + (unsigned)st.s * TC_STAGE;
-                    const unsigned b_lo = ((vb >> 4) & 0x3FFFu) | ((16384u >> 4) << 16);
-                    tc_pv<CG>(tmem + O_COL + (TILES == 2 ? tile * 128u : h * 128u), tmem + (unsigned)slot_i * 128u, b_lo, id_pv, first ? 0u : 1u, elected);
+                    const unsigned b_lo = ((vb >> 4) & 0x3FFFu) | ((vl.slab >> 4) << 16);
+                    tc_pv<CG>(tmem + O_COL + (TILES == 2 ? tile * 128u : h * 128u), tmem + (unsigned)slot_i * 128u, b_lo, vl.hi(), vl.group >> 3, id_pv,
+                              first ? 0u : 1u, elected);
                     if (release) pk_commit<CG>(smem_u32(&empty[st.s]), elected);
                     st.step(1);
                 }
@@ -644,56 +680,61 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
             const int32_t* trow = A.table ? A.table + (int64_t)U.slot * A.max_blocks : nullptr;
             const int page_lo = A.table ? lo_unit / A.page : 0, page_hi = A.table ? p_last / A.page : 0;
             Ring st(NS);
-            auto load = [&](int i, bool is_v) {
+            // Lane l: the table entry of the step's page l.  Pages that no row attends to are filled with zeros, not read.
+            auto entries = [&](int i) {
+                int e = (int)A.blocks;
+                const int pg = (jb + i) * TC_KV / A.page + lane;
+                if (trow && i < n && lane * A.box_v < TC_KV && pg >= page_lo && pg <= page_hi) {
+                    e = trow[pg];
+                    if (e < 0 || e >= A.blocks) {
+                        atomicOr(A.status, LEV_DEV_BAD_INDEX);
+                        bad_s = 1;
+                        e = (int)A.blocks;
+                    }
+                }
+                __syncwarp();
+                return e;
+            };
+            auto load = [&](int i, bool is_v, int entry) {
                 const CUtensorMap* map = is_v ? &vmap : &kmap;
                 const int c0 = (jb + i) * TC_KV;
                 const int r_first = CG == 2 && !is_v ? (int)rank * 64 : 0, r_n = CG == 2 && !is_v ? 64 : 128;   // rows of this CTA
-                const unsigned slab = (unsigned)r_n * 128u;
                 constexpr int kSlabsV = 2, kSlabsK = CG == 2 ? HD / 64 : 2;
-                int entry = 0;
                 const int box = is_v ? A.box_v : A.box_k;
-                if (trow) {   // lane l: the table entry of box l; pages that no row attends to are filled with zeros, not read
-                    const int pg = (c0 + r_first + lane * box) / A.page;
-                    entry = (int)A.blocks;
-                    if (lane * box < r_n && pg >= page_lo && pg <= page_hi) {
-                        entry = trow[pg];
-                        if (entry < 0 || entry >= A.blocks) {
-                            atomicOr(A.status, LEV_DEV_BAD_INDEX);
-                            bad_s = 1;
-                            entry = (int)A.blocks;
-                        }
-                    }
-                    __syncwarp();
-                }
+                const unsigned row_bytes = (is_v ? kSlabsV : kSlabsK) * 128u;
 #pragma unroll
                 for (int h = 0; h < KV_STAGES; h++) {
                     pk_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
                     const unsigned bar = full_c + 8u * (unsigned)st.s, dst = ring + (unsigned)st.s * TC_STAGE;
                     if (rank == 0) pk_expect(smem_u32(&full[st.s]), TC_STAGE * CG, elected);
                     const int x0 = CG == 2 ? (is_v ? (int)rank * 128 : 0) : h * 128;
-                    for (int r = 0; r < r_n; r += box) {
-                        const int e = trow ? __shfl_sync(0xffffffffu, entry, r / box) : 0;
-                        const int at = c0 + r_first + r;
+                    if (trow) {
+                        const int slab = (kvh * HD + x0) >> 6;
+                        const int in_page = A.page >= TC_KV ? (c0 + r_first) % A.page >> 3 : 0;   // first group of eight rows
+                        for (int r = 0; r < r_n; r += box)
+                            tc_box_page<CG>(dst + (unsigned)r * row_bytes, map, slab, in_page, __shfl_sync(0xffffffffu, entry, (r_first + r) / A.box_v), bar, elected);
+                    } else {
 #pragma unroll
-                        for (int b = 0; b < (is_v ? kSlabsV : kSlabsK); b++) {
-                            const unsigned to = dst + (unsigned)b * slab + (unsigned)r * 128u;
-                            if (trow) tc_box<CG, 4>(to, map, x0 + 64 * b, kvh, at % A.page, e, bar, elected);
-                            else tc_box<CG, 3>(to, map, x0 + 64 * b, kvh, U.row0 + at, 0, bar, elected);
-                        }
+                        for (int b = 0; b < (is_v ? kSlabsV : kSlabsK); b++)
+                            tc_box_rows<CG>(dst + (unsigned)(b * r_n) * 128u, map, x0 + 64 * b, kvh, U.row0 + c0 + r_first, bar, elected);
                     }
                     st.step(1);
                 }
             };
-            if (TILES == 2) {
-                for (int i = 0; i < n; i++) {
-                    load(i, false);
-                    load(i, true);
+            int e_now = entries(0), e_before = 0;
+            for (int i = 0; i <= n; i++) {
+                const int e_next = entries(i + 1);   // read a step ahead
+                if (TILES == 2) {
+                    if (i < n) {
+                        load(i, false, e_now);
+                        load(i, true, e_now);
+                    }
+                } else {
+                    if (i < n) load(i, false, e_now);
+                    if (i > 0) load(i - 1, true, e_before);
                 }
-            } else {
-                for (int i = 0; i <= n; i++) {
-                    if (i < n) load(i, false);
-                    if (i > 0) load(i - 1, true);
-                }
+                e_before = e_now;
+                e_now = e_next;
             }
             for (int s = 0; s < NS; s++) {   // the tensor core's last releases have arrived
                 pk_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
@@ -946,20 +987,22 @@ extern "C" int lev_attn_chunk(lev_ctx* ctx, const lev_kv_layout* L, const void* 
     A.max_blocks = L->max_blocks;
     A.slots = L->slots;
     // pages that make up whole steps of 128 positions out of whole swizzle atoms go by TMA, others are copied by warps
-    const bool boxes = A.kv_type == TC_F16 && L->page % 8 == 0 && (TC_KV % L->page == 0 || L->page % TC_KV == 0) && L->blocks < (1ll << 31);
+    const bool boxes = A.kv_type == TC_F16 && LEV_KV_ROW(0, 0, 1, L->page, L->kv_heads) == 1 && L->page % 8 == 0 && (TC_KV % L->page == 0 || L->page % TC_KV == 0) && L->blocks < (1ll << 31);
     const int64_t cap = (int64_t)L->max_blocks * L->page, span = window > 0 && window < cap ? window : cap;
     const TcPlan P = tc_plan(ctx, n_rows, n_chunks, L->kv_heads, A.tpt, hd, span, boxes);
     A.splits = P.splits;
     CUtensorMap kmap = {}, vmap = {};
     if (boxes) {
         const int box_v = L->page < TC_KV ? L->page : TC_KV, box_k = box_v > TC_KV / P.cg ? TC_KV / P.cg : box_v;
-        const cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)L->kv_heads, (cuuint64_t)L->page, (cuuint64_t)L->blocks};
-        const cuuint64_t strides[3] = {(cuuint64_t)(LEV_KV_ROW(0, 0, 1, L->page, L->kv_heads) * hd * 2), (cuuint64_t)(LEV_KV_ROW(0, 1, 0, L->page, L->kv_heads) * hd * 2),
-                                       (cuuint64_t)L->kv_heads * L->page * hd * 2};
-        const cuuint32_t one[4] = {1, 1, 1, 1};
+        // an atom's 64 columns and eight rows, then slabs of 64 columns over all heads, groups of eight rows, blocks
+        const int64_t row = LEV_KV_ROW(0, 1, 0, L->page, L->kv_heads) * hd * 2;
+        const cuuint64_t dims[5] = {64, 8, (cuuint64_t)L->kv_heads * hd / 64, (cuuint64_t)L->page / 8, (cuuint64_t)L->blocks};
+        const cuuint64_t strides[4] = {(cuuint64_t)row, 128, (cuuint64_t)row * 8, (cuuint64_t)row * L->page};
+        const cuuint32_t one[5] = {1, 1, 1, 1, 1};
         for (int i = 0; i < 2; i++) {
-            const cuuint32_t box[4] = {64, 1, (cuuint32_t)(i ? box_v : box_k), 1};
-            const CUresult cr = enc(i ? &vmap : &kmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(i ? v_pool : k_pool), dims, strides, box, one,
+            const cuuint32_t cols = P.cg == 2 && i == 0 ? hd / 64 : 2;
+            const cuuint32_t box[5] = {64, 8, cols, (cuuint32_t)(i ? box_v : box_k) / 8, 1};
+            const CUresult cr = enc(i ? &vmap : &kmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(i ? v_pool : k_pool), dims, strides, box, one,
                                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
             if (cr != CUDA_SUCCESS) return lev_fail(ctx, LEV_KERNEL_FAILED, "cuTensorMapEncodeTiled failed (%d)", (int)cr);

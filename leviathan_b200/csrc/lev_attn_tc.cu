@@ -98,6 +98,17 @@ __device__ __forceinline__ void tmem_st32(unsigned a, const unsigned* v) {
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+// arrives at `bar` of the CTAs of a pair (lead: the leader's rank in the cluster) when the MMAs issued so far are done
+template <int CG>
+__device__ __forceinline__ void tc_commit(unsigned bar, unsigned lead, unsigned elected) {
+    if (CG == 2)
+        asm volatile(
+            "{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
+            " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}\n" ::"r"(bar),
+            "h"((unsigned short)(3u << lead)), "r"(elected)
+            : "memory");
+    else pk_commit<1>(bar, elected);
+}
 __device__ __forceinline__ void wg_sync(int id) { asm volatile("bar.sync %0, 128;\n" ::"r"(id) : "memory"); }
 
 // How the 16-bit rows of a stage lie in shared memory: eight rows of 64 columns make a 1024-byte swizzle atom; `group` bytes
@@ -319,12 +330,12 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
     __shared__ __align__(8) unsigned long long full[NS], empty[NS], s_full[2], p_full[2], pv_done[2], q_full;
     __shared__ unsigned tmem_base_s;
     __shared__ int abort_s, bad_s;
-    __shared__ __align__(16) float merge_ml[128][2];   // splits: a row's reference and sum
+    __shared__ unsigned again_s[TILES * 4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const unsigned rank = CG == 2 ? cluster_rank() : 0u;
-    const int kvh = blockIdx.y;
-    const int split = CG == 2 ? 0 : (int)blockIdx.x % A.splits;
-    const int unit = (int)blockIdx.x / (CG == 2 ? 2 : A.splits);
+    // a cluster is a unit: the pair (one CTA without pairs) of split 0, then that of split 1, ...
+    const unsigned in_cluster = (int)blockIdx.x % (CG * A.splits);
+    const unsigned rank = in_cluster % CG, lead = in_cluster - rank;
+    const int kvh = blockIdx.y, split = (int)in_cluster / CG, unit = (int)blockIdx.x / (CG * A.splits);
     const int per = A.tpt * TILES * CG;
     pdl_wait();
     pdl_launch_dependents();
@@ -389,6 +400,11 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
     tc_after();
     const unsigned tmem = tmem_base_s;
     volatile int* abort_flag = &abort_s;
+    // splits: partial sums [tile][row][HD] where the queries and stages were, behind them 8 KB for one row's work or the
+    // merge's weights, then a row's reference and sum
+    unsigned char* const base = smem_dyn + (smem - smem_u32(smem_dyn));
+    constexpr unsigned kMergeAt = TILES * 128 * HD * 4, kStatsAt = kMergeAt + 8192;
+    float(*merge_ml)[2] = reinterpret_cast<float(*)[2]>(base + kStatsAt);
 
     if (warp < 4 * TILES) {
         // ---- softmax: thread = row of the tile ----
@@ -398,30 +414,49 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         const bool live = tok < A.tpt && tile_tok + tok < tokens;
         {   // the tile's queries, rounded to 16 bits, in the swizzled K-major layout
             const unsigned qs = smem + (unsigned)tile * D::kQTile;
-            constexpr int kPieces = HD / 8, kRows = 32 / kPieces < 1 ? 1 : 32 / kPieces;   // 16-byte pieces of a row; rows of a warp's step
+            constexpr int kPieces = HD / 8, kRows = 32 / kPieces;   // 16-byte pieces of a row; rows of a warp's step
+            constexpr int kBatch = TILES == 2 ? 8 : 16;             // steps requested before the first is stored
             const int piece = lane % kPieces, sub = lane / kPieces;
-#pragma unroll 4
-            for (int r0 = w4 * 32; r0 < w4 * 32 + 32; r0 += kRows) {
-                const int r = r0 + sub, rt = r / A.group;
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (rt < A.tpt && tile_tok + rt < tokens) {
-                    const int64_t at = (int64_t)(U.row0 + U.t0 + tile_tok + rt) * A.q_ld + (int64_t)(kvh * A.group + r - rt * A.group) * HD + piece * 8;
-                    if (A.q_type == TC_F32) {
-                        const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(A.q) + at);
-                        const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(A.q) + at + 4);
-                        v = make_uint4(pack16(a.x, a.y, TC_F16), pack16(a.z, a.w, TC_F16), pack16(b.x, b.y, TC_F16), pack16(b.z, b.w, TC_F16));
-                    } else {
-                        v = *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(A.q) + at);
-                    }
-                    if (A.negate) v = make_uint4(v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
-                }
+            auto row_at = [&](int r) -> int64_t {   // element offset of this lane's piece; negative: no such row
+                const int rt = r / A.group;
+                if (rt >= A.tpt || tile_tok + rt >= tokens) return -1;
+                return (int64_t)(U.row0 + U.t0 + tile_tok + rt) * A.q_ld + (int64_t)(kvh * A.group + r - rt * A.group) * HD + piece * 8;
+            };
+            auto put = [&](int r, uint4 v) {
+                if (A.negate) v = make_uint4(v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
                 const unsigned dst = qs + (unsigned)(piece >> 3) * 16384u + (unsigned)r * 128u + (unsigned)(((piece & 7) ^ (r & 7)) << 4);
                 asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+            };
+#pragma unroll 1
+            for (int r0 = w4 * 32 + sub; r0 < w4 * 32 + 32; r0 += kRows * kBatch) {
+                if (A.q_type == TC_F32) {
+                    float4 a[kBatch], b[kBatch];
+#pragma unroll
+                    for (int i = 0; i < kBatch; i++) {
+                        const int64_t at = row_at(r0 + i * kRows);
+                        const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(A.q) + at);
+                        a[i] = at >= 0 ? src[0] : make_float4(0.f, 0.f, 0.f, 0.f);
+                        b[i] = at >= 0 ? src[1] : make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+#pragma unroll
+                    for (int i = 0; i < kBatch; i++)
+                        put(r0 + i * kRows, make_uint4(pack16(a[i].x, a[i].y, TC_F16), pack16(a[i].z, a[i].w, TC_F16), pack16(b[i].x, b[i].y, TC_F16),
+                                                       pack16(b[i].z, b[i].w, TC_F16)));
+                } else {
+                    uint4 v[kBatch];
+#pragma unroll
+                    for (int i = 0; i < kBatch; i++) {
+                        const int64_t at = row_at(r0 + i * kRows);
+                        v[i] = at >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(A.q) + at) : make_uint4(0u, 0u, 0u, 0u);
+                    }
+#pragma unroll
+                    for (int i = 0; i < kBatch; i++) put(r0 + i * kRows, v[i]);
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
             if (lane == 0) {
-                if (CG == 2) mbar_arrive_cluster(map_to_rank(smem_u32(&q_full), 0));
+                if (CG == 2) mbar_arrive_cluster(map_to_rank(smem_u32(&q_full), lead));
                 else mbar_arrive(smem_u32(&q_full));
             }
         }
@@ -509,13 +544,14 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
             __syncwarp();
             if (lane == 0) {
                 const unsigned bar = smem_u32(&p_full[slot_i]);
-                if (CG == 2) mbar_arrive_cluster(map_to_rank(bar, 0));
+                if (CG == 2) mbar_arrive_cluster(map_to_rank(bar, lead));
                 else mbar_arrive(bar);
             }
         }
         if (n > 0) {
             const int last = TILES == 2 ? tile : (n - 1) & 1, lpar = TILES == 2 ? (n - 1) & 1 : ((n - 1) >> 1) & 1;
             pk_wait(smem_u32(&pv_done[last]), lpar, abort_flag);
+            if (TILES == 2 && A.splits > 1) pk_wait(smem_u32(&pv_done[tile ^ 1]), lpar, abort_flag);   // the partial sums go where K and V were
             __syncwarp();
             tc_after();
         }
@@ -526,7 +562,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         const int64_t out_at = (int64_t)(U.row0 + U.t0 + tile_tok + tok) * A.out_ld + (int64_t)head * HD;
         const float inv = bad ? NAN : 1.f / l;
         float probe = 0.f;   // NaN when a sum is not finite
-        float* part_o = reinterpret_cast<float*>(smem_dyn + (smem - smem_u32(smem_dyn)));   // splits: [row][HD], 16-byte pieces swizzled
+        float* part_o = reinterpret_cast<float*>(base) + tile * 128 * HD;   // splits: [row][HD], 16-byte pieces swizzled
         if (n > 0) {
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
@@ -552,15 +588,13 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         tc_before();
         // rows that met a non-finite value where they do not attend (or where they do: the answer is then the same)
         const unsigned again_warp = __ballot_sync(0xffffffffu, live && n > 0 && !bad && probe != 0.f);
-        unsigned* again_s = reinterpret_cast<unsigned*>(&merge_ml[0][0]) + 4 * tile;   // the statistics are stored behind this
-        if (lane == 0) again_s[w4] = again_warp;
+        if (lane == 0) again_s[tile * 4 + w4] = again_warp;
         wg_sync(1 + tile);
         unsigned again[4];
 #pragma unroll
-        for (int q = 0; q < 4; q++) again[q] = again_s[q];
-        wg_sync(1 + tile);
+        for (int q = 0; q < 4; q++) again[q] = again_s[tile * 4 + q];
         if (again[0] | again[1] | again[2] | again[3]) {
-            float* scratch = reinterpret_cast<float*>(smem_dyn + (smem - smem_u32(smem_dyn)) + (A.splits > 1 ? 128 * HD * 4 : tile * (int)D::kQTile));
+            float* scratch = reinterpret_cast<float*>(base + (A.splits > 1 ? kMergeAt + tile * 2048 : tile * D::kQTile));
 #pragma unroll 1
             for (int r = 0; r < 128; r++) {
                 if (!((again[r >> 5] >> (r & 31)) & 1u)) continue;
@@ -584,8 +618,8 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
             }
         }
         if (A.splits > 1) {
-            merge_ml[t][0] = bad ? 0.f : m;
-            merge_ml[t][1] = bad ? NAN : l;
+            merge_ml[tile * 128 + t][0] = bad ? 0.f : m;
+            merge_ml[tile * 128 + t][1] = bad ? NAN : l;
         }
     } else if (warp == D::kMma) {
         // ---- MMA issue (of a pair: the leader): the whole warp walks the loop, one elected lane issues ----
@@ -609,10 +643,10 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                     for (int b = 0; b < kSlabs; b++)
                         tc_qk<CG>(tmem + (unsigned)slot_i * 128u, pk_desc_lo(smem + (unsigned)tile * D::kQTile + (unsigned)(h * kSlabs + b) * 16384u),
                                   pk_desc_lo(kb + (unsigned)b * kl.slab), kl.hi(), id_qk, (h | b) ? 1u : 0u, elected);
-                    if (release) pk_commit<CG>(smem_u32(&empty[st.s]), elected);
+                    if (release) tc_commit<CG>(smem_u32(&empty[st.s]), lead, elected);
                     st.step(1);
                 }
-                pk_commit<CG>(smem_u32(&s_full[slot_i]), elected);
+                tc_commit<CG>(smem_u32(&s_full[slot_i]), lead, elected);
             };
             auto pv = [&](int tile, int slot_i, bool first, bool release) {   // O[tile] += P[slot] V
                 Ring st = vr;
@@ -624,10 +658,10 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                     const unsigned b_lo = ((vb >> 4) & 0x3FFFu) | ((vl.slab >> 4) << 16);
                     tc_pv<CG>(tmem + O_COL + (TILES == 2 ? tile * 128u : h * 128u), tmem + (unsigned)slot_i * 128u, b_lo, vl.hi(), vl.group >> 3, id_pv,
                               first ? 0u : 1u, elected);
-                    if (release) pk_commit<CG>(smem_u32(&empty[st.s]), elected);
+                    if (release) tc_commit<CG>(smem_u32(&empty[st.s]), lead, elected);
                     st.step(1);
                 }
-                pk_commit<CG>(smem_u32(&pv_done[slot_i]), elected);
+                tc_commit<CG>(smem_u32(&pv_done[slot_i]), lead, elected);
             };
             pk_wait(smem_u32(&q_full), 0, abort_flag);
             tc_after();
@@ -673,10 +707,11 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
             }
         }
     } else if (tma) {
-        // ---- TMA boxes, in the order in which the MMA warp takes the stages ----
-        if (warp == D::kTma) {
+        // ---- TMA boxes, in the order in which the MMA warp takes the stages; three warps share a stage's boxes ----
+        {
+            const int w = warp - D::kTma;
             const unsigned elected = elect_lane();
-            const unsigned full_c = CG == 2 ? map_to_rank(smem_u32(&full[0]), 0) : smem_u32(&full[0]);
+            const unsigned full_c = CG == 2 ? map_to_rank(smem_u32(&full[0]), lead) : smem_u32(&full[0]);
             const int32_t* trow = A.table ? A.table + (int64_t)U.slot * A.max_blocks : nullptr;
             const int page_lo = A.table ? lo_unit / A.page : 0, page_hi = A.table ? p_last / A.page : 0;
             Ring st(NS);
@@ -706,16 +741,15 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 for (int h = 0; h < KV_STAGES; h++) {
                     pk_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
                     const unsigned bar = full_c + 8u * (unsigned)st.s, dst = ring + (unsigned)st.s * TC_STAGE;
-                    if (rank == 0) pk_expect(smem_u32(&full[st.s]), TC_STAGE * CG, elected);
+                    if (rank == 0 && w == 0) pk_expect(smem_u32(&full[st.s]), TC_STAGE * CG, elected);
                     const int x0 = CG == 2 ? (is_v ? (int)rank * 128 : 0) : h * 128;
                     if (trow) {
                         const int slab = (kvh * HD + x0) >> 6;
                         const int in_page = A.page >= TC_KV ? (c0 + r_first) % A.page >> 3 : 0;   // first group of eight rows
-                        for (int r = 0; r < r_n; r += box)
+                        for (int r = w * box; r < r_n; r += TC_LOAD_WARPS * box)
                             tc_box_page<CG>(dst + (unsigned)r * row_bytes, map, slab, in_page, __shfl_sync(0xffffffffu, entry, (r_first + r) / A.box_v), bar, elected);
                     } else {
-#pragma unroll
-                        for (int b = 0; b < (is_v ? kSlabsV : kSlabsK); b++)
+                        for (int b = w; b < (is_v ? kSlabsV : kSlabsK); b += TC_LOAD_WARPS)
                             tc_box_rows<CG>(dst + (unsigned)(b * r_n) * 128u, map, x0 + 64 * b, kvh, U.row0 + c0 + r_first, bar, elected);
                     }
                     st.step(1);
@@ -805,43 +839,79 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         }
     }
     pk_finish(abort_flag, A.status, LEV_DEV_TIMEOUT);
-    if (CG == 1 && A.splits > 1) {
-        // ---- merge: CTA z of the cluster adds its share of the rows, the parts in order ----
+    if (A.splits > 1) {
+        // ---- merge: the CTA of split z adds its share of the rows over all splits, in their order ----
         cluster_sync_all();
-        const int used = tokens * A.group, Z = A.splits;
-        const int ra = used * split / Z, rb = used * (split + 1) / Z;
-        const unsigned ml = smem_u32(&merge_ml[0][0]);
-        constexpr int kQuads = HD / 4;
-        for (int item = ra * kQuads + threadIdx.x; item < rb * kQuads; item += blockDim.x) {
-            const int r = item / kQuads, qd = item - r * kQuads;
-            float mm = -INFINITY;
-            for (int z = 0; z < Z; z++) {
-                float mz;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(mz) : "r"(map_to_rank(ml + 8u * r, z)) : "memory");
-                mm = fmaxf(mm, mz);
+        const int Z = A.splits;
+        float* wts = reinterpret_cast<float*>(base + kMergeAt);   // [row][Z]: a part's share of a row
+#pragma unroll 1
+        for (int tile = 0; tile < TILES; tile++) {
+            const int tile_tok = (int)(rank * TILES + tile) * A.tpt;
+            const int used = tokens > tile_tok ? (tokens - tile_tok < A.tpt ? tokens - tile_tok : A.tpt) * A.group : 0;
+            const int ra = used * split / Z, rb = used * (split + 1) / Z;
+            __syncthreads();   // the weights of the tile before are read
+            for (int r = ra + (int)threadIdx.x; r < rb; r += blockDim.x) {
+                float m[16], l[16], mm = -INFINITY, ll = 0.f;
+#pragma unroll
+                for (int z = 0; z < 16; z++) {
+                    m[z] = -INFINITY, l[z] = 0.f;
+                    if (z < Z)
+                        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];\n"
+                                     : "=f"(m[z]), "=f"(l[z])
+                                     : "r"(map_to_rank(smem + kStatsAt + 8u * (unsigned)(tile * 128 + r), z * CG + rank))
+                                     : "memory");
+                }
+#pragma unroll
+                for (int z = 0; z < 16; z++) mm = fmaxf(mm, m[z]);
+#pragma unroll
+                for (int z = 0; z < 16; z++) {
+                    m[z] = m[z] == -INFINITY && l[z] == 0.f ? 0.f : ex2((m[z] - mm) * A.sl);   // 0: the part attends to nothing
+                    ll = fmaf(l[z], m[z], ll);
+                }
+                const float inv = 1.f / ll;
+#pragma unroll
+                for (int z = 0; z < 16; z++)
+                    if (z < Z) wts[r * Z + z] = m[z] * inv;
             }
-            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-            float l = 0.f;
-            for (int z = 0; z < Z; z++) {
-                float mz, lz;
-                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];\n" : "=f"(mz), "=f"(lz) : "r"(map_to_rank(ml + 8u * r, z)) : "memory");
-                if (mz == -INFINITY && lz == 0.f) continue;   // this part attends to nothing
-                const float w = ex2((mz - mm) * A.sl);
-                float4 o;
-                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n"
-                             : "=f"(o.x), "=f"(o.y), "=f"(o.z), "=f"(o.w)
-                             : "r"(map_to_rank(smem + (unsigned)(r * HD + ((qd ^ (r & 7)) << 2)) * 4u, z))
-                             : "memory");
-                l = fmaf(lz, w, l);
-                a.x = fmaf(o.x, w, a.x);
-                a.y = fmaf(o.y, w, a.y);
-                a.z = fmaf(o.z, w, a.z);
-                a.w = fmaf(o.w, w, a.w);
+            __syncthreads();
+            constexpr int kQuads = HD / 4, kItems = 4;
+            const int first = ra * kQuads + (int)threadIdx.x, end = rb * kQuads;
+            for (int i0 = first; i0 < end; i0 += kItems * (int)blockDim.x) {
+                float4 a[kItems];
+#pragma unroll
+                for (int k = 0; k < kItems; k++) a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+                for (int z = 0; z < Z; z++) {
+                    const unsigned part = map_to_rank(smem + (unsigned)(tile * 128 * HD) * 4u, z * CG + rank);
+                    float4 o[kItems];
+                    float w[kItems];
+#pragma unroll
+                    for (int k = 0; k < kItems; k++) {
+                        const int item = i0 + k * (int)blockDim.x, r = item / kQuads, qd = item - r * kQuads;
+                        w[k] = item < end ? wts[r * Z + z] : 0.f;
+                        o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (w[k] != 0.f)
+                            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n"
+                                         : "=f"(o[k].x), "=f"(o[k].y), "=f"(o[k].z), "=f"(o[k].w)
+                                         : "r"(part + (unsigned)(r * HD + ((qd ^ (r & 7)) << 2)) * 4u));
+                    }
+#pragma unroll
+                    for (int k = 0; k < kItems; k++) {
+                        a[k].x = fmaf(o[k].x, w[k], a[k].x);
+                        a[k].y = fmaf(o[k].y, w[k], a[k].y);
+                        a[k].z = fmaf(o[k].z, w[k], a[k].z);
+                        a[k].w = fmaf(o[k].w, w[k], a[k].w);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < kItems; k++) {
+                    const int item = i0 + k * (int)blockDim.x, r = item / kQuads, qd = item - r * kQuads, tok = r / A.group;
+                    if (item >= end) continue;
+                    unsigned short* dst = static_cast<unsigned short*>(A.out) + (int64_t)(U.row0 + U.t0 + tile_tok + tok) * A.out_ld +
+                                          (int64_t)(kvh * A.group + r - tok * A.group) * HD + 4 * qd;
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(pack16(a[k].x, a[k].y, A.out_type), pack16(a[k].z, a[k].w, A.out_type));
+                }
             }
-            const float inv = 1.f / l;
-            const int tok = r / A.group;
-            unsigned short* dst = static_cast<unsigned short*>(A.out) + (int64_t)(U.row0 + U.t0 + tok) * A.out_ld + (int64_t)(kvh * A.group + r - tok * A.group) * HD + 4 * qd;
-            *reinterpret_cast<uint2*>(dst) = make_uint2(pack16(a.x * inv, a.y * inv, A.out_type), pack16(a.z * inv, a.w * inv, A.out_type));
         }
         cluster_sync_all();   // a CTA's shared memory stays until its peers have read it
     }
@@ -865,14 +935,13 @@ struct TcPlan {
 TcPlan tc_plan(const lev_ctx* ctx, int64_t rows, int seqs, int kv_heads, int tpt, int hd, int64_t span, bool boxes) {
     TcPlan P = {1, 1, 1, 0};
     const int64_t mean = (rows + seqs - 1) / seqs, sms = ctx->prop.multiProcessorCount;
-    const int64_t tiles = (mean + tpt - 1) / tpt * seqs * kv_heads;   // 128-row tiles, about
-    if (2 * tiles <= sms) {
-        // few tiles: the CTAs of a cluster share the positions of one
-        while (P.splits < 16 && 2 * P.splits * tiles <= sms && 2 * P.splits * TC_KV <= span) P.splits *= 2;
-    } else if (mean > tpt) {
+    if (mean > tpt) {
         if (hd == 128) P.tiles = 2;
         else if (boxes) P.cg = 2;
     }
+    // few units: the CTAs of a cluster share the positions of one
+    const int64_t ctas = (mean + tpt * P.tiles * P.cg - 1) / (tpt * P.tiles * P.cg) * P.cg * seqs * kv_heads;
+    while (2 * P.splits * P.cg <= 8 && 2 * P.splits * ctas <= sms && 2 * P.splits * TC_KV <= span) P.splits *= 2;
     const int64_t per = (int64_t)tpt * P.tiles * P.cg;
     P.units = rows / per + seqs < rows ? rows / per + seqs : rows;
     return P;
@@ -884,10 +953,9 @@ int tc_launch(lev_ctx* ctx, const CUtensorMap& kmap, const CUtensorMap& vmap, co
     static bool configured[16] = {};
     if (!configured[ctx->device & 15]) {
         LEV_CUDA(ctx, cudaFuncSetAttribute(k_attn_tc<HD, TILES, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)D::kSmem));
-        if (TILES == 1 && CG == 1) LEV_CUDA(ctx, cudaFuncSetAttribute(k_attn_tc<HD, TILES, CG>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         configured[ctx->device & 15] = true;
     }
-    const int cluster = CG == 2 ? 2 : A.splits;
+    const int cluster = CG * A.splits;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(units * cluster), (unsigned)A.kv_heads);
     cfg.blockDim = dim3(D::kWarps * 32);

@@ -260,6 +260,20 @@ int lev_rmsnorm_cached(lev_ctx* ctx, const float* x, int64_t vectors, int64_t n,
                        const float* weight, const float* inverse, float* y);
 int lev_gelu_up(lev_ctx* ctx, const float* gate_up, int64_t vectors, int64_t inter, float* out);
 int lev_axpy(lev_ctx* ctx, float alpha, const float* x, const float* r, int64_t n, float* y);
+/* Element types of the activations that lev_norm_residual, lev_logprobs, lev_attn_chunk and lev_attn_prompt take or leave. */
+enum { LEV_ELEM_F32 = 0, LEV_ELEM_F16 = 1, LEV_ELEM_BF16 = 2 };
+/* The norm behind a block, its gate, the residual sum and scale and the norm before the next block, in one launch
+ * (the axpy and rmsnorm pair between two blocks of the layer loop, Gemma4.swift:3740-3760, :3878, and the conversion of
+ * lev_act_bf16 behind it):
+ *   b = x * inv_rms(x) * post   (norm_post 0: b = x, post NULL; post NULL: no scale)
+ *   out = scale * (residual + alpha * gate * b)
+ *   h = out * inv_rms(out) * pre  (h NULL: left out; pre NULL: no scale), h of type h_type
+ * x, residual, out f32 [rows][n], any n.  gate f32 (NULL: 1): one row for all (gate_ld 0) or rows gate_ld elements apart.
+ * out may be x or residual; h overlaps nothing.  Fastest on 16-byte boundaries with n % 4 == 0, up to 4096 elements. */
+int lev_norm_residual(lev_ctx* ctx, const float* x, const float* residual, int64_t rows, int64_t n,
+                      int norm_post, const float* post, const float* gate, int64_t gate_ld,
+                      float alpha, float scale, const float* pre, float eps, float* out, void* h,
+                      int h_type);
 /* The per-head steps between the q / k / v projections and the cache append of a local layer
  * (Sources/LeviathanCore/Gemma4.swift:3662-3687) in one launch, in place on rows laid out as
  * [q_heads | kv_heads (k) | kv_heads (v)] x head_dim: q heads RMSNorm(q_weight) then rotary, k heads
@@ -286,6 +300,21 @@ int lev_argmax(lev_ctx* ctx, const float* x, int64_t vectors, int64_t n, int32_t
 int lev_embed_rows(lev_ctx* ctx, const lev_weights* w, const int32_t* tokens, int64_t n_tokens,
                    float scale, float* y);
 int lev_softcap(lev_ctx* ctx, float* x, int64_t n, float cap);
+
+/* Scores of rows of logits (type LEV_ELEM_*, rows ld elements apart, 1 to LEV_MAX_DIM logits), in one pass; what evaluates
+ * a prompt where lev_softcap + lev_argmax choose a token.  x = cap * tanh(l / cap) (cap 0: x = l):
+ *   logprob[r] = x[tokens[r]] - log sum e^x   (NULL: left out).  tokens int32 on the device; LEV_NO_TOKEN gives 0; another id
+ *     outside [0, n) gives NaN and is reported by the next status read
+ *   entropy[r] = -sum p log p   (NULL: left out)
+ *   top_index, top_logprob [rows][top]: the `top` (0 ... LEV_MAX_TOP_K) largest logits, largest first, ties to the lowest index
+ *     (-0 ties with 0, NaN comes last), with their log probabilities
+ * Logits of -inf have probability 0 (with a cap: that of -cap).  A row with NaN or +inf, or with nothing above -inf, has no
+ * distribution: its log probabilities and entropy are NaN, its top_index is still in order.  No work buffers; repeat runs give
+ * the same bits. */
+#define LEV_NO_TOKEN (-1)
+int lev_logprobs(lev_ctx* ctx, const void* logits, int type, int64_t rows, int64_t n, int64_t ld,
+                 float cap, const int32_t* tokens, int top, float* logprob, float* entropy,
+                 int32_t* top_index, float* top_logprob);
 
 /* The same steps folded into the matvec launch: the prologue is applied while the kernel builds
  * its activation tables (the norm's statistic is reduced by every thread block for itself), the
@@ -390,9 +419,7 @@ int lev_qkv_norm_rope_append_split(lev_ctx* ctx, float* q, float* k, float* v, i
                                    void* v_pool, const int32_t* block_table, const int32_t* slot);
 
 /* ---- attention of many rows per sequence (prompts, prompt pieces, drafted tokens) ------
- * Element types of activations that these and the scoring entry points take. */
-enum { LEV_ELEM_F32 = 0, LEV_ELEM_F16 = 1, LEV_ELEM_BF16 = 2 };
-/* lev_attn_chunk: a chunk of new tokens per sequence over the paged cache that already holds their K and V rows
+ * lev_attn_chunk: a chunk of new tokens per sequence over the paged cache that already holds their K and V rows
  * (lev_kv_append or lev_qkv_norm_rope_append first): the prompt side of lev_attn_decode.  Rows start[c] ... start[c+1]-1
  * of q and out belong to chunk c, whose first row is at position pos[c] of sequence slot[c]; the row at position p attends to
  * (p - window, p] (window 0: [0, p]), weights softmax(scale * q.k), query head h reads KV head h / (q_heads / kv_heads).

@@ -114,6 +114,8 @@ SIGNATURES = {
     "lev_kv_append": (_I, [_P, C.POINTER(KVLayout), _P, _P, _P, _P, _P, _I, _P, _P]),
     "lev_attn_decode": (_I, [_P, C.POINTER(KVLayout), _P, _P, _P, _P, _P, _I, _I, _P, _I, C.c_float, _P]),
     "lev_attn_decode_ld": (_I, [_P, C.POINTER(KVLayout), _P, _P, _P, _P, _P, _I, _I, _P, _L, _I, C.c_float, _P]),
+    "lev_norm_residual": (_I, [_P, _P, _P, _L, _L, _I, _P, _P, _L, C.c_float, C.c_float, _P, C.c_float, _P, _P, _I]),
+    "lev_logprobs": (_I, [_P, _P, _I, _L, _L, _L, C.c_float, _P, _I, _P, _P, _P, _P]),
     "lev_attn_chunk": (_I, [_P, C.POINTER(KVLayout), _P, _P, _P, _I, _P, _P, _P, _L, _I, _P, _I, _L, _I, C.c_float, _P, _I, _L]),
     "lev_attn_prompt": (_I, [_P, _I, _P, _L, _I, _I, _I, _I, _P, _L, _P, _L, _P, _L, _I, C.c_float, _P, _L]),
     "lev_gemm_prefill": (_I, [_P, _P, _P, _L, _P, _U]),
@@ -186,7 +188,8 @@ class _CtypesHost:
 
     def __init__(self, lib: C.CDLL):
         self._lib = lib
-        for name in ("matvec", "rmsnorm", "axpy", "act_bf16", "gemm_prefill", "moe_layer", "moe_layer_residual", "attn_prompt"):
+        for name in ("matvec", "rmsnorm", "axpy", "act_bf16", "gemm_prefill", "moe_layer", "moe_layer_residual", "attn_prompt",
+                     "norm_residual", "logprobs"):
             setattr(self, name, getattr(lib, "lev_" + name))
 
     def matvec_fused(self, ctx, w, row0, rows, x, x_count, n_cols, prologue, norm_weight, eps, residual, alpha, y, cap):

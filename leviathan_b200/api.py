@@ -315,6 +315,62 @@ class Context:
         self._check(self.host.axpy(self._h, alpha, _ptr(x), _ptr(r), x.numel(), _ptr(out)))
         return out
 
+    def norm_residual(self, x, residual, post=None, pre=None, gate=None, alpha: float = 1.0, scale: float = 1.0, eps: float = 1e-6,
+                      norm_post: bool | None = None, out=None, h=None, dtype=None):
+        """lev_norm_residual: (out, h) with out = scale * (residual + alpha * gate * rmsnorm(x) * post) and h = rmsnorm(out) * pre.
+        x and residual are f32 [rows][n]; the norm behind the block runs when `post` is given (or norm_post=True: without a scale);
+        gate is [n] or [rows][n]; h is f32 or of `dtype` (float16, bfloat16).  out may be residual or x; h=False leaves h out."""
+        import torch
+
+        rows, n = x.shape
+        out = torch.empty_like(residual) if out is None else out
+        if h is None:
+            h = torch.empty((rows, n), dtype=dtype or torch.float32, device=x.device)
+        elif h is False:
+            h = None
+        _on(self.device, x, residual, post, pre, gate, out, h)
+        for what, t, shape in (("x", x, (rows, n)), ("residual", residual, (rows, n)), ("out", out, (rows, n)), ("post", post, (n,)), ("pre", pre, (n,))):
+            if t is not None and (t.shape != shape or t.dtype is not torch.float32 or not t.is_contiguous()):
+                raise ValueError(f"{what}: contiguous float32 {shape} is wanted, got {tuple(t.shape)} of {t.dtype}")
+        gate_ld = 0
+        if gate is not None:
+            if gate.dtype is not torch.float32 or gate.stride(-1) != 1 or tuple(gate.shape) not in ((n,), (rows, n)):
+                raise ValueError(f"gate: float32 ({n},) or ({rows}, {n}) is wanted, got {tuple(gate.shape)} of {gate.dtype}")
+            gate_ld = gate.stride(0) if gate.ndim == 2 and rows > 1 else 0
+        ht = L.ELEM_F32
+        if h is not None:
+            ht = _elem(h, "h", "float32 float16 bfloat16")
+            if h.shape != (rows, n) or not h.is_contiguous():
+                raise ValueError(f"h: contiguous {(rows, n)} is wanted, got {tuple(h.shape)}")
+        self._flags(False, False)
+        self._check(self.host.norm_residual(self._h, _ptr(x), _ptr(residual), rows, n, int(post is not None if norm_post is None else norm_post),
+                                            _ptr(post), _ptr(gate), gate_ld, alpha, scale, _ptr(pre), eps, _ptr(out), _ptr(h), ht))
+        return out, h
+
+    def logprobs(self, logits, tokens=None, top: int = 0, softcap: float = 0.0):
+        """lev_logprobs over the rows of logits [rows][n] (f32, f16 or bf16; rows may be a stride apart): (logprob of tokens int32 [rows],
+        entropy, top_index [rows][top], top_logprob [rows][top]); logprob is None without tokens, the last two without `top`."""
+        import torch
+
+        rows, n = logits.shape
+        if logits.stride(1) != 1:
+            raise ValueError("logits: rows of contiguous values are wanted")
+        ty = _elem(logits, "logits", "float32 float16 bfloat16")
+        _on(self.device, logits, tokens)
+        lp = ids = lps = None
+        if tokens is not None:
+            _i32(tokens, rows, "tokens")
+        vals = torch.empty((2, rows), dtype=torch.float32, device=logits.device)
+        if tokens is not None:
+            lp = vals[0]
+        if top > 0:
+            ids = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
+            lps = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
+        self._flags(False, False)
+        self._check(self.host.logprobs(self._h, _ptr(logits), ty, rows, n, logits.stride(0) if rows > 1 else n, softcap, _ptr(tokens), top, _ptr(lp),
+                                       _ptr(vals[1]), _ptr(ids), _ptr(lps)))
+        return lp, vals[1], ids, lps
+
     def qkv_norm_rope(self, qkv, q_heads: int, kv_heads: int, head_dim: int, q_weight=None, k_weight=None, eps: float = 1e-6,
                       inv_freq=None, pos=None):
         """lev_qkv_norm_rope, in place on qkv [n_cols][(q_heads + 2 * kv_heads) * head_dim]."""

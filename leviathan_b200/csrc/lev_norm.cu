@@ -6,6 +6,7 @@
 // (Sources/LeviathanCore/Gemma4.swift:4247-4268; the tiled form :4323-4358 reassociates the sum and
 // is gated against an f64 oracle, as this one is), g4_gelu_up (Gemma4.swift:4364-4377) and
 // g4_axpy (Gemma4.swift:4459).
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include "lev_stream.h"
@@ -102,6 +103,114 @@ __global__ void __launch_bounds__(kNormThreads) k_rmsnorm(const float* x, int n,
     }
 }
 
+// The norm behind a block, its gate, the residual sum and scale and the norm before the next block in one pass:
+//   b = x * inv_rms(x) * post,  r = scale * (residual + alpha * gate * b),  h = r * inv_rms(r) * pre
+// One CTA per row; both statistics are reduced in the order of k_rmsnorm.  Rows of up to kMixRegs * 1024 elements on
+// 16-byte boundaries stay in registers between the steps, and everything that does not wait for a statistic is requested up
+// front, so x and residual are read once and out and h written once.  Longer or unaligned rows are read again (r from out,
+// which every thread wrote itself).  out may be residual or x: a thread touches only its own elements.
+struct MixArgs {
+    const float *x, *residual, *post, *gate, *pre;
+    int64_t gate_ld;
+    float alpha, scale, eps;
+    float* out;
+    void* h;
+    int n, norm_post, h_type, vec;
+};
+constexpr int kMixRegs = 4;
+__device__ __forceinline__ float mix_block_sum(float v, float* part) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float tot = 0.f;
+#pragma unroll
+    for (int k = 0; k < kNormThreads / 32; k++) tot += part[k];
+    return tot;
+}
+__device__ __forceinline__ void mix_store(const MixArgs& A, int64_t at, float v) {
+    if (A.h_type == LEV_ELEM_F32) static_cast<float*>(A.h)[at] = v;
+    else if (A.h_type == LEV_ELEM_BF16) static_cast<__nv_bfloat16*>(A.h)[at] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(A.h)[at] = __float2half_rn(v);
+}
+__global__ void __launch_bounds__(kNormThreads) k_norm_residual(MixArgs A) {
+    __shared__ float part[2][kNormThreads / 32];
+    const int n = A.n;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int64_t row = blockIdx.x, base = row * n;
+    const float *x = A.x + base, *res = A.residual + base, *gate = A.gate ? A.gate + row * A.gate_ld : nullptr;
+    if (A.vec) {
+        float4 xv[kMixRegs], rv[kMixRegs], gv[kMixRegs], pv[kMixRegs];
+        const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < kMixRegs; k++) {
+            const int i = (threadIdx.x + k * kNormThreads) * 4;
+            const bool in = i < n;
+            xv[k] = in ? *reinterpret_cast<const float4*>(x + i) : none;
+            rv[k] = in ? *reinterpret_cast<const float4*>(res + i) : none;
+            gv[k] = in && gate ? *reinterpret_cast<const float4*>(gate + i) : make_float4(1.f, 1.f, 1.f, 1.f);
+            if (in && A.norm_post && A.post) {
+                const float4 w = __ldg(reinterpret_cast<const float4*>(A.post + i));
+                gv[k] = make_float4(gv[k].x * w.x, gv[k].y * w.y, gv[k].z * w.z, gv[k].w * w.w);
+            }
+            pv[k] = in && A.h && A.pre ? __ldg(reinterpret_cast<const float4*>(A.pre + i)) : make_float4(1.f, 1.f, 1.f, 1.f);
+        }
+        float mul = A.alpha;
+        if (A.norm_post) {
+            float ss = 0.f;
+#pragma unroll
+            for (int k = 0; k < kMixRegs; k++) ss = fmaf(xv[k].w, xv[k].w, fmaf(xv[k].z, xv[k].z, fmaf(xv[k].y, xv[k].y, fmaf(xv[k].x, xv[k].x, ss))));
+            mul *= 1.0f / sqrtf(mix_block_sum(ss, part[0]) / (float)n + A.eps);
+        }
+        float ss = 0.f;
+#pragma unroll
+        for (int k = 0; k < kMixRegs; k++) {
+            const int i = (threadIdx.x + k * kNormThreads) * 4;
+            float4 r = make_float4(A.scale * fmaf(mul * gv[k].x, xv[k].x, rv[k].x), A.scale * fmaf(mul * gv[k].y, xv[k].y, rv[k].y),
+                                   A.scale * fmaf(mul * gv[k].z, xv[k].z, rv[k].z), A.scale * fmaf(mul * gv[k].w, xv[k].w, rv[k].w));
+            rv[k] = r;
+            if (i < n) *reinterpret_cast<float4*>(A.out + base + i) = r;
+            ss = fmaf(r.w, r.w, fmaf(r.z, r.z, fmaf(r.y, r.y, fmaf(r.x, r.x, ss))));
+        }
+        if (!A.h) return;
+        const float inv = 1.0f / sqrtf(mix_block_sum(ss, part[1]) / (float)n + A.eps);
+#pragma unroll
+        for (int k = 0; k < kMixRegs; k++) {
+            const int i = (threadIdx.x + k * kNormThreads) * 4;
+            if (i >= n) continue;
+            const float4 h = make_float4(rv[k].x * inv * pv[k].x, rv[k].y * inv * pv[k].y, rv[k].z * inv * pv[k].z, rv[k].w * inv * pv[k].w);
+            if (A.h_type == LEV_ELEM_F32) {
+                *reinterpret_cast<float4*>(static_cast<float*>(A.h) + base + i) = h;
+            } else if (A.h_type == LEV_ELEM_BF16) {
+                const __nv_bfloat162 a = __floats2bfloat162_rn(h.x, h.y), b = __floats2bfloat162_rn(h.z, h.w);
+                *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(A.h) + base + i) = make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
+            } else {
+                const __half2 a = __floats2half2_rn(h.x, h.y), b = __floats2half2_rn(h.z, h.w);
+                *reinterpret_cast<uint2*>(static_cast<__half*>(A.h) + base + i) = make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
+            }
+        }
+        return;
+    }
+    float mul = A.alpha;
+    if (A.norm_post) {
+        float ss = 0.f;
+        for (int i = threadIdx.x; i < n; i += kNormThreads) ss = fmaf(x[i], x[i], ss);
+        mul *= 1.0f / sqrtf(mix_block_sum(ss, part[0]) / (float)n + A.eps);
+    }
+    float ss = 0.f;
+    for (int i = threadIdx.x; i < n; i += kNormThreads) {
+        float g = mul * (gate ? gate[i] : 1.f);
+        if (A.norm_post && A.post) g *= A.post[i];
+        const float r = A.scale * fmaf(g, x[i], res[i]);
+        A.out[base + i] = r;
+        ss = fmaf(r, r, ss);
+    }
+    if (!A.h) return;
+    const float inv = 1.0f / sqrtf(mix_block_sum(ss, part[1]) / (float)n + A.eps);
+    for (int i = threadIdx.x; i < n; i += kNormThreads) mix_store(A, base + i, A.out[base + i] * inv * (A.pre ? A.pre[i] : 1.f));
+}
+
 // out[v][e] = gelu_tanh(src[v][e]) * src[v][inter + e]
 __global__ void k_gelu_up(const float* __restrict__ src, int64_t inter, int64_t total, float* __restrict__ out) {
     pdl_wait();
@@ -180,6 +289,32 @@ extern "C" int lev_rmsnorm_cached(lev_ctx* ctx, const float* x, int64_t vectors,
     LEV_TRY(check_vectors(ctx, vectors, n));
     LEV_CUDA(ctx, cudaSetDevice(ctx->device));
     return rmsnorm_dev(ctx, x, vectors, n, weight, 0.f, y, nullptr, inverse);
+}
+
+extern "C" int lev_norm_residual(lev_ctx* ctx, const float* x, const float* residual, int64_t rows, int64_t n, int norm_post, const float* post,
+                                 const float* gate, int64_t gate_ld, float alpha, float scale, const float* pre, float eps, float* out, void* h,
+                                 int h_type) {
+    if (!ctx || !x || !residual || !out) return LEV_BAD_ARGUMENT;
+    LEV_TRY(check_vectors(ctx, rows, n));
+    if (!(eps >= 0.f) || !isfinite(eps) || !isfinite(alpha) || !isfinite(scale))
+        return lev_fail(ctx, LEV_BAD_ARGUMENT, "epsilon %g, alpha %g, scale %g", (double)eps, (double)alpha, (double)scale);
+    if (h && h_type != LEV_ELEM_F32 && h_type != LEV_ELEM_F16 && h_type != LEV_ELEM_BF16) return lev_fail(ctx, LEV_BAD_ARGUMENT, "element type %d", h_type);
+    if (post && !norm_post) return lev_fail(ctx, LEV_BAD_ARGUMENT, "a weight of the norm behind the block without that norm");
+    if (gate && gate_ld != 0 && gate_ld < n) return lev_fail(ctx, LEV_BAD_DIMENSIONS, "gate rows %lld elements apart (0 or at least %lld)", (long long)gate_ld, (long long)n);
+    const size_t bytes = (size_t)rows * n * 4, h_bytes = h ? (size_t)rows * n * (h_type == LEV_ELEM_F32 ? 4 : 2) : 0;
+    const size_t gate_bytes = gate ? ((size_t)(gate_ld ? (rows - 1) * gate_ld : 0) + n) * 4 : 0;
+    if ((out != x && overlap(out, bytes, x, bytes)) || (out != residual && overlap(out, bytes, residual, bytes)))
+        return lev_fail(ctx, LEV_BAD_ARGUMENT, "the output overlaps an input without being it");
+    if ((gate && overlap(out, bytes, gate, gate_bytes)) || (h && (overlap(h, h_bytes, x, bytes) || overlap(h, h_bytes, residual, bytes) || overlap(h, h_bytes, out, bytes) ||
+                                                                  (gate && overlap(h, h_bytes, gate, gate_bytes)))))
+        return lev_fail(ctx, LEV_BAD_ARGUMENT, "an output overlaps another argument");
+    LEV_CUDA(ctx, cudaSetDevice(ctx->device));
+    MixArgs A = {x, residual, post, gate, pre, gate_ld, alpha, scale, eps, out, h, (int)n, norm_post != 0, h_type, 0};
+    const uintptr_t all = (uintptr_t)x | (uintptr_t)residual | (uintptr_t)out | (uintptr_t)post | (uintptr_t)gate | (uintptr_t)pre | (uintptr_t)h;
+    A.vec = n % 4 == 0 && n <= kMixRegs * 4 * kNormThreads && (all & 15) == 0 && gate_ld % 4 == 0;
+    LEV_CUDA(ctx, launch_pdl(k_norm_residual, dim3((unsigned)rows), dim3(kNormThreads), 0, ctx->stream, A));
+    ctx->launches++;
+    return LEV_OK;
 }
 
 extern "C" int lev_gelu_up(lev_ctx* ctx, const float* gate_up, int64_t vectors, int64_t inter, float* out) {

@@ -74,10 +74,18 @@ HOST_FN(attn_prompt, 18, lev_ctx* c = P(a[0]); long long nc = I(a[1]); int32_t* 
         long long kl = I(a[11]); void* v = P(a[12]); long long vl = I(a[13]); long long win = I(a[14]); float sc = F(a[15]); void* y = P(a[16]);
         long long yl = I(a[17]),
         lev_attn_prompt(c, (int)nc, st0, rows, (int)qh, (int)kh, (int)hd, (int)ty, q, ql, k, kl, v, vl, (int)win, sc, y, yl))
+HOST_FN(norm_residual, 16, lev_ctx* c = P(a[0]); float* x = P(a[1]); float* r = P(a[2]); long long rows = I(a[3]); long long k = I(a[4]);
+        long long np = I(a[5]); float* post = P(a[6]); float* g = P(a[7]); long long gl = I(a[8]); float al = F(a[9]); float sc = F(a[10]);
+        float* pre = P(a[11]); float e = F(a[12]); float* y = P(a[13]); void* h = P(a[14]); long long ht = I(a[15]),
+        lev_norm_residual(c, x, r, rows, k, (int)np, post, g, gl, al, sc, pre, e, y, h, (int)ht))
+HOST_FN(logprobs, 13, lev_ctx* c = P(a[0]); void* x = P(a[1]); long long ty = I(a[2]); long long rows = I(a[3]); long long k = I(a[4]);
+        long long ld = I(a[5]); float cap = F(a[6]); int32_t* tok = P(a[7]); long long top = I(a[8]); float* lp = P(a[9]); float* en = P(a[10]);
+        int32_t* ti = P(a[11]); float* tl = P(a[12]), lev_logprobs(c, x, (int)ty, rows, k, ld, cap, tok, (int)top, lp, en, ti, tl))
 
 #define ENTRY(NAME) {#NAME, (PyCFunction)(void (*)(void))NAME, METH_FASTCALL, NULL}
 static PyMethodDef methods[] = {ENTRY(matvec), ENTRY(matvec_fused), ENTRY(matvec_chain), ENTRY(rmsnorm), ENTRY(axpy),
                                 ENTRY(act_bf16), ENTRY(gemm_prefill), ENTRY(moe_layer), ENTRY(moe_layer_residual), ENTRY(kv_append),
-                                ENTRY(attn_decode), ENTRY(attn_chunk), ENTRY(attn_prompt), {NULL, NULL, 0, NULL}};
+                                ENTRY(attn_decode), ENTRY(attn_chunk), ENTRY(attn_prompt),
+                                ENTRY(norm_residual), ENTRY(logprobs), {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pyhost", NULL, -1, methods, NULL, NULL, NULL, NULL};
 PyMODINIT_FUNC PyInit__pyhost(void) { return PyModule_Create(&module); }

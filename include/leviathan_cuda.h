@@ -308,7 +308,7 @@ int lev_softcap(lev_ctx* ctx, float* x, int64_t n, float cap);
  *   entropy[r] = -sum p log p   (NULL: left out)
  *   top_index, top_logprob [rows][top]: the `top` (0 ... LEV_MAX_TOP_K) largest logits, largest first, ties to the lowest index
  *     (-0 ties with 0, NaN comes last), with their log probabilities
- * Logits of -inf have probability 0 (with a cap: that of -cap).  A row with NaN or +inf, or with nothing above -inf, has no
+ * The capped value is off by up to cap * 2^-21.  Logits of -inf have probability 0 (with a cap: that of -cap).  A row with NaN or +inf, or with nothing above -inf, has no
  * distribution: its log probabilities and entropy are NaN, its top_index is still in order.  No work buffers; repeat runs give
  * the same bits. */
 #define LEV_NO_TOKEN (-1)

@@ -27,6 +27,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "lev_math2.cuh"
 #include "lev_stream.h"
 #include "lev_umma.cuh"
 
@@ -57,33 +58,11 @@ struct TcArgs {
     int* status;
 };
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ unsigned pack16(float lo, float hi, int type) {
     unsigned r;
     if (type == TC_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
     else asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
-}
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 two(float lo, float hi) {
-    f32x2 v;
-    asm("mov.b64 %0, {%1, %2};\n" : "=l"(v) : "f"(lo), "f"(hi));
-    return v;
-}
-__device__ __forceinline__ void both(f32x2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ f32x2 fma_2(f32x2 a, f32x2 b, f32x2 c) {
-    f32x2 v;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(v) : "l"(a), "l"(b), "l"(c));
-    return v;
-}
-__device__ __forceinline__ f32x2 add_2(f32x2 a, f32x2 b) {
-    f32x2 v;
-    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(v) : "l"(a), "l"(b));
-    return v;
 }
 __device__ __forceinline__ void tmem_st32(unsigned a, const unsigned* v) {
     asm volatile(

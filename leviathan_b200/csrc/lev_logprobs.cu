@@ -4,11 +4,17 @@
 //   lse = log sum_i e^x_i,   logprob = x_token - lse,   entropy = lse - sum_i e^(x_i - lse) x_i
 //   alternatives: the `top` largest l_i (the cap is monotone), ties to the lowest index like lev_argmax, with x_i - lse
 //
-// The row is read once.  Each thread keeps a running maximum m, s1 = sum e^(x - m) and s2 = sum e^(x - m) (x - m), f32 over a
-// few hundred to a few thousand values, then trees in a fixed order.  Alternatives: values that reach a threshold go to a buffer
-// as 64-bit keys (value in order, then index); the threshold starts as the least of at least `top` group maxima of the first
-// round and rises to the top-th key whenever the buffer is sorted, so that a few hundred of a row's values ever reach it.
-// The result is that of a full sort: keys are distinct, so the order in which threads append does not matter.
+// The row is read once.  Each thread keeps a running maximum m, s1 = sum e^(x - m) and s2 = sum e^(x - m) (x - m) (all in units
+// of log 2), f32 over a few hundred to a few thousand values, then trees in a fixed order.
+//
+// Alternatives: a thread's values of one round make a batch, and all that the pass over the row does for them is to leave the
+// batch's maximum in shared memory (with keys pushed under a running threshold in every round, 512 rows of 262144 took a
+// third longer).  The `top` largest values lie in the `top` batches with the largest best values: were a value's batch not
+// among them, `top` other batches would each hold a larger one.  So, behind the pass: a threshold that at least `top` values reach
+// (the least of the maxima of as many groups of threads); the batches that reach it, some hundred, are read again for the index of
+// their best value, go to a buffer as 64-bit keys (value in order, then index) and are sorted; then the values of the best `top`
+// batches that reach the last of these keys are.  Where the buffer would overflow (long ties) it is sorted in between and the threshold
+// rises.  The result is that of a full sort: keys are distinct, so the order in which threads append does not matter.
 //
 // A row belongs to a cluster of up to eight thread blocks, whose partial results the first one joins through distributed
 // shared memory: no work buffer, no second launch.
@@ -16,36 +22,55 @@
 #include <cuda_fp16.h>
 
 #include "lev_stream.h"
+#include "lev_math2.cuh"
 #include "lev_umma.cuh"
 
 namespace {
 
-constexpr int kLpRound = 16;     // values per thread and round
-constexpr int kLpKeys = 1024;    // keys of the buffer
-constexpr int kLpKeep = 384;     // it is sorted when it holds more after a round
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kLpRound = 16;     // values per thread and round: a batch
+constexpr int kLpCount = 192;    // up to so many keys are sorted by counting the larger ones
+constexpr int kLpKeys = 2048;    // keys of the buffer
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct LpArgs {
     const void* x;
     int64_t n, ld;
     const int32_t* tokens;
-    float cap, cap_k;   // cap_k = -2 log2(e) / cap
-    int top, group;     // group: lanes whose maximum counts as one in the first threshold
+    float cap_k, cap2;      // 2 log2(e) / cap, cap log2(e)
+    int top, group, keep;   // group: lanes whose maximum counts as one in the first threshold; keep: keys that the buffer may hold after a round
     float *logprob, *entropy, *top_logprob;
     int32_t* top_index;
     int* status;
 };
 
-__device__ __forceinline__ float lp_ex2(float x) {
+__device__ __forceinline__ float min_nan(float a, float b) {   // NaN if one is NaN
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
+// x in units of log 2 relative to ref2: tanh from a power of two and a reciprocal, 1 - 2 / (1 + e^(2 l / cap)); from an exponent of
+// 30 on the quotient is below f32's grid at 1
 template <bool CAP>
-__device__ __forceinline__ float lp_value(const LpArgs& A, float l) {
-    if (!CAP) return l;
-    const float e = lp_ex2(fabsf(l) * A.cap_k);   // e^(-2 |l| / cap)
-    return A.cap * copysignf(__fdividef(1.f - e, 1.f + e), l);
+__device__ __forceinline__ float lp_value(const LpArgs& A, float l, float ref2) {
+    if (!CAP) return fmaf(l, kLog2e, -ref2);
+    return fmaf(-2.f * A.cap2, rcp(1.f + ex2(min_nan(l * A.cap_k, 30.f))), A.cap2 - ref2);
+}
+// four at once: one reciprocal (of the product, at most 2^120) for four, because the special function unit bounds this kernel
+template <bool CAP>
+__device__ __forceinline__ void lp_values(const LpArgs& A, const float* l, float ref2, float* d) {
+    if constexpr (!CAP) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) d[i] = fmaf(l[i], kLog2e, -ref2);
+    } else {
+        float a[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) a[i] = 1.f + ex2(min_nan(l[i] * A.cap_k, 30.f));
+        const float ab = a[0] * a[1], cd = a[2] * a[3], r = rcp(ab * cd) * (-2.f * A.cap2), r0 = r * cd, r1 = r * ab, at = A.cap2 - ref2;
+        d[0] = fmaf(r0, a[1], at);
+        d[1] = fmaf(r0, a[0], at);
+        d[2] = fmaf(r1, a[3], at);
+        d[3] = fmaf(r1, a[2], at);
+    }
 }
 __device__ __forceinline__ float lp_load(const float* p) { return *p; }
 __device__ __forceinline__ float lp_load(const __half* p) { return __half2float(*p); }
@@ -78,14 +103,14 @@ __device__ __forceinline__ float lp_from_order(unsigned o) {
 }
 __device__ __forceinline__ unsigned long long lp_key(float l, int64_t i) { return ((unsigned long long)lp_order(l) << 32) | (unsigned)~(unsigned)i; }
 
-// running statistics; m = -inf: no value above -inf yet (s1 is then 0, or NaN)
+// running statistics in units of log 2; m = -inf: no value above -inf yet (s1 is then 0, or NaN)
 struct LpStats {
-    float m, s1, s2;
+    float m, s1, s2;   // reference, sum 2^(x - m), sum 2^(x - m) (x - m)
 };
 __device__ __forceinline__ LpStats lp_merge(LpStats a, LpStats b) {
     const float m = fmaxf(a.m, b.m);
     const float da = a.m == -INFINITY ? 0.f : a.m - m, db = b.m == -INFINITY ? 0.f : b.m - m;
-    const float wa = lp_ex2(da * kLog2e), wb = lp_ex2(db * kLog2e);
+    const float wa = ex2(da), wb = ex2(db);
     LpStats r;
     r.m = m;
     r.s1 = fmaf(a.s1, wa, b.s1 * wb);
@@ -110,16 +135,38 @@ __device__ void lp_sort(unsigned long long* keys, int P) {
         }
     __syncthreads();
 }
+// the same for c <= kLpCount distinct keys (and zeros up to `least`) in three barriers: a key's place is the number of larger ones
+template <int NT>
+__device__ void lp_sort_few(unsigned long long* keys, int c, int least, unsigned long long* tmp) {
+    __syncthreads();
+    const int t = threadIdx.x;
+    if (t == 0) keys[c] = 0;   // pairs are read
+    __syncthreads();
+    if (t < c) {
+        const unsigned long long k = keys[t];
+        int at = 0;
+        for (int i = 0; i < c; i += 2) {
+            const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(keys + i);
+            at += (o.x > k) + (o.y > k);
+        }
+        tmp[at] = k;
+    }
+    __syncthreads();
+    for (int i = t; i < c || i < least; i += NT) keys[i] = i < c ? tmp[i] : 0;
+    __syncthreads();
+}
 __device__ __forceinline__ int lp_pow2(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
 
 template <typename T, int NT, bool CAP>
-__global__ void __launch_bounds__(NT) k_logprobs(LpArgs A, int splits) {
+__global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) k_logprobs(LpArgs A, int splits) {
     constexpr int V = 16 / (int)sizeof(T), UNITS = kLpRound / V;   // values of a 16-byte unit; units per thread and round
-    __shared__ unsigned long long cand[kLpKeys];
+    __shared__ __align__(16) unsigned long long cand[kLpKeys], sorted_s[kLpCount];
+    extern __shared__ float batch_max[];   // [round][thread]
     __shared__ LpStats warp_stats[NT / 32], block_stats;
     __shared__ unsigned long long thr_key;
     __shared__ float thr_value, group_low[NT / 32], lse_s[2];
     __shared__ int count;
+    __shared__ unsigned batch_s[kLpKeys / kLpRound];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int64_t row = blockIdx.x / splits;
     const int z = (int)(blockIdx.x % splits);
@@ -127,13 +174,13 @@ __global__ void __launch_bounds__(NT) k_logprobs(LpArgs A, int splits) {
     pdl_launch_dependents();
     const T* x = static_cast<const T*>(A.x) + row * A.ld;
     // head and tail that are no whole 16-byte units go to the first block, one value per thread
-    int64_t head = ((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T);
-    head = head < A.n ? head : A.n;
-    const int64_t units = (A.n - head) / V, rest = A.n - units * V;   // rest: head and tail
-    const int64_t ub = units * z / splits, ue = units * (z + 1) / splits;
+    const int n = (int)A.n, skip = (int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T)), head = skip < n ? skip : n;
+    const int units = (n - head) / V, rest = n - units * V;   // rest: head and tail
+    const int ub = (int)((int64_t)units * z / splits), ue = (int)((int64_t)units * (z + 1) / splits);
     const uint4* body = reinterpret_cast<const uint4*>(x + head);
-    LpStats s = {-INFINITY, 0.f, 0.f};
-    float ref = 0.f;   // what weights are relative to: s.m once that is not -inf
+    // the thread's statistics: relative to ref2, which is the value of the largest logit so far (0 before there is one)
+    float raw_max = -INFINITY, ref2 = 0.f;
+    float s1[2] = {0.f, 0.f}, s2[2] = {0.f, 0.f};   // two chains of additions
     if (t == 0) {
         count = 0;
         thr_key = 0;
@@ -141,42 +188,49 @@ __global__ void __launch_bounds__(NT) k_logprobs(LpArgs A, int splits) {
     }
     __syncthreads();
 
-    // the values of one round (n of them valid, a multiple of the unit or one) into the statistics
-    auto raise = [&](float raw_max) {
-        if (raw_max == -INFINITY) return;
-        const float m = lp_value<CAP>(A, raw_max);
-        if (m > s.m) {
-            if (s.m != -INFINITY) {
-                const float d = s.m - m, w = lp_ex2(d * kLog2e);
-                s.s2 = w * fmaf(d, s.s1, s.s2);
-                s.s1 *= w;
+    auto raise = [&](float top) {
+        if (!(top > raw_max)) return;
+        const float m = lp_value<CAP>(A, top, 0.f);
+        if (raw_max != -INFINITY) {
+            const float d = ref2 - m, w = ex2(d);
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                s2[c] = w * fmaf(d, s1[c], s2[c]);
+                s1[c] *= w;
             }
-            s.m = ref = m;
+        }
+        raw_max = top;
+        ref2 = m;
+    };
+    auto add = [&](const float* l) {   // four values
+        float d[4];
+        lp_values<CAP>(A, l, ref2, d);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float e = ex2(d[i]);
+            s1[i & 1] += e;
+            s2[i & 1] = fmaf(e, CAP ? d[i] : fmaxf(d[i], -1e30f), s2[i & 1]);   // a weight of 0 times -inf is not 0
         }
     };
-    auto add = [&](float l) {
-        const float d = lp_value<CAP>(A, l) - ref, e = lp_ex2(d * kLog2e);
-        s.s1 += e;
-        s.s2 = fmaf(e, fmaxf(d, -1e30f), s.s2);   // e is 0 where d is -inf, and 0 * -inf is not
-    };
-    // appends a value that reaches the threshold; false when the buffer is full
     int over = 0;
-    auto push = [&](float l, int64_t i) {
-        if (l < thr_value) return true;
-        const unsigned long long k = lp_key(l, i);
-        if (k <= thr_key) return true;
+    auto append = [&](unsigned long long k) {
         const int at = atomicAdd(&count, 1);
-        over |= at >= kLpKeep;
-        if (at >= kLpKeys) return false;
-        cand[at] = k;
-        return true;
+        over |= at >= A.keep;
+        if (at < kLpKeys) cand[at] = k;   // always: the buffer is looked after in time
     };
-    // sorts the buffer, keeps the first `top` keys and raises the threshold to the last of them
+    auto push = [&](unsigned long long k) {
+        if (k > thr_key) append(k);
+    };
+    // sorts the buffer and keeps the first `top` keys; the threshold rises to the last of them
     auto settle = [&]() {
         __syncthreads();
         const int c = count < kLpKeys ? count : kLpKeys, P = lp_pow2(c > A.top ? c : A.top);
-        for (int i = c + t; i < P; i += NT) cand[i] = 0;
-        lp_sort<NT>(cand, P);
+        if (c <= kLpCount) {
+            lp_sort_few<NT>(cand, c, A.top, sorted_s);
+        } else {
+            for (int i = c + t; i < P; i += NT) cand[i] = 0;
+            lp_sort<NT>(cand, P);
+        }
         if (t == 0) {
             count = c < A.top ? c : A.top;
             if (c >= A.top) {
@@ -185,21 +239,23 @@ __global__ void __launch_bounds__(NT) k_logprobs(LpArgs A, int splits) {
                 if (thr_value != thr_value) thr_value = -INFINITY;
             }
         }
-        over = 0;
         __syncthreads();
     };
     if (z == 0 && t < rest) {
-        const int64_t i = t < head ? t : units * V + t;
+        const int i = t < head ? t : units * V + t;
         const float l = lp_load(x + i);
         raise(l);
-        add(l);
-        if (A.top) push(l, i);
+        float d = lp_value<CAP>(A, l, ref2);
+        const float e = ex2(d);
+        s1[0] = e;
+        s2[0] = e * fmaxf(d, -1e30f);
     }
-    const int64_t per_round = (int64_t)NT * UNITS;
+    constexpr int per_round = NT * UNITS;
     uint4 next[UNITS];
 #pragma unroll
     for (int j = 0; j < UNITS; j++) next[j] = ub + j * NT + t < ue ? __ldcs(body + ub + j * NT + t) : make_uint4(0u, 0u, 0u, 0u);
-    for (int64_t u0 = ub; u0 < ue; u0 += per_round) {
+    int round = 0;
+    for (int u0 = ub; u0 < ue; u0 += per_round, round++) {
         float l[UNITS][V];
         float mx = -INFINITY;
 #pragma unroll
@@ -207,11 +263,11 @@ __global__ void __launch_bounds__(NT) k_logprobs(LpArgs A, int splits) {
             lp_unpack(next[j], l[j], x);
             if (u0 + j * NT + t < ue)
 #pragma unroll
-                for (int i = 0; i < V; i++) mx = fmaxf(mx, l[j][i]);
+                for (int i = 0; i < V; i += 2) mx = max3(mx, l[j][i], l[j][i + 1]);
         }
 #pragma unroll
         for (int j = 0; j < UNITS; j++) {
-            const int64_t u = u0 + per_round + j * NT + t;
+            const int u = u0 + per_round + j * NT + t;
             next[j] = u < ue ? __ldcs(body + u) : make_uint4(0u, 0u, 0u, 0u);
         }
         raise(mx);
@@ -219,45 +275,16 @@ __global__ void __launch_bounds__(NT) k_logprobs(LpArgs A, int splits) {
         for (int j = 0; j < UNITS; j++)
             if (u0 + j * NT + t < ue)
 #pragma unroll
-                for (int i = 0; i < V; i++) add(l[j][i]);
-        if (A.top) {
-            if (u0 == ub) {   // the first threshold: at least `top` groups, each with a value that reaches the least of their maxima
-                float g = mx;
-                for (int o = 1; o < A.group; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) g = fminf(g, __shfl_xor_sync(0xffffffffu, g, o));
-                if (lane == 0) group_low[warp] = g;
-                __syncthreads();
-                if (t == 0) {
-                    float low = group_low[0];
-                    for (int w = 1; w < NT / 32; w++) low = fminf(low, group_low[w]);
-                    if (low > -INFINITY) {
-                        thr_value = low;
-                        thr_key = ((unsigned long long)lp_order(low) << 32) - 1;
-                    }
-                }
-                __syncthreads();
-            }
-            unsigned left = 0;   // values that the buffer has not taken yet
-            if (!(mx < thr_value))
-#pragma unroll
-                for (int j = 0; j < UNITS; j++)
-                    if (u0 + j * NT + t < ue) left |= ((1u << V) - 1) << (j * V);
-            for (;;) {
-                if (left)
-#pragma unroll
-                    for (int j = 0; j < UNITS; j++)
-#pragma unroll
-                        for (int i = 0; i < V; i++)
-                            if ((left >> (j * V + i)) & 1u)
-                                if (push(l[j][i], head + (u0 + j * NT + t) * V + i)) left &= ~(1u << (j * V + i));
-                if (!__syncthreads_or(left != 0 || over)) break;
-                settle();
-                if (!__syncthreads_or(left != 0)) break;
-            }
-        }
+                for (int i = 0; i < V; i += 4) add(l[j] + i);
+        if (A.top) batch_max[round * NT + t] = mx;
     }
     // ---- the block's results ----
+    LpStats s;
+    {
+        s.s1 = s1[0] + s1[1];
+        s.s2 = s2[0] + s2[1];
+        s.m = raw_max == -INFINITY ? -INFINITY : ref2;
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         LpStats b;
@@ -267,8 +294,116 @@ __global__ void __launch_bounds__(NT) k_logprobs(LpArgs A, int splits) {
         s = lp_merge(s, b);
     }
     if (lane == 0) warp_stats[warp] = s;
-    if (A.top) settle();
-    else __syncthreads();
+    if (A.top) {
+        // a threshold that at least `top` values reach: each group of threads has one that reaches the least of their maxima
+        float g = raw_max;
+        for (int o = 1; o < A.group; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) g = fminf(g, __shfl_xor_sync(0xffffffffu, g, o));
+        if (lane == 0) group_low[warp] = g;
+        __syncthreads();
+        if (t == 0) {
+            float low = group_low[0];
+            for (int w = 1; w < NT / 32; w++) low = fminf(low, group_low[w]);
+            if (low > -INFINITY) {
+                thr_value = low;
+                thr_key = ((unsigned long long)lp_order(low) << 32) - 1;
+            }
+        }
+        __syncthreads();
+        // The batches that reach it, by their maxima and numbers.  `look` replaces the entries behind the first `known` by their
+        // batches' best values and indices, all of them read at once, and sorts.
+        constexpr int kEvery = (kLpKeys - 3 * LEV_MAX_TOP_K) / NT;   // rounds for which the buffer has room
+        int known = 0;
+        auto look = [&]() {
+            __syncthreads();
+            const int c = count < kLpKeys ? count : kLpKeys;
+            for (int i = known + t; i < c; i += NT) {
+                const int b = (int)(unsigned)cand[i], u0 = ub + b / NT * per_round + b % NT;
+                unsigned long long best = 0;
+#pragma unroll
+                for (int j = 0; j < UNITS; j++) {
+                    const int u = u0 + j * NT;
+                    if (u < ue) {
+                        float l[V];
+                        lp_unpack(body[u], l, x);
+#pragma unroll
+                        for (int k = 0; k < V; k++) {
+                            const unsigned long long key = lp_key(l[k], head + u * V + k);
+                            best = key > best ? key : best;
+                        }
+                    }
+                }
+                cand[i] = best;
+            }
+            settle();
+            known = count;
+            over = 0;
+        };
+        for (int r = 0; r < round; r++) {
+            if (ub + r * per_round + t < ue && !(batch_max[r * NT + t] < thr_value))
+                append((unsigned long long)lp_order(batch_max[r * NT + t]) << 32 | (unsigned)(r * NT + t));
+            if (r % kEvery == kEvery - 1)
+                if (__syncthreads_or(over)) look();
+        }
+        // Nearly always the maxima alone decide: all batches that reach the top-th maximum, if they are few enough.  Otherwise
+        // (ties without end, or nothing above -inf) their best values' indices do.
+        __syncthreads();
+        const int found = count < kLpKeys ? count : kLpKeys;
+        int batches = found;
+        if (known == 0) {
+            settle();
+            if (found >= A.top) {
+                const unsigned least = (unsigned)(thr_key >> 32);
+                batches = kLpKeys;
+                __syncthreads();
+                if (thr_value > -INFINITY) {
+                    int mine = 0;
+                    for (int i = t; i < found; i += NT) mine += (unsigned)(cand[i] >> 32) >= least;
+                    if (t == 0) count = 0;
+                    __syncthreads();
+                    if (mine) atomicAdd(&count, mine);
+                    __syncthreads();
+                    batches = count;
+                }
+                if (t == 0) thr_key = ((unsigned long long)least << 32) - 1;
+            }
+        }
+        if (known == 0 && batches * kLpRound + 2 * V <= kLpKeys) {
+            for (int i = t; i < batches; i += NT) batch_s[i] = (unsigned)cand[i];
+        } else {
+            if (known == 0) {   // the entries again, all of them
+                __syncthreads();
+                if (t == 0) count = found;
+                __syncthreads();
+            }
+            look();
+            batches = known;
+            for (int i = t; i < batches; i += NT) {
+                const int u = ((int)~(unsigned)cand[i] - head) / V - ub, r = u / per_round;
+                batch_s[i] = r * NT + (u - r * per_round) % NT;
+            }
+            if (t == 0 && thr_key) thr_key--;   // the threshold itself counts too
+        }
+        // the values of these batches (and those outside the units) that reach the threshold
+        __syncthreads();
+        if (t == 0) count = 0;
+        __syncthreads();
+        for (int i = t; i < batches * kLpRound; i += NT) {
+            const int b = (int)batch_s[i / kLpRound], at = ub + b / NT * per_round + b % NT + (i % kLpRound) / V * NT;
+            if (at < ue) {
+                const int e = head + at * V + i % V;
+                push(lp_key(lp_load(x + e), e));
+            }
+        }
+        if (z == 0 && t < rest) {
+            const int e = t < head ? t : units * V + t;
+            push(lp_key(lp_load(x + e), e));
+        }
+        settle();
+    } else {
+        __syncthreads();
+    }
     if (t == 0) {
         s = warp_stats[0];
         for (int w = 1; w < NT / 32; w++) s = lp_merge(s, warp_stats[w]);
@@ -288,21 +423,21 @@ __global__ void __launch_bounds__(NT) k_logprobs(LpArgs A, int splits) {
                 s = lp_merge(s, b);
             }
             // a row without a value above -inf, and one with NaN or +inf, has no distribution
-            const float log_s = s.s1 > 0.f ? logf(s.s1) : NAN;
+            const float log_s = s.s1 > 0.f ? log2f(s.s1) : NAN;
             lse_s[0] = s.m;
             lse_s[1] = log_s;
             if (A.logprob) {
                 const int tok = A.tokens[row];
                 float lp = 0.f;   // LEV_NO_TOKEN
                 if (tok >= 0 && tok < A.n) {
-                    lp = (lp_value<CAP>(A, lp_load(x + tok)) - s.m) - log_s;
+                    lp = kLn2 * (lp_value<CAP>(A, lp_load(x + tok), s.m) - log_s);
                 } else if (tok != LEV_NO_TOKEN) {
                     atomicOr(A.status, LEV_DEV_BAD_INDEX);
                     lp = NAN;
                 }
                 A.logprob[row] = lp;
             }
-            if (A.entropy) A.entropy[row] = log_s - s.s2 / s.s1;
+            if (A.entropy) A.entropy[row] = kLn2 * (log_s - s.s2 / s.s1);
         }
         if (A.top) {
             const int total = splits * A.top, P = lp_pow2(total);
@@ -313,12 +448,15 @@ __global__ void __launch_bounds__(NT) k_logprobs(LpArgs A, int splits) {
                 cand[i] = k;
             }
             __syncthreads();
-            if (splits > 1) lp_sort<NT>(cand, P);
+            if (splits > 1) {
+                if (total <= kLpCount) lp_sort_few<NT>(cand, total, 0, sorted_s);
+                else lp_sort<NT>(cand, P);
+            }
             for (int i = t; i < A.top; i += NT) {
                 const unsigned long long k = cand[i];
                 const float l = lp_from_order((unsigned)(k >> 32));
                 A.top_index[row * A.top + i] = (int32_t)~(unsigned)k;
-                A.top_logprob[row * A.top + i] = (lp_value<CAP>(A, l) - lse_s[0]) - lse_s[1];
+                A.top_logprob[row * A.top + i] = kLn2 * (lp_value<CAP>(A, l, lse_s[0]) - lse_s[1]);
             }
         }
     }
@@ -327,9 +465,17 @@ __global__ void __launch_bounds__(NT) k_logprobs(LpArgs A, int splits) {
 
 template <typename T, int NT, bool CAP>
 int lp_launch(lev_ctx* ctx, const LpArgs& A, int64_t rows, int splits) {
+    const int64_t per = (A.n + splits - 1) / splits + kLpRound, rounds = (per + NT * kLpRound - 1) / (NT * kLpRound);
+    const size_t smem = A.top ? (size_t)rounds * NT * sizeof(float) : 0;
+    static size_t configured[16] = {};   // the most that a launch may ask for so far
+    if (smem > configured[ctx->device & 15]) {
+        LEV_CUDA(ctx, cudaFuncSetAttribute(k_logprobs<T, NT, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        configured[ctx->device & 15] = 160 * 1024;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * splits));
     cfg.blockDim = dim3(NT);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -349,10 +495,10 @@ int lp_run(lev_ctx* ctx, const LpArgs& A, int64_t rows, int splits) {
     LpArgs B = A;
     if (rows * splits < ctx->prop.multiProcessorCount) {   // few blocks: wide ones, so that a row's loads are in flight together
         B.group = A.top <= 32 ? 32 : 16;                   // 32 or 64 groups
-        return A.cap > 0.f ? lp_launch<T, 1024, true>(ctx, B, rows, splits) : lp_launch<T, 1024, false>(ctx, B, rows, splits);
+        return A.cap2 > 0.f ? lp_launch<T, 1024, true>(ctx, B, rows, splits) : lp_launch<T, 1024, false>(ctx, B, rows, splits);
     }
     B.group = A.top <= 8 ? 32 : A.top <= 32 ? 8 : 4;       // 8, 32 or 64 groups
-    return A.cap > 0.f ? lp_launch<T, 256, true>(ctx, B, rows, splits) : lp_launch<T, 256, false>(ctx, B, rows, splits);
+    return A.cap2 > 0.f ? lp_launch<T, 256, true>(ctx, B, rows, splits) : lp_launch<T, 256, false>(ctx, B, rows, splits);
 }
 
 }  // namespace
@@ -364,7 +510,7 @@ extern "C" int lev_logprobs(lev_ctx* ctx, const void* logits, int type, int64_t 
     if (rows < 1 || rows > (1 << 24) || n < 1 || n > LEV_MAX_DIM || ld < n || ld > (int64_t)1 << 31)
         return lev_fail(ctx, LEV_BAD_DIMENSIONS, "%lld rows of %lld logits, %lld apart", (long long)rows, (long long)n, (long long)ld);
     if (top < 0 || top > LEV_MAX_TOP_K || top > n) return lev_fail(ctx, LEV_BAD_DIMENSIONS, "%d alternatives of %lld logits (at most %d)", top, (long long)n, LEV_MAX_TOP_K);
-    if (!(cap >= 0.f) || !isfinite(cap)) return lev_fail(ctx, LEV_BAD_ARGUMENT, "cap %g", (double)cap);
+    if (!(cap >= 0.f) || !isfinite(cap * kLog2e) || (cap > 0.f && !isfinite(2.f * kLog2e / cap))) return lev_fail(ctx, LEV_BAD_ARGUMENT, "cap %g", (double)cap);
     const size_t size = type == LEV_ELEM_F32 ? 4 : 2;
     if ((uintptr_t)logits % size != 0) return lev_fail(ctx, LEV_BAD_ARGUMENT, "logits are not aligned to their type");
     if (!logprob && !entropy && top == 0) return lev_fail(ctx, LEV_BAD_ARGUMENT, "nothing is asked for");
@@ -374,15 +520,18 @@ extern "C" int lev_logprobs(lev_ctx* ctx, const void* logits, int type, int64_t 
     A.n = n;
     A.ld = ld;
     A.tokens = tokens;
-    A.cap = cap;
-    A.cap_k = cap > 0.f ? -2.f * kLog2e / cap : 0.f;
+    A.cap_k = cap > 0.f ? 2.f * kLog2e / cap : 0.f;
+    A.cap2 = cap * kLog2e;
     A.top = top;
+    A.keep = 3 * LEV_MAX_TOP_K;
     A.logprob = logprob;
     A.entropy = entropy;
     A.top_index = top_index;
     A.top_logprob = top_logprob;
     A.status = ctx->d_status;
+    // four blocks per SM or 128 K logits per block (whose batch maxima take 32 KB), whichever asks for more
     int splits = 1;
+    while (splits < 8 && n / splits > 1 << 17) splits *= 2;
     while (splits < 8 && rows * splits < 4 * (int64_t)ctx->prop.multiProcessorCount && n / (2 * splits) >= 4096) splits *= 2;
     if (type == LEV_ELEM_F32) return lp_run<float>(ctx, A, rows, splits);
     if (type == LEV_ELEM_F16) return lp_run<__half>(ctx, A, rows, splits);

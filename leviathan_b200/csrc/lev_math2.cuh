@@ -1,0 +1,49 @@
+// Arithmetic that the softmax kernels share (lev_attn_tc.cu, lev_logprobs.cu): two f32 operations per instruction, each
+// rounded as on its own, the hardware's power of two and maxima of three.
+#pragma once
+#include <cuda_runtime.h>
+
+namespace {
+
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 two(float lo, float hi) {
+    f32x2 v;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+__device__ __forceinline__ f32x2 twice(float v) { return two(v, v); }
+__device__ __forceinline__ void both(f32x2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma_2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+__device__ __forceinline__ f32x2 add_2(f32x2 a, f32x2 b) {
+    f32x2 v;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ f32x2 mul_2(f32x2 a, f32x2 b) {
+    f32x2 v;
+    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+// 2^x, relative error 2^-22 (the rounding of x comes on top), 0 for -inf
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+// 1 / x, relative error 2^-23, 0 for inf
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+// a NaN among the three is passed over
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+}  // namespace

@@ -316,35 +316,6 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
     const unsigned rank = in_cluster % CG, lead = in_cluster - rank;
     const int kvh = blockIdx.y, split = (int)in_cluster / CG, unit = (int)blockIdx.x / (CG * A.splits);
     const int per = A.tpt * TILES * CG;
-    pdl_wait();
-    pdl_launch_dependents();
-    TcUnit U;
-    if (!tc_find(A, unit, per, lane, &U)) return;   // the same answer in every CTA of the unit
-    U.ok = 1;
-    U.pos0 = 0;
-    U.slot = 0;
-    if (A.table) {
-        U.slot = A.slot[U.seq];
-        U.pos0 = A.pos[U.seq];
-        U.ok = U.slot >= 0 && U.slot < A.slots && U.pos0 >= 0 && (int64_t)U.pos0 + U.len <= (int64_t)A.max_blocks * A.page;
-    }
-    const int tokens = U.len - U.t0 < per ? U.len - U.t0 : per;   // of the unit
-    if (!U.ok) {   // nothing is followed: the rows are NaN
-        if (threadIdx.x == 0 && rank == 0 && split == 0) atomicOr(A.status, LEV_DEV_BAD_INDEX);
-        if (rank == 0 && split == 0)
-            for (int i = threadIdx.x; i < tokens * A.group * HD; i += blockDim.x) {
-                const int r = i / HD, tok = r / A.group;
-                tc_store16(A, (int64_t)(U.row0 + U.t0 + tok) * A.out_ld + (int64_t)(kvh * A.group + r - tok * A.group) * HD + (i - r * HD), NAN);
-            }
-        return;
-    }
-    // positions of the unit: its first row's lowest to its last row's own
-    const int p_first = U.pos0 + U.t0, p_last = p_first + tokens - 1;
-    const int lo_unit = A.window > 0 && p_first + 1 > A.window ? p_first + 1 - A.window : 0;
-    const int j_all = lo_unit / TC_KV, n_all = p_last / TC_KV - j_all + 1;
-    const int jb = j_all + (int)((int64_t)n_all * split / A.splits), je = j_all + (int)((int64_t)n_all * (split + 1) / A.splits);
-    const int n = je - jb;
-
     const unsigned smem = (smem_u32(smem_dyn) + 1023u) & ~1023u;
     const unsigned ring = smem + TILES * D::kQTile;
     const int tma = A.box_k > 0;
@@ -373,6 +344,36 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
         }
     }
+    pdl_wait();
+    pdl_launch_dependents();
+    TcUnit U;
+    const bool found = tc_find(A, unit, per, lane, &U);   // the same answer in every CTA of the unit
+    if (!found) U = TcUnit{0, 0, 0, 0, 0, 0, 0};
+    U.ok = 1;
+    U.pos0 = 0;
+    U.slot = 0;
+    if (found && A.table) {
+        U.slot = A.slot[U.seq];
+        U.pos0 = A.pos[U.seq];
+        U.ok = U.slot >= 0 && U.slot < A.slots && U.pos0 >= 0 && (int64_t)U.pos0 + U.len <= (int64_t)A.max_blocks * A.page;
+    }
+    int tokens = U.len - U.t0 < per ? U.len - U.t0 : per;   // of the unit
+    if (found && !U.ok) {   // nothing is followed: the rows are NaN
+        if (threadIdx.x == 0 && rank == 0 && split == 0) atomicOr(A.status, LEV_DEV_BAD_INDEX);
+        if (rank == 0 && split == 0)
+            for (int i = threadIdx.x; i < tokens * A.group * HD; i += blockDim.x) {
+                const int r = i / HD, tok = r / A.group;
+                tc_store16(A, (int64_t)(U.row0 + U.t0 + tok) * A.out_ld + (int64_t)(kvh * A.group + r - tok * A.group) * HD + (i - r * HD), NAN);
+            }
+    }
+    if (!U.ok) tokens = 0;
+    // positions of the unit: its first row's lowest to its last row's own
+    const int p_first = U.pos0 + U.t0, p_last = p_first + tokens - 1;
+    const int lo_unit = A.window > 0 && p_first + 1 > A.window ? p_first + 1 - A.window : 0;
+    const int j_all = lo_unit / TC_KV, n_all = p_last / TC_KV - j_all + 1;
+    const int jb = j_all + (int)((int64_t)n_all * split / A.splits), je = j_all + (int)((int64_t)n_all * (split + 1) / A.splits);
+    const int n = found && U.ok ? je - jb : 0;
+
     tc_before();
     __syncthreads();
     if (CG == 2) cluster_sync_all();
@@ -468,9 +469,8 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
 #pragma unroll
             for (int c = 0; c < 128; c += 8)
 #pragma unroll
-                for (int q = 0; q < 4; q++)
-                    mx[q] = fmaxf(mx[q], fmaxf(__uint_as_float(s[c + 2 * q]), __uint_as_float(s[c + 2 * q + 1])));
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                for (int q = 0; q < 4; q++) mx[q] = max3(mx[q], __uint_as_float(s[c + 2 * q]), __uint_as_float(s[c + 2 * q + 1]));
+            const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
             // the reference follows when the maximum has run away from it
             float corr = 1.f;
             if (top > m && (i == 0 || m == -INFINITY || (top - m) * A.sl > TC_LAZY)) {
@@ -507,10 +507,15 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
 #pragma unroll
                 for (int c = 0; c < 32; c++) {
                     float a, b;
+                    f32x2 e;
                     both(fma_2(two(__uint_as_float(s[64 * h + 2 * c]), __uint_as_float(s[64 * h + 2 * c + 1])), sl2, neg2), a, b);
-                    a = ex2(a);
-                    b = ex2(b);
-                    const f32x2 e = two(a, b);
+                    if (c % 4 == 1) {   // a quarter on the multiply-add units
+                        both(exp2_cubic(two(max_nan(a, -126.f), max_nan(b, -126.f))), a, b);
+                    } else {
+                        a = ex2(a);
+                        b = ex2(b);
+                    }
+                    e = two(a, b);
                     if (c & 1) part = add_2(part, e);
                     else sum = add_2(sum, e);
                     pk[c] = pack16(a, b, A.mma_type);
@@ -543,7 +548,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         float probe = 0.f;   // NaN when a sum is not finite
         float* part_o = reinterpret_cast<float*>(base) + tile * 128 * HD;   // splits: [row][HD], 16-byte pieces swizzled
         if (n > 0) {
-#pragma unroll 1
+#pragma unroll 2
             for (int c = 0; c < HD; c += 32) {
                 unsigned o[32];
                 tmem_ld32(o_addr + c, o);

@@ -27,6 +27,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "lev_math2.cuh"
 #include "lev_stream.h"
 #include "lev_umma.cuh"
@@ -43,7 +45,7 @@ enum { TC_F32 = LEV_ELEM_F32, TC_F16 = LEV_ELEM_F16, TC_BF16 = LEV_ELEM_BF16 };
 struct TcArgs {
     const void* q;
     int64_t q_ld;
-    int q_type, mma_type, out_type, kv_type;   // LEV_ELEM_*; mma_type: what the tensor core multiplies
+    int q_type, out_type, kv_type;   // LEV_ELEM_*
     void* out;
     int64_t out_ld;
     const int32_t *start, *slot, *pos, *table; // table NULL: packed prompts, positions count from start[]
@@ -53,7 +55,7 @@ struct TcArgs {
     int seqs, q_heads, kv_heads, group, tpt;   // tpt: tokens of a 128-row tile
     int page, max_blocks, slots;
     int box_k, box_v;                          // rows of a TMA box; 0: rows are copied by warps
-    int window, splits, negate;
+    int window, splits, negate, q_boxes;       // q_boxes: the queries come by TMA
     float sl;                                  // |scale| * log2(e)
     int* status;
 };
@@ -74,6 +76,18 @@ __device__ __forceinline__ void tmem_st32(unsigned a, const unsigned* v) {
         "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]),
         "r"(v[31])
         : "memory");
+}
+// of two pieces each of a pair of lanes (lanes that differ in `bit`): the lower lane ends with both lanes' a, the upper with both b
+__device__ __forceinline__ void swap_pieces(uint4& a, uint4& b, int bit, int lane) {
+    const bool up = lane & bit;
+    const uint4 send = up ? a : b;
+    uint4 got;
+    got.x = __shfl_xor_sync(0xffffffffu, send.x, bit);
+    got.y = __shfl_xor_sync(0xffffffffu, send.y, bit);
+    got.z = __shfl_xor_sync(0xffffffffu, send.z, bit);
+    got.w = __shfl_xor_sync(0xffffffffu, send.w, bit);
+    if (up) a = got;
+    else b = got;
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
@@ -163,19 +177,23 @@ __device__ __forceinline__ void tc_box_page(unsigned dst, const CUtensorMap* map
 struct TcUnit {
     int seq, t0, len;   // sequence, first token of the unit, tokens of the sequence
     int row0;           // first row of the sequence
-    int pos0;           // position of its first token
-    int slot;
+    int kvh, slot;
     int ok;             // slot and positions inside the layout
+    int tokens;         // of the unit
+    int p_first, lo;    // position of its first row, lowest position that the unit attends to
+    int jb, n;          // steps of 128 positions: the first one of this CTA's split and how many
+    __device__ __forceinline__ int p_last() const { return p_first + tokens - 1; }
 };
 
-// unit u of all sequences' units (each sequence has ceil(tokens / per), the last tokens first: they attend to most).
-// One warp; false when there are fewer units.  A pair of start[] entries that is no range counts as an empty sequence.
+// Unit u of all sequences' units (each sequence has ceil(tokens / per)), those with most work first: of every 32 sequences the ones
+// with the longest context, of a sequence its last tokens.  One warp; false when there are fewer units.  A pair of start[] entries
+// that is no range counts as an empty sequence.
 __device__ bool tc_find(const TcArgs& A, int u, int per, int lane, TcUnit* U) {
     int before = 0;
     bool found = false;
     for (int s0 = 0; s0 < A.seqs && (!found || u == 0); s0 += 32) {   // the first unit looks all of start[] over
         const int s = s0 + lane;
-        int a = 0, n = 0;
+        int a = 0, n = 0, context = -1;
         if (s < A.seqs) {
             a = A.start[s];
             const int b = A.start[s + 1];
@@ -184,6 +202,22 @@ __device__ bool tc_find(const TcArgs& A, int u, int per, int lane, TcUnit* U) {
             } else {
                 n = b - a;
             }
+            context = A.table ? A.pos[s] : 0;
+            context = n == 0 || context < 0 || context > (1 << 30) ? 0 : context + n;
+        }
+        // a lane takes the sequence whose rank is its number
+        int rank = 0, from = 0;
+        if (A.seqs > 1) {
+#pragma unroll
+            for (int l = 0; l < 32; l++) {
+                const int c = __shfl_sync(0xffffffffu, context, l);
+                rank += c > context || (c == context && l < lane);
+            }
+#pragma unroll
+            for (int l = 0; l < 32; l++)
+                if (__shfl_sync(0xffffffffu, rank, l) == lane) from = l;
+            a = __shfl_sync(0xffffffffu, a, from);
+            n = __shfl_sync(0xffffffffu, n, from);
         }
         const int units = (n + per - 1) / per;
         int scan = units;
@@ -196,7 +230,7 @@ __device__ bool tc_find(const TcArgs& A, int u, int per, int lane, TcUnit* U) {
         if (has && !found) {
             const int l = __ffs(has) - 1;
             const int mine = u - before - (scan - units);   // of lane l: the unit's number inside its sequence
-            U->seq = s0 + l;
+            U->seq = s0 + __shfl_sync(0xffffffffu, from, l);
             U->t0 = __shfl_sync(0xffffffffu, (units - 1 - mine) * per, l);
             U->len = __shfl_sync(0xffffffffu, n, l);
             U->row0 = __shfl_sync(0xffffffffu, a, l);
@@ -215,14 +249,41 @@ __device__ __forceinline__ TcLayout tc_layout(const TcArgs& A, int rows, int col
     return L;
 }
 
+// All of unit `id` (KV heads fastest: the units with most work come first) for the CTA of split `split`; a whole warp.
+// False: there is no such unit.
+__device__ bool tc_unit(const TcArgs& A, int id, int per, int split, int lane, TcUnit* U) {
+    U->kvh = id % A.kv_heads;
+    if (!tc_find(A, id / A.kv_heads, per, lane, U)) return false;
+    int pos0 = 0;
+    U->slot = 0;
+    U->ok = 1;
+    if (A.table) {
+        U->slot = A.slot[U->seq];
+        pos0 = A.pos[U->seq];
+        U->ok = U->slot >= 0 && U->slot < A.slots && pos0 >= 0 && (int64_t)pos0 + U->len <= (int64_t)A.max_blocks * A.page;
+        if (!U->ok && lane == 0) atomicOr(A.status, LEV_DEV_BAD_INDEX);
+    }
+    U->tokens = U->len - U->t0 < per ? U->len - U->t0 : per;
+    U->p_first = pos0 + U->t0;
+    U->lo = A.window > 0 && U->p_first + 1 > A.window ? U->p_first + 1 - A.window : 0;
+    if (!U->ok) {   // nothing is followed: the rows are NaN
+        U->p_first = U->lo = U->jb = U->n = 0;
+        return true;
+    }
+    const int first = U->lo / TC_KV, all = U->p_last() / TC_KV - first + 1;
+    U->jb = first + (int)((int64_t)all * split / A.splits);
+    U->n = first + (int)((int64_t)all * (split + 1) / A.splits) - U->jb;
+    return true;
+}
+
 // element address of position p of this unit's KV head; NULL for a table entry outside the pool
-__device__ __forceinline__ const unsigned char* tc_row(const TcArgs& A, const TcUnit& U, int kvh, int hd, int p, bool is_v) {
+__device__ __forceinline__ const unsigned char* tc_row(const TcArgs& A, const TcUnit& U, int hd, int p, bool is_v) {
     const int size = A.kv_type == TC_F32 ? 4 : 2;
     const unsigned char* base = static_cast<const unsigned char*>(is_v ? A.v : A.k);
-    if (!A.table) return base + ((int64_t)(U.row0 + p) * (is_v ? A.v_ld : A.k_ld) + (int64_t)kvh * hd) * size;
+    if (!A.table) return base + ((int64_t)(U.row0 + p) * (is_v ? A.v_ld : A.k_ld) + (int64_t)U.kvh * hd) * size;
     const int pg = p / A.page, e = A.table[(int64_t)U.slot * A.max_blocks + pg];
     if (e < 0 || e >= A.blocks) return nullptr;
-    return base + LEV_KV_ROW(e, p - pg * A.page, kvh, A.page, A.kv_heads) * (int64_t)hd * size;
+    return base + LEV_KV_ROW(e, p - pg * A.page, U.kvh, A.page, A.kv_heads) * (int64_t)hd * size;
 }
 __device__ __forceinline__ float tc_value(const unsigned char* row, int i, int kv_type) {
     if (kv_type == TC_F32) return __half2float(__float2half_rn(reinterpret_cast<const float*>(row)[i]));
@@ -243,24 +304,21 @@ __device__ __forceinline__ void tc_store16(const TcArgs& A, int64_t at, float x)
 }
 
 // One row again, position by position over [lo, hi): for rows whose sums met a non-finite value where they do not attend.
-// 128 threads of the tile's warpgroup; scratch: HD + 128 floats.  Returns thread t's dims t (and t + 128) unnormalised.
+// 128 threads of the tile's warpgroup; ws: 128 floats.  Returns thread t's dims t (and t + 128) unnormalised.
 template <int HD>
-__device__ void tc_row_again(const TcArgs& A, const TcUnit& U, int kvh, int64_t q_at, int lo, int hi, int t, int bar, float* scratch,
-                             float* o, float* m_out, float* l_out) {
-    float *qs = scratch, *ws = scratch + HD;
-    wg_sync(bar);
-    for (int i = t; i < HD; i += 128) qs[i] = tc_query(A, q_at + i);
+__device__ void tc_row_again(const TcArgs& A, const TcUnit& U, int64_t q_at, int lo, int hi, int t, int bar, float* ws, float* o, float* m_out,
+                             float* l_out) {
     float m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int i = 0; i < HD / 128; i++) o[i] = 0.f;
     for (int b = lo; b < hi; b += 128) {
-        wg_sync(bar);   // qs is written; the weights of the step before are read
+        wg_sync(bar);   // the weights of the step before are read
         float s = -INFINITY;
         if (b + t < hi) {
-            const unsigned char* row = tc_row(A, U, kvh, HD, b + t, false);
+            const unsigned char* row = tc_row(A, U, HD, b + t, false);
             s = row ? 0.f : NAN;
             if (row)
-                for (int i = 0; i < HD; i++) s = fmaf(qs[i], tc_value(row, i, A.kv_type), s);
+                for (int i = 0; i < HD; i++) s = fmaf(tc_query(A, q_at + i), tc_value(row, i, A.kv_type), s);
         }
         ws[t] = s;
         wg_sync(bar);
@@ -275,13 +333,80 @@ __device__ void tc_row_again(const TcArgs& A, const TcUnit& U, int kvh, int64_t 
         for (int j = 0; j < n; j++) {
             const float w = ex2((ws[j] - ref) * A.sl);
             l += w;
-            const unsigned char* row = tc_row(A, U, kvh, HD, b + j, true);
+            const unsigned char* row = tc_row(A, U, HD, b + j, true);
 #pragma unroll
             for (int i = 0; i < HD / 128; i++) o[i] = fmaf(w, row ? tc_value(row, t + 128 * i, A.kv_type) : NAN, o[i]);
         }
     }
     *m_out = m;
     *l_out = l;
+}
+
+// The queries of `tiles` 128-row tiles, rounded to 16 bits, to the swizzled K-major tiles at `smem`, by `warps` warps of which
+// this one is number `me`.  BATCH rows are requested before the first is stored.
+template <int HD, int BATCH>
+__device__ __forceinline__ void tc_load_q(const TcArgs& A, const TcUnit& U, unsigned smem, int first_tok, int tiles, int me, int warps, int lane) {
+    constexpr int kPieces = HD / 8, kRows = 32 / kPieces;   // 16-byte pieces of a row; rows of a warp's step
+    const int piece = lane % kPieces, sub = lane / kPieces, rows = tiles * 128;
+    auto source = [&](int r) -> int64_t {   // element offset of this lane's piece; negative: no such row
+        const int rr = r & 127, tok = rr / A.group, at = first_tok + (r >> 7) * A.tpt + tok;
+        if (r >= rows || tok >= A.tpt || at >= U.tokens) return -1;
+        return (int64_t)(U.row0 + U.t0 + at) * A.q_ld + (int64_t)(U.kvh * A.group + rr - tok * A.group) * HD + piece * 8;
+    };
+    auto put = [&](int r, uint4 v) {
+        if (r >= rows) return;
+        if (A.negate) v = make_uint4(v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
+        const unsigned dst = smem + (unsigned)(r >> 7) * (128u * HD * 2) + (unsigned)(piece >> 3) * 16384u + (unsigned)(r & 127) * 128u +
+                             (unsigned)(((piece & 7) ^ (r & 7)) << 4);
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+    };
+    const int step = warps * kRows;
+#pragma unroll 1
+    for (int r0 = me * kRows + sub; r0 < rows + sub; r0 += BATCH * step) {
+        if (A.q_type == TC_F32) {
+            float4 a[BATCH], b[BATCH];
+#pragma unroll
+            for (int k = 0; k < BATCH; k++) {
+                const int64_t at = source(r0 + k * step);
+                const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(A.q) + at);
+                a[k] = at >= 0 ? src[0] : make_float4(0.f, 0.f, 0.f, 0.f);
+                b[k] = at >= 0 ? src[1] : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int k = 0; k < BATCH; k++)
+                put(r0 + k * step, make_uint4(pack16(a[k].x, a[k].y, TC_F16), pack16(a[k].z, a[k].w, TC_F16), pack16(b[k].x, b[k].y, TC_F16),
+                                              pack16(b[k].z, b[k].w, TC_F16)));
+        } else {
+            uint4 v[BATCH];
+#pragma unroll
+            for (int k = 0; k < BATCH; k++) {
+                const int64_t at = source(r0 + k * step);
+                v[k] = at >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(A.q) + at) : make_uint4(0u, 0u, 0u, 0u);
+            }
+#pragma unroll
+            for (int k = 0; k < BATCH; k++) put(r0 + k * step, v[k]);
+        }
+    }
+    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");   // the tensor core reads through the async proxy
+    __syncwarp();
+}
+
+// The hardware hands a running cluster the next one of the grid that has not started: `request` asks (the answer, 16 bytes, arrives
+// at `bar`), `taken` reads it: the first CTA's index in x, or -1 when all have started.  Not to be asked again after that.
+__device__ __forceinline__ void tc_next_request(unsigned answer, unsigned bar) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], 16;\n" ::"r"(bar) : "memory");
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];\n" ::"r"(answer), "r"(bar) : "memory");
+}
+__device__ __forceinline__ int tc_next_taken(unsigned answer) {
+    int ok, x;
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b128 a;\n ld.shared.b128 a, [%2];\n"
+        " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n selp.s32 %0, 1, 0, p;\n mov.s32 %1, 0;\n"
+        " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, a;\n}\n"
+        : "=r"(ok), "=r"(x)
+        : "r"(answer)
+        : "memory");
+    return ok ? x : -1;
 }
 
 template <int HD, int TILES>
@@ -295,33 +420,38 @@ struct TcDims {
     static constexpr size_t kSmem = 1024 + TILES * kQTile + (size_t)kStages * TC_STAGE;
 };
 
-// HD: head dimension.  TILES: 128-row tiles of a CTA, each with a softmax warpgroup; one tile has two S buffers, two
+// HD: head dimension.  TYPE: what the tensor core multiplies (LEV_ELEM_F16 or LEV_ELEM_BF16).  TILES: 128-row tiles of a CTA, each with a softmax warpgroup; one tile has two S buffers, two
 // tiles have one each.  CG = 2: a pair of CTAs (cta_group::2) with one tile each that share K and V.  splits > 1: the
 // CTAs of a cluster take parts of the positions and merge through distributed shared memory.
-template <int HD, int TILES, int CG>
+template <int HD, int TILES, int CG, int TYPE>
 __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
-    k_attn_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ TcArgs A) {
+    k_attn_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap,
+              const __grid_constant__ TcArgs A) {
     using D = TcDims<HD, TILES>;
     constexpr int NS = D::kStages;
     constexpr int KV_STAGES = CG == 2 ? 1 : HD / 128;   // stages of a K (or V) tile of this CTA
     constexpr int O_COL = 256;                          // tensor memory: S slots at 0 and 128, then O
     extern __shared__ unsigned char smem_dyn[];
-    __shared__ __align__(8) unsigned long long full[NS], empty[NS], s_full[2], p_full[2], pv_done[2], q_full;
+    __shared__ __align__(8) unsigned long long full[NS], empty[NS], s_full[2], p_full[2], pv_done[2], q_first, q_full, q_empty;
+    __shared__ __align__(8) unsigned long long unit_full[2], unit_empty[2], answer_bar, told_bar[2];
+    __shared__ __align__(16) unsigned answer_s[4];
     __shared__ unsigned tmem_base_s;
-    __shared__ int abort_s, bad_s;
+    __shared__ int abort_s, bad_s[2], told_s[2];
+    __shared__ TcUnit unit_s[2];
     __shared__ unsigned again_s[TILES * 4];
+    __shared__ float again_w[TILES][128];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // a cluster is a unit: the pair (one CTA without pairs) of split 0, then that of split 1, ...
-    const unsigned in_cluster = (int)blockIdx.x % (CG * A.splits);
+    const int cluster = CG * A.splits;
+    const unsigned in_cluster = (int)blockIdx.x % cluster;
     const unsigned rank = in_cluster % CG, lead = in_cluster - rank;
-    const int kvh = blockIdx.y, split = (int)in_cluster / CG, unit = (int)blockIdx.x / (CG * A.splits);
-    const int per = A.tpt * TILES * CG;
+    const int split = (int)in_cluster / CG, per = A.tpt * TILES * CG;
     const unsigned smem = (smem_u32(smem_dyn) + 1023u) & ~1023u;
     const unsigned ring = smem + TILES * D::kQTile;
     const int tma = A.box_k > 0;
     if (threadIdx.x == 0) {
         abort_s = 0;
-        bad_s = 0;
+        bad_s[0] = bad_s[1] = 0;
         for (int s = 0; s < NS; s++) {
             mbar_init(smem_u32(&full[s]), tma ? 1 : TC_LOAD_WARPS);
             mbar_init(smem_u32(&empty[s]), 1);
@@ -330,8 +460,14 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
             mbar_init(smem_u32(&s_full[s]), 1);
             mbar_init(smem_u32(&p_full[s]), 4 * CG);
             mbar_init(smem_u32(&pv_done[s]), 1);
+            mbar_init(smem_u32(&unit_full[s]), 1);
+            mbar_init(smem_u32(&unit_empty[s]), 4 * TILES + TC_LOAD_WARPS);   // softmax and MMA warps, the other loading warps
+            mbar_init(smem_u32(&told_bar[s]), 1);
         }
-        mbar_init(smem_u32(&q_full), 4 * TILES * CG);
+        mbar_init(smem_u32(&q_full), A.q_boxes ? 1 : TC_LOAD_WARPS * CG);
+        mbar_init(smem_u32(&q_first), 4 * TILES * CG);   // without boxes: the softmax warps load the first unit's queries
+        mbar_init(smem_u32(&q_empty), 1);
+        mbar_init(smem_u32(&answer_bar), 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
     }
@@ -346,40 +482,28 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
     }
     pdl_wait();
     pdl_launch_dependents();
-    TcUnit U;
-    const bool found = tc_find(A, unit, per, lane, &U);   // the same answer in every CTA of the unit
-    if (!found) U = TcUnit{0, 0, 0, 0, 0, 0, 0};
-    U.ok = 1;
-    U.pos0 = 0;
-    U.slot = 0;
-    if (found && A.table) {
-        U.slot = A.slot[U.seq];
-        U.pos0 = A.pos[U.seq];
-        U.ok = U.slot >= 0 && U.slot < A.slots && U.pos0 >= 0 && (int64_t)U.pos0 + U.len <= (int64_t)A.max_blocks * A.page;
-    }
-    int tokens = U.len - U.t0 < per ? U.len - U.t0 : per;   // of the unit
-    if (found && !U.ok) {   // nothing is followed: the rows are NaN
-        if (threadIdx.x == 0 && rank == 0 && split == 0) atomicOr(A.status, LEV_DEV_BAD_INDEX);
-        if (rank == 0 && split == 0)
-            for (int i = threadIdx.x; i < tokens * A.group * HD; i += blockDim.x) {
-                const int r = i / HD, tok = r / A.group;
-                tc_store16(A, (int64_t)(U.row0 + U.t0 + tok) * A.out_ld + (int64_t)(kvh * A.group + r - tok * A.group) * HD + (i - r * HD), NAN);
-            }
-    }
-    if (!U.ok) tokens = 0;
-    // positions of the unit: its first row's lowest to its last row's own
-    const int p_first = U.pos0 + U.t0, p_last = p_first + tokens - 1;
-    const int lo_unit = A.window > 0 && p_first + 1 > A.window ? p_first + 1 - A.window : 0;
-    const int j_all = lo_unit / TC_KV, n_all = p_last / TC_KV - j_all + 1;
-    const int jb = j_all + (int)((int64_t)n_all * split / A.splits), je = j_all + (int)((int64_t)n_all * (split + 1) / A.splits);
-    const int n = found && U.ok ? je - jb : 0;
-
+    TcUnit U;   // the first unit: the same answer in every warp and every CTA of the cluster
+    bool have = tc_unit(A, (int)blockIdx.x / cluster, per, split, lane, &U);
+    if (!have) U.tokens = 0;
+    const TcUnit U0 = U;
+    if (threadIdx.x == 0) unit_s[0] = U;
     tc_before();
     __syncthreads();
     if (CG == 2) cluster_sync_all();
     tc_after();
     const unsigned tmem = tmem_base_s;
     volatile int* abort_flag = &abort_s;
+    // Unit k (from 0) of this CTA is in unit_s[k & 1].  Ends unit k and goes on to the next one; false: there is none.
+    auto next_unit = [&](int k) {
+        if (A.splits > 1) return false;   // a cluster that merges has one unit
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&unit_empty[k & 1]));
+        k++;
+        pk_wait(smem_u32(&unit_full[k & 1]), ((k - 1) >> 1) & 1, abort_flag);
+        __syncwarp();
+        U = unit_s[k & 1];
+        return U.tokens > 0 && !*abort_flag;
+    };
     // splits: partial sums [tile][row][HD] where the queries and stages were, behind them 8 KB for one row's work or the
     // merge's weights, then a row's reference and sum
     unsigned char* const base = smem_dyn + (smem - smem_u32(smem_dyn));
@@ -390,66 +514,27 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         // ---- softmax: thread = row of the tile ----
         const int tile = warp >> 2, w4 = warp & 3, t = threadIdx.x & 127;
         const int tile_tok = (int)(rank * TILES + tile) * A.tpt;   // first token of the tile inside the unit
-        const int tok = t / A.group, head = kvh * A.group + t - tok * A.group;
-        const bool live = tok < A.tpt && tile_tok + tok < tokens;
-        {   // the tile's queries, rounded to 16 bits, in the swizzled K-major layout
-            const unsigned qs = smem + (unsigned)tile * D::kQTile;
-            constexpr int kPieces = HD / 8, kRows = 32 / kPieces;   // 16-byte pieces of a row; rows of a warp's step
-            constexpr int kBatch = TILES == 2 ? 8 : 16;             // steps requested before the first is stored
-            const int piece = lane % kPieces, sub = lane / kPieces;
-            auto row_at = [&](int r) -> int64_t {   // element offset of this lane's piece; negative: no such row
-                const int rt = r / A.group;
-                if (rt >= A.tpt || tile_tok + rt >= tokens) return -1;
-                return (int64_t)(U.row0 + U.t0 + tile_tok + rt) * A.q_ld + (int64_t)(kvh * A.group + r - rt * A.group) * HD + piece * 8;
-            };
-            auto put = [&](int r, uint4 v) {
-                if (A.negate) v = make_uint4(v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
-                const unsigned dst = qs + (unsigned)(piece >> 3) * 16384u + (unsigned)r * 128u + (unsigned)(((piece & 7) ^ (r & 7)) << 4);
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-            };
-#pragma unroll 1
-            for (int r0 = w4 * 32 + sub; r0 < w4 * 32 + 32; r0 += kRows * kBatch) {
-                if (A.q_type == TC_F32) {
-                    float4 a[kBatch], b[kBatch];
-#pragma unroll
-                    for (int i = 0; i < kBatch; i++) {
-                        const int64_t at = row_at(r0 + i * kRows);
-                        const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(A.q) + at);
-                        a[i] = at >= 0 ? src[0] : make_float4(0.f, 0.f, 0.f, 0.f);
-                        b[i] = at >= 0 ? src[1] : make_float4(0.f, 0.f, 0.f, 0.f);
-                    }
-#pragma unroll
-                    for (int i = 0; i < kBatch; i++)
-                        put(r0 + i * kRows, make_uint4(pack16(a[i].x, a[i].y, TC_F16), pack16(a[i].z, a[i].w, TC_F16), pack16(b[i].x, b[i].y, TC_F16),
-                                                       pack16(b[i].z, b[i].w, TC_F16)));
-                } else {
-                    uint4 v[kBatch];
-#pragma unroll
-                    for (int i = 0; i < kBatch; i++) {
-                        const int64_t at = row_at(r0 + i * kRows);
-                        v[i] = at >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(A.q) + at) : make_uint4(0u, 0u, 0u, 0u);
-                    }
-#pragma unroll
-                    for (int i = 0; i < kBatch; i++) put(r0 + i * kRows, v[i]);
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-            __syncwarp();
-            if (lane == 0) {
-                if (CG == 2) mbar_arrive_cluster(map_to_rank(smem_u32(&q_full), lead));
-                else mbar_arrive(smem_u32(&q_full));
-            }
-        }
-        const int p = p_first + tile_tok + tok;                     // this row's position
-        const int row_lo = A.window > 0 ? p + 1 - A.window : 0;     // and its first one (may be negative)
-        const int p_tile0 = p_first + tile_tok, p_tile1 = p_tile0 + A.tpt - 1;   // positions of the tile's rows
+        const int tok = t / A.group;
         const unsigned lane_base = tmem + ((unsigned)(w4 * 32) << 16);
         const unsigned o_addr = lane_base + O_COL + (TILES == 2 ? tile * 128 : 0);
+        const f32x2 sl2 = twice(A.sl);
+        if (have && !A.q_boxes) {
+            tc_load_q<HD, TILES == 2 ? 8 : 16>(A, U, smem, (int)rank * TILES * A.tpt, TILES, warp, 4 * TILES, lane);
+            if (lane == 0) {
+                if (CG == 2) mbar_arrive_cluster(map_to_rank(smem_u32(&q_first), lead));
+                else mbar_arrive(smem_u32(&q_first));
+            }
+        }
+        int g = 0;   // steps of all units so far
+        for (int k = 0; have; have = next_unit(k++)) {
+        const int n = U.n, jb = U.jb;
+        const int p = U.p_first + tile_tok + tok;                   // this row's position
+        const int row_lo = A.window > 0 ? p + 1 - A.window : 0;     // and its first one (may be negative)
+        const int p_tile0 = U.p_first + tile_tok, p_tile1 = p_tile0 + A.tpt - 1;   // positions of the tile's rows
         float m = -INFINITY;   // reference of the row's weights, in units of S
         f32x2 sum = two(0.f, 0.f);
-        const f32x2 sl2 = two(A.sl, A.sl);
-        for (int i = 0; i < n; i++) {
-            const int slot_i = TILES == 2 ? tile : i & 1, par = TILES == 2 ? i & 1 : (i >> 1) & 1;
+        for (int i = 0; i < n; i++, g++) {
+            const int slot_i = TILES == 2 ? tile : g & 1, par = TILES == 2 ? g & 1 : (g >> 1) & 1;
             const unsigned s_addr = lane_base + (unsigned)slot_i * 128u;
             pk_wait(smem_u32(&s_full[slot_i]), par, abort_flag);
             __syncwarp();
@@ -478,7 +563,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 m = top;
             }
             if (i > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
-                const int prev = TILES == 2 ? tile : (i - 1) & 1, ppar = TILES == 2 ? (i - 1) & 1 : ((i - 1) >> 1) & 1;
+                const int prev = TILES == 2 ? tile : (g - 1) & 1, ppar = TILES == 2 ? (g - 1) & 1 : ((g - 1) >> 1) & 1;
                 pk_wait(smem_u32(&pv_done[prev]), ppar, abort_flag);
                 __syncwarp();
                 tc_after();
@@ -518,7 +603,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                     e = two(a, b);
                     if (c & 1) part = add_2(part, e);
                     else sum = add_2(sum, e);
-                    pk[c] = pack16(a, b, A.mma_type);
+                    pk[c] = pack16(a, b, TYPE);
                 }
                 tmem_st32(s_addr + 32u * h, pk);
             }
@@ -533,7 +618,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
             }
         }
         if (n > 0) {
-            const int last = TILES == 2 ? tile : (n - 1) & 1, lpar = TILES == 2 ? (n - 1) & 1 : ((n - 1) >> 1) & 1;
+            const int last = TILES == 2 ? tile : (g - 1) & 1, lpar = TILES == 2 ? (g - 1) & 1 : ((g - 1) >> 1) & 1;
             pk_wait(smem_u32(&pv_done[last]), lpar, abort_flag);
             if (TILES == 2 && A.splits > 1) pk_wait(smem_u32(&pv_done[tile ^ 1]), lpar, abort_flag);   // the partial sums go where K and V were
             __syncwarp();
@@ -542,32 +627,58 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         float l0, l1;
         both(sum, l0, l1);
         float l = l0 + l1;
-        const bool bad = bad_s != 0;   // a table entry outside the pool: the rows are NaN
-        const int64_t out_at = (int64_t)(U.row0 + U.t0 + tile_tok + tok) * A.out_ld + (int64_t)head * HD;
+        const volatile TcUnit& V = unit_s[k & 1];   // (not held in registers over the steps)
+        const bool ok = V.ok, bad = !ok || bad_s[k & 1] == k + 1;   // an index outside the layout: the rows are NaN
+        const bool live = tok < A.tpt && tile_tok + tok < V.tokens;
+        const int kvh = V.kvh, row_first = V.row0 + V.t0;
+        const int64_t out_at = (int64_t)(row_first + tile_tok + tok) * A.out_ld + (int64_t)(kvh * A.group + t - tok * A.group) * HD;
         const float inv = bad ? NAN : 1.f / l;
         float probe = 0.f;   // NaN when a sum is not finite
+        int64_t quad_out[4];   // where the four rows of this lane's quad go; negative: nowhere
+#pragma unroll
+        for (int q = 0; q < 4; q++) quad_out[q] = __shfl_sync(0xffffffffu, live ? out_at : -1, (lane & 28) + q);
         float* part_o = reinterpret_cast<float*>(base) + tile * 128 * HD;   // splits: [row][HD], 16-byte pieces swizzled
         if (n > 0) {
+            auto rows_out = [&](auto type_tag) {
+                constexpr int OUT = decltype(type_tag)::value;
 #pragma unroll 2
-            for (int c = 0; c < HD; c += 32) {
-                unsigned o[32];
-                tmem_ld32(o_addr + c, o);
-                asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+                for (int c = 0; c < HD; c += 32) {
+                    unsigned o[32];
+                    tmem_ld32(o_addr + c, o);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
-                for (int q = 0; q < 32; q++) probe = fmaf(__uint_as_float(o[q]), 0.f, probe);
-                if (A.splits > 1) {
+                    for (int q = 0; q < 32; q++) probe = fmaf(__uint_as_float(o[q]), 0.f, probe);
+                    if (OUT == TC_F32) {   // partial sums for the merge
 #pragma unroll
-                    for (int q = 0; q < 32; q += 4)
-                        *reinterpret_cast<uint4*>(part_o + t * HD + (((c + q) >> 2 ^ (t & 7)) << 2)) = make_uint4(o[q], o[q + 1], o[q + 2], o[q + 3]);
-                } else if (live) {
-                    unsigned v[16];
+                        for (int q = 0; q < 32; q += 4)
+                            *reinterpret_cast<uint4*>(part_o + t * HD + (((c + q) >> 2 ^ (t & 7)) << 2)) = make_uint4(o[q], o[q + 1], o[q + 2], o[q + 3]);
+                        continue;
+                    }
+                    uint4 v[4];
 #pragma unroll
-                    for (int q = 0; q < 16; q++) v[q] = pack16(__uint_as_float(o[2 * q]) * inv, __uint_as_float(o[2 * q + 1]) * inv, A.out_type);
-                    uint4* dst = reinterpret_cast<uint4*>(static_cast<unsigned short*>(A.out) + out_at + c);
+                    for (int q = 0; q < 4; q++)
+                        v[q] = make_uint4(pack16(__uint_as_float(o[8 * q]) * inv, __uint_as_float(o[8 * q + 1]) * inv, OUT),
+                                          pack16(__uint_as_float(o[8 * q + 2]) * inv, __uint_as_float(o[8 * q + 3]) * inv, OUT),
+                                          pack16(__uint_as_float(o[8 * q + 4]) * inv, __uint_as_float(o[8 * q + 5]) * inv, OUT),
+                                          pack16(__uint_as_float(o[8 * q + 6]) * inv, __uint_as_float(o[8 * q + 7]) * inv, OUT));
+                    // four lanes hand their rows' 16-byte pieces round, so that a store writes 64 bytes of a row
+                    swap_pieces(v[0], v[1], 1, lane);
+                    swap_pieces(v[2], v[3], 1, lane);
+                    swap_pieces(v[0], v[2], 2, lane);
+                    swap_pieces(v[1], v[3], 2, lane);
 #pragma unroll
-                    for (int q = 0; q < 4; q++) dst[q] = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                    for (int q = 0; q < 4; q++)
+                        if (quad_out[q] >= 0) *reinterpret_cast<uint4*>(static_cast<unsigned short*>(A.out) + quad_out[q] + c + (lane & 3) * 8) = v[q];
                 }
-            }
+            };
+            if (A.splits > 1) rows_out(std::integral_constant<int, TC_F32>());
+            else if (A.out_type == TC_BF16) rows_out(std::integral_constant<int, TC_BF16>());
+            else rows_out(std::integral_constant<int, TC_F16>());
+        }
+        if (!ok && live && A.splits == 1) {
+            const unsigned nan = A.out_type == TC_BF16 ? 0x7FC07FC0u : 0x7E007E00u;
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<unsigned short*>(A.out) + out_at);
+            for (int q = 0; q < HD / 8; q++) dst[q] = make_uint4(nan, nan, nan, nan);
         }
         tc_before();
         // rows that met a non-finite value where they do not attend (or where they do: the answer is then the same)
@@ -578,17 +689,17 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
 #pragma unroll
         for (int q = 0; q < 4; q++) again[q] = again_s[tile * 4 + q];
         if (again[0] | again[1] | again[2] | again[3]) {
-            float* scratch = reinterpret_cast<float*>(base + (A.splits > 1 ? kMergeAt + tile * 2048 : tile * D::kQTile));
 #pragma unroll 1
             for (int r = 0; r < 128; r++) {
                 if (!((again[r >> 5] >> (r & 31)) & 1u)) continue;
-                const int rt = r / A.group, rp = p_first + tile_tok + rt;
-                const int64_t row = U.row0 + U.t0 + tile_tok + rt, rh = kvh * A.group + r - rt * A.group;
+                const TcUnit W = unit_s[k & 1];
+                const int rt = r / A.group, rp = W.p_first + tile_tok + rt, je = W.jb + W.n;
+                const int64_t row = row_first + tile_tok + rt, rh = kvh * A.group + r - rt * A.group;
                 int lo = A.window > 0 && rp + 1 > A.window ? rp + 1 - A.window : 0, hi = rp + 1;
                 lo = lo > jb * TC_KV ? lo : jb * TC_KV;
                 hi = hi < je * TC_KV ? hi : je * TC_KV;
                 float o[HD / 128], m2, l2;
-                tc_row_again<HD>(A, U, kvh, row * A.q_ld + rh * HD, lo, hi, t, 1 + tile, scratch, o, &m2, &l2);
+                tc_row_again<HD>(A, W, row * A.q_ld + rh * HD, lo, hi, t, 1 + tile, again_w[tile], o, &m2, &l2);
 #pragma unroll
                 for (int q = 0; q < HD / 128; q++) {
                     const int d = t + 128 * q;
@@ -605,11 +716,13 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
             merge_ml[tile * 128 + t][0] = bad ? 0.f : m;
             merge_ml[tile * 128 + t][1] = bad ? NAN : l;
         }
+        wg_sync(1 + tile);   // again_s is free for the next unit
+        }
     } else if (warp == D::kMma) {
         // ---- MMA issue (of a pair: the leader): the whole warp walks the loop, one elected lane issues ----
         if (rank == 0) {
             const unsigned elected = elect_lane();
-            const unsigned fmt = A.mma_type == TC_BF16 ? (1u << 7) | (1u << 10) : 0u;
+            const unsigned fmt = TYPE == TC_BF16 ? (1u << 7) | (1u << 10) : 0u;
             const unsigned m_field = (unsigned)((128 * CG) >> 4) << 24;
             const unsigned id_qk = (1u << 4) | fmt | ((128u >> 3) << 17) | m_field;
             const unsigned id_pv = (1u << 4) | fmt | (1u << 16) | ((unsigned)((CG == 2 ? HD : 128) >> 3) << 17) | m_field;   // B is N-major
@@ -647,74 +760,96 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 }
                 tc_commit<CG>(smem_u32(&pv_done[slot_i]), lead, elected);
             };
-            pk_wait(smem_u32(&q_full), 0, abort_flag);
-            tc_after();
-            if (TILES == 2) {
-                // stages: K0 V0 K1 V1 ...
-                vr.step(1);
-                if (n > 0) {
-                    qk(0, 0, false);
-                    qk(1, 1, true);
-                    kr.step(2);
-                }
-                for (int i = 0; i < n; i++) {
-#pragma unroll
-                    for (int tile = 0; tile < 2; tile++) {
-                        pk_wait(smem_u32(&p_full[tile]), i & 1, abort_flag);
-                        tc_after();
-                        pv(tile, tile, i == 0, tile == 1);
-                        if (i + 1 < n) qk(tile, tile, tile == 1);
+            int g = 0;   // steps of all units so far
+            Ring st(NS);
+            for (int k = 0; have; have = next_unit(k++)) {
+                const int n = U.n;
+                if (A.q_boxes) pk_wait(smem_u32(&q_full), k & 1, abort_flag);
+                else if (k == 0) pk_wait(smem_u32(&q_first), 0, abort_flag);
+                else pk_wait(smem_u32(&q_full), (k - 1) & 1, abort_flag);
+                tc_after();
+                if (TILES == 2) {
+                    // stages: K0 V0 K1 V1 ...
+                    kr = vr = st;
+                    vr.step(1);
+                    if (n > 0) {
+                        qk(0, 0, false);
+                        qk(1, 1, true);
+                        kr.step(2);
                     }
-                    kr.step(2);
-                    vr.step(2);
-                }
-            } else {
-                // stages: K0 K1 V0 K2 V1 ... (each KV_STAGES long)
-                Ring st(NS);
-                if (n > 0) {
-                    kr = st;
-                    qk(0, 0, true);
-                    st.step(KV_STAGES);
-                }
-                for (int i = 0; i < n; i++) {
-                    if (i + 1 < n) {
+                    if (n <= 1) tc_commit<CG>(smem_u32(&q_empty), lead, elected);
+                    for (int i = 0; i < n; i++, g++) {
+#pragma unroll
+                        for (int tile = 0; tile < 2; tile++) {
+                            pk_wait(smem_u32(&p_full[tile]), g & 1, abort_flag);
+                            tc_after();
+                            pv(tile, tile, i == 0, tile == 1);
+                            if (i + 1 < n) qk(tile, tile, tile == 1);
+                        }
+                        if (i + 2 == n) tc_commit<CG>(smem_u32(&q_empty), lead, elected);   // the unit's last use of its queries
+                        kr.step(2);
+                        vr.step(2);
+                        st.step(2);
+                    }
+                } else {
+                    // stages: K0 K1 V0 K2 V1 ... (each KV_STAGES long)
+                    if (n > 0) {
                         kr = st;
-                        qk(0, (i + 1) & 1, true);
+                        qk(0, g & 1, true);
                         st.step(KV_STAGES);
                     }
-                    pk_wait(smem_u32(&p_full[i & 1]), (i >> 1) & 1, abort_flag);
-                    tc_after();
-                    vr = st;
-                    pv(0, i & 1, i == 0, true);
-                    st.step(KV_STAGES);
+                    if (n <= 1) tc_commit<CG>(smem_u32(&q_empty), lead, elected);
+                    for (int i = 0; i < n; i++, g++) {
+                        if (i + 1 < n) {
+                            kr = st;
+                            qk(0, (g + 1) & 1, true);
+                            st.step(KV_STAGES);
+                            if (i + 2 == n) tc_commit<CG>(smem_u32(&q_empty), lead, elected);
+                        }
+                        pk_wait(smem_u32(&p_full[g & 1]), (g >> 1) & 1, abort_flag);
+                        tc_after();
+                        vr = st;
+                        pv(0, g & 1, i == 0, true);
+                        st.step(KV_STAGES);
+                    }
                 }
             }
+        } else {
+            for (int k = 0; have; have = next_unit(k++)) {}   // of a pair's second CTA: keeps the units' slots moving
         }
-    } else if (tma) {
-        // ---- TMA boxes, in the order in which the MMA warp takes the stages; three warps share a stage's boxes ----
-        {
-            const int w = warp - D::kTma;
-            const unsigned elected = elect_lane();
-            const unsigned full_c = CG == 2 ? map_to_rank(smem_u32(&full[0]), lead) : smem_u32(&full[0]);
+    } else {
+        // ---- loads, by three warps, in the order in which the MMA warp takes the stages; the first of them also hands out units ----
+        const int w = warp - D::kTma;
+        const unsigned elected = elect_lane();
+        const unsigned full_c = CG == 2 ? map_to_rank(smem_u32(&full[0]), lead) : smem_u32(&full[0]);
+        Ring st(NS);
+        const bool more = A.splits == 1;   // a cluster that merges has one unit
+        int units = 0;
+        if (more && have && w == 0 && rank == 0 && lane == 0) tc_next_request(smem_u32(answer_s), smem_u32(&answer_bar));
+        for (int k = 0; have; k++) {
+            units++;
+            const int n = U.n, jb = U.jb, p_last = U.p_last();
             const int32_t* trow = A.table ? A.table + (int64_t)U.slot * A.max_blocks : nullptr;
-            const int page_lo = A.table ? lo_unit / A.page : 0, page_hi = A.table ? p_last / A.page : 0;
-            Ring st(NS);
+            const int page_lo = trow ? U.lo / A.page : 0, page_hi = trow ? p_last / A.page : 0;
             // Lane l: the table entry of the step's page l.  Pages that no row attends to are filled with zeros, not read.
             auto entries = [&](int i) {
                 int e = (int)A.blocks;
-                const int pg = (jb + i) * TC_KV / A.page + lane;
-                if (trow && i < n && lane * A.box_v < TC_KV && pg >= page_lo && pg <= page_hi) {
-                    e = trow[pg];
-                    if (e < 0 || e >= A.blocks) {
-                        atomicOr(A.status, LEV_DEV_BAD_INDEX);
-                        bad_s = 1;
-                        e = (int)A.blocks;
+                if (tma && trow && i < n) {
+                    const int pg = (jb + i) * TC_KV / A.page + lane;
+                    if (lane * A.box_v < TC_KV && pg >= page_lo && pg <= page_hi) {
+                        e = trow[pg];
+                        if (e < 0 || e >= A.blocks) {
+                            atomicOr(A.status, LEV_DEV_BAD_INDEX);
+                            bad_s[k & 1] = k + 1;
+                            e = (int)A.blocks;
+                        }
                     }
                 }
                 __syncwarp();
                 return e;
             };
-            auto load = [&](int i, bool is_v, int entry) {
+            // boxes of a step's K or V; three warps share a stage's
+            auto boxes = [&](int i, bool is_v, int entry) {
                 const CUtensorMap* map = is_v ? &vmap : &kmap;
                 const int c0 = (jb + i) * TC_KV;
                 const int r_first = CG == 2 && !is_v ? (int)rank * 64 : 0, r_n = CG == 2 && !is_v ? 64 : 128;   // rows of this CTA
@@ -728,95 +863,138 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                     if (rank == 0 && w == 0) pk_expect(smem_u32(&full[st.s]), TC_STAGE * CG, elected);
                     const int x0 = CG == 2 ? (is_v ? (int)rank * 128 : 0) : h * 128;
                     if (trow) {
-                        const int slab = (kvh * HD + x0) >> 6;
+                        const int slab = (U.kvh * HD + x0) >> 6;
                         const int in_page = A.page >= TC_KV ? (c0 + r_first) % A.page >> 3 : 0;   // first group of eight rows
                         for (int r = w * box; r < r_n; r += TC_LOAD_WARPS * box)
                             tc_box_page<CG>(dst + (unsigned)r * row_bytes, map, slab, in_page, __shfl_sync(0xffffffffu, entry, (r_first + r) / A.box_v), bar, elected);
                     } else {
                         for (int b = w; b < (is_v ? kSlabsV : kSlabsK); b += TC_LOAD_WARPS)
-                            tc_box_rows<CG>(dst + (unsigned)(b * r_n) * 128u, map, x0 + 64 * b, kvh, U.row0 + c0 + r_first, bar, elected);
+                            tc_box_rows<CG>(dst + (unsigned)(b * r_n) * 128u, map, x0 + 64 * b, U.kvh, U.row0 + c0 + r_first, bar, elected);
                     }
                     st.step(1);
                 }
             };
+            // rows copied (and converted): pages of any size, f32 pools (never in pairs)
+            auto copies = [&](int i, bool is_v) {
+                const int c0 = (jb + i) * TC_KV;
+                for (int h = 0; h < KV_STAGES; h++) {
+                    pk_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
+                    const unsigned dst = ring + (unsigned)st.s * TC_STAGE;
+                    // two rows of 16 pieces (8 values each) per step of a warp
+                    const int piece = lane & 15, sub = lane >> 4;
+                    for (int r0 = 2 * w; r0 < 128; r0 += 2 * TC_LOAD_WARPS * 4) {
+                        uint4 v[4];
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            const int r = r0 + q * 2 * TC_LOAD_WARPS + sub, at = c0 + r;
+                            v[q] = make_uint4(0u, 0u, 0u, 0u);
+                            if (r < 128 && at >= U.lo && at <= p_last) {
+                                const unsigned char* src = tc_row(A, U, HD, at, is_v);
+                                if (!src) {
+                                    atomicOr(A.status, LEV_DEV_BAD_INDEX);
+                                    bad_s[k & 1] = k + 1;
+                                } else if (A.kv_type == TC_F32) {
+                                    const float4* f = reinterpret_cast<const float4*>(src) + (h * 16 + piece) * 2;
+                                    const float4 a = f[0], b = f[1];
+                                    v[q] = make_uint4(pack16(a.x, a.y, TC_F16), pack16(a.z, a.w, TC_F16), pack16(b.x, b.y, TC_F16), pack16(b.z, b.w, TC_F16));
+                                } else {
+                                    v[q] = *(reinterpret_cast<const uint4*>(src) + h * 16 + piece);
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            const int r = r0 + q * 2 * TC_LOAD_WARPS + sub;
+                            if (r < 128)
+                                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst + (unsigned)(piece >> 3) * 16384u + (unsigned)r * 128u +
+                                                                                                (unsigned)(((piece & 7) ^ (r & 7)) << 4)),
+                                             "r"(v[q].x), "r"(v[q].y), "r"(v[q].z), "r"(v[q].w)
+                                             : "memory");
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&full[st.s]));
+                    st.step(1);
+                }
+            };
+            auto load = [&](int i, bool is_v, int entry) {
+                if (tma) boxes(i, is_v, entry);
+                else copies(i, is_v);
+            };
             int e_now = entries(0), e_before = 0;
             for (int i = 0; i <= n; i++) {
                 const int e_next = entries(i + 1);   // read a step ahead
-                if (TILES == 2) {
-                    if (i < n) {
-                        load(i, false, e_now);
-                        load(i, true, e_now);
+                if (i < n) load(i, false, e_now);
+                if (i == 0) {
+                    // This unit's queries, when the last product that read the ones before is done.  The first K tile has been asked
+                    // for: waiting any later could wait for a stage that only these queries would free.
+                    if (k > 0) pk_wait(smem_u32(&q_empty), (k - 1) & 1, abort_flag);
+                    __syncwarp();
+                    if (A.q_boxes) {   // one box of 64 columns: the group's heads of a tile's tokens
+                        if (w == 0) {
+                            const unsigned bar = CG == 2 ? map_to_rank(smem_u32(&q_full), lead) : smem_u32(&q_full);
+                            if (rank == 0) pk_expect(smem_u32(&q_full), (unsigned)(CG * TILES * (HD / 64) * A.group * A.tpt) * 128u, elected);
+#pragma unroll
+                            for (int b = 0; b < TILES * (HD / 64); b++)
+                                tc_box_rows<CG>(smem + (unsigned)b * 16384u, &qmap, (b % (HD / 64)) * 64, U.kvh * A.group,
+                                                U.row0 + U.t0 + ((int)rank * TILES + b / (HD / 64)) * A.tpt, bar, elected);
+                        }
+                    } else if (k > 0) {
+                        tc_load_q<HD, TILES == 2 ? 8 : 16>(A, U, smem, (int)rank * TILES * A.tpt, TILES, w, TC_LOAD_WARPS, lane);
+                        if (lane == 0) {
+                            if (CG == 2) mbar_arrive_cluster(map_to_rank(smem_u32(&q_full), lead));
+                            else mbar_arrive(smem_u32(&q_full));
+                        }
                     }
+                }
+                if (TILES == 2) {
+                    if (i < n) load(i, true, e_now);
                 } else {
-                    if (i < n) load(i, false, e_now);
                     if (i > 0) load(i - 1, true, e_before);
                 }
                 e_before = e_now;
                 e_now = e_next;
             }
-            for (int s = 0; s < NS; s++) {   // the tensor core's last releases have arrived
-                pk_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
-                st.step(1);
-            }
-        }
-    } else {
-        // ---- rows copied (and converted) by warps: pages of any size, f32 pools ----
-        const int w = warp - D::kTma;
-        Ring st(NS);
-        auto load = [&](int i, bool is_v) {
-            const int c0 = (jb + i) * TC_KV;
-            for (int h = 0; h < KV_STAGES; h++) {
-                pk_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
-                const unsigned dst = ring + (unsigned)st.s * TC_STAGE;
-                // two rows of 16 pieces (8 values each) per step of a warp
-                const int piece = lane & 15, sub = lane >> 4;
-                for (int r0 = 2 * w; r0 < 128; r0 += 2 * TC_LOAD_WARPS * 4) {
-                    uint4 v[4];
-#pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        const int r = r0 + q * 2 * TC_LOAD_WARPS + sub, at = c0 + r;
-                        v[q] = make_uint4(0u, 0u, 0u, 0u);
-                        if (r < 128 && at >= lo_unit && at <= p_last) {
-                            const unsigned char* src = tc_row(A, U, kvh, HD, at, is_v);
-                            if (!src) {
-                                atomicOr(A.status, LEV_DEV_BAD_INDEX);
-                                bad_s = 1;
-                            } else if (A.kv_type == TC_F32) {
-                                const float4* f = reinterpret_cast<const float4*>(src) + (h * 16 + piece) * 2;
-                                const float4 a = f[0], b = f[1];
-                                v[q] = make_uint4(pack16(a.x, a.y, TC_F16), pack16(a.z, a.w, TC_F16), pack16(b.x, b.y, TC_F16), pack16(b.z, b.w, TC_F16));
-                            } else {
-                                v[q] = *(reinterpret_cast<const uint4*>(src) + h * 16 + piece);
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        const int r = r0 + q * 2 * TC_LOAD_WARPS + sub;
-                        if (r < 128)
-                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst + (unsigned)(piece >> 3) * 16384u + (unsigned)r * 128u +
-                                                                                            (unsigned)(((piece & 7) ^ (r & 7)) << 4)),
-                                         "r"(v[q].x), "r"(v[q].y), "r"(v[q].z), "r"(v[q].w)
+            if (!more) break;
+            // ---- the next unit ----
+            if (w == 0) {
+                int x;
+                if (rank == 0) {
+                    pk_wait(smem_u32(&answer_bar), k & 1, abort_flag);
+                    x = *abort_flag ? -1 : tc_next_taken(smem_u32(answer_s));
+                    __syncwarp();
+                    if (lane == 0) {
+                        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");   // the answer has been read
+                        if (CG == 2)   // a pair's second CTA is told
+                            asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.u32 [%0], %1, [%2];\n" ::"r"(
+                                             map_to_rank(smem_u32(&told_s[k & 1]), lead + 1)),
+                                         "r"(x), "r"(map_to_rank(smem_u32(&told_bar[k & 1]), lead + 1))
                                          : "memory");
                     }
+                } else {
+                    if (lane == 0) mbar_expect(smem_u32(&told_bar[k & 1]), 4);
+                    pk_wait(smem_u32(&told_bar[k & 1]), (k >> 1) & 1, abort_flag);
+                    __syncwarp();
+                    x = *abort_flag ? -1 : *(volatile int*)&told_s[k & 1];
                 }
-                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                have = x >= 0 && tc_unit(A, x / cluster, per, split, lane, &U);
+                if (have && rank == 0 && lane == 0) tc_next_request(smem_u32(answer_s), smem_u32(&answer_bar));
+                // unit k + 1 goes where unit k - 1 was
+                if (k > 0) pk_wait(smem_u32(&unit_empty[(k + 1) & 1]), ((k - 1) >> 1) & 1, abort_flag);
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&full[st.s]));
-                st.step(1);
-            }
-        };
-        if (TILES == 2) {
-            for (int i = 0; i < n; i++) {
-                load(i, false);
-                load(i, true);
-            }
-        } else {
-            for (int i = 0; i <= n; i++) {
-                if (i < n) load(i, false);
-                if (i > 0) load(i - 1, true);
+                if (lane == 0) {
+                    if (!have) U.tokens = 0;
+                    unit_s[(k + 1) & 1] = U;
+                    mbar_arrive(smem_u32(&unit_full[(k + 1) & 1]));
+                }
+                __syncwarp();
+                if (*abort_flag) have = false;
+            } else {
+                have = next_unit(k);
             }
         }
+        if (units) pk_wait(smem_u32(&q_empty), (units - 1) & 1, abort_flag);   // the tensor core's last releases have arrived
         for (int s = 0; s < NS; s++) {
             pk_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
             st.step(1);
@@ -824,6 +1002,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
     }
     pk_finish(abort_flag, A.status, LEV_DEV_TIMEOUT);
     if (A.splits > 1) {
+        const int tokens = U0.tokens;
         // ---- merge: the CTA of split z adds its share of the rows over all splits, in their order ----
         cluster_sync_all();
         const int Z = A.splits;
@@ -831,7 +1010,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
 #pragma unroll 1
         for (int tile = 0; tile < TILES; tile++) {
             const int tile_tok = (int)(rank * TILES + tile) * A.tpt;
-            const int used = tokens > tile_tok ? (tokens - tile_tok < A.tpt ? tokens - tile_tok : A.tpt) * A.group : 0;
+            const int used = tokens > tile_tok ? (tokens - tile_tok < A.tpt ? tokens - tile_tok : A.tpt) * A.group : 0;   // rows
             const int ra = used * split / Z, rb = used * (split + 1) / Z;
             __syncthreads();   // the weights of the tile before are read
             for (int r = ra + (int)threadIdx.x; r < rb; r += blockDim.x) {
@@ -891,8 +1070,8 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 for (int k = 0; k < kItems; k++) {
                     const int item = i0 + k * (int)blockDim.x, r = item / kQuads, qd = item - r * kQuads, tok = r / A.group;
                     if (item >= end) continue;
-                    unsigned short* dst = static_cast<unsigned short*>(A.out) + (int64_t)(U.row0 + U.t0 + tile_tok + tok) * A.out_ld +
-                                          (int64_t)(kvh * A.group + r - tok * A.group) * HD + 4 * qd;
+                    unsigned short* dst = static_cast<unsigned short*>(A.out) + (int64_t)(U0.row0 + U0.t0 + tile_tok + tok) * A.out_ld +
+                                          (int64_t)(U0.kvh * A.group + r - tok * A.group) * HD + 4 * qd;
                     *reinterpret_cast<uint2*>(dst) = make_uint2(pack16(a[k].x, a[k].y, A.out_type), pack16(a[k].z, a[k].w, A.out_type));
                 }
             }
@@ -931,17 +1110,17 @@ TcPlan tc_plan(const lev_ctx* ctx, int64_t rows, int seqs, int kv_heads, int tpt
     return P;
 }
 
-template <int HD, int TILES, int CG>
-int tc_launch(lev_ctx* ctx, const CUtensorMap& kmap, const CUtensorMap& vmap, const TcArgs& A, int64_t units) {
+template <int HD, int TILES, int CG, int TYPE>
+int tc_launch(lev_ctx* ctx, const CUtensorMap& kmap, const CUtensorMap& vmap, const CUtensorMap& qmap, const TcArgs& A, int64_t units) {
     using D = TcDims<HD, TILES>;
     static bool configured[16] = {};
     if (!configured[ctx->device & 15]) {
-        LEV_CUDA(ctx, cudaFuncSetAttribute(k_attn_tc<HD, TILES, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)D::kSmem));
+        LEV_CUDA(ctx, cudaFuncSetAttribute(k_attn_tc<HD, TILES, CG, TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)D::kSmem));
         configured[ctx->device & 15] = true;
     }
     const int cluster = CG * A.splits;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(units * cluster), (unsigned)A.kv_heads);
+    cfg.gridDim = dim3((unsigned)(units * A.kv_heads * cluster));
     cfg.blockDim = dim3(D::kWarps * 32);
     cfg.dynamicSmemBytes = D::kSmem;
     cfg.stream = ctx->stream;
@@ -953,14 +1132,30 @@ int tc_launch(lev_ctx* ctx, const CUtensorMap& kmap, const CUtensorMap& vmap, co
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
-    LEV_CUDA(ctx, cudaLaunchKernelEx(&cfg, k_attn_tc<HD, TILES, CG>, kmap, vmap, A));
+    LEV_CUDA(ctx, cudaLaunchKernelEx(&cfg, k_attn_tc<HD, TILES, CG, TYPE>, kmap, vmap, qmap, A));
     ctx->launches++;
     return lev_cuda_check(ctx, cudaGetLastError(), "k_attn_tc");
 }
 
-int tc_run(lev_ctx* ctx, const CUtensorMap& kmap, const CUtensorMap& vmap, const TcArgs& A, const TcPlan& P, int hd) {
-    if (hd == 256) return P.cg == 2 ? tc_launch<256, 1, 2>(ctx, kmap, vmap, A, P.units) : tc_launch<256, 1, 1>(ctx, kmap, vmap, A, P.units);
-    return P.tiles == 2 ? tc_launch<128, 2, 1>(ctx, kmap, vmap, A, P.units) : tc_launch<128, 1, 1>(ctx, kmap, vmap, A, P.units);
+int tc_run(lev_ctx* ctx, EncodeTiledFn enc, const CUtensorMap& kmap, const CUtensorMap& vmap, TcArgs A, const TcPlan& P, int hd) {
+    // 16-bit queries come as boxes of (64 columns, the heads of a group, the tokens of a tile)
+    CUtensorMap qmap = {};
+    A.q_boxes = A.q_type != TC_F32 && !A.negate;
+    if (A.q_boxes) {
+        const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)A.q_heads, (cuuint64_t)A.rows}, strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)A.q_ld * 2};
+        const cuuint32_t box[3] = {64, (cuuint32_t)A.group, (cuuint32_t)A.tpt}, one[3] = {1, 1, 1};
+        const CUresult cr = enc(&qmap, A.q_type == TC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(A.q), dims,
+                                strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (cr != CUDA_SUCCESS) return lev_fail(ctx, LEV_KERNEL_FAILED, "cuTensorMapEncodeTiled failed (%d)", (int)cr);
+    }
+    auto launch = [&](auto type_tag) {
+        constexpr int TYPE = decltype(type_tag)::value;
+        if (hd == 256)
+            return P.cg == 2 ? tc_launch<256, 1, 2, TYPE>(ctx, kmap, vmap, qmap, A, P.units) : tc_launch<256, 1, 1, TYPE>(ctx, kmap, vmap, qmap, A, P.units);
+        return P.tiles == 2 ? tc_launch<128, 2, 1, TYPE>(ctx, kmap, vmap, qmap, A, P.units) : tc_launch<128, 1, 1, TYPE>(ctx, kmap, vmap, qmap, A, P.units);
+    };
+    return A.kv_type == TC_BF16 ? launch(std::integral_constant<int, TC_BF16>()) : launch(std::integral_constant<int, TC_F16>());
 }
 
 bool ranges_meet(const void* a, int64_t an, const void* b, int64_t bn) {
@@ -1027,7 +1222,6 @@ extern "C" int lev_attn_chunk(lev_ctx* ctx, const lev_kv_layout* L, const void* 
     LEV_CUDA(ctx, cudaSetDevice(ctx->device));
     TcArgs A = tc_args(ctx, n_chunks, start, n_rows, q_heads, L->kv_heads, q, q_type, q_ld, window, scale, out, out_type, out_ld);
     const int hd = L->head_dim;
-    A.mma_type = TC_F16;
     A.kv_type = L->kv_type == LEV_KV_F32 ? TC_F32 : TC_F16;
     A.slot = slot;
     A.pos = pos;
@@ -1062,7 +1256,7 @@ extern "C" int lev_attn_chunk(lev_ctx* ctx, const lev_kv_layout* L, const void* 
         A.box_k = box_k;
         A.box_v = box_v;
     }
-    return tc_run(ctx, kmap, vmap, A, P, hd);
+    return tc_run(ctx, enc, kmap, vmap, A, P, hd);
 }
 
 extern "C" int lev_attn_prompt(lev_ctx* ctx, int n_seqs, const int32_t* start, int64_t n_rows, int q_heads, int kv_heads, int head_dim, int type,
@@ -1083,7 +1277,7 @@ extern "C" int lev_attn_prompt(lev_ctx* ctx, int n_seqs, const int32_t* start, i
     if (!enc) return lev_fail(ctx, LEV_UNSUPPORTED, "cuTensorMapEncodeTiled is not available");
     LEV_CUDA(ctx, cudaSetDevice(ctx->device));
     TcArgs A = tc_args(ctx, n_seqs, start, n_rows, q_heads, kv_heads, q, type, q_ld, window, scale, out, type, out_ld);
-    A.mma_type = A.kv_type = type;
+    A.kv_type = type;
     A.k = k;
     A.v = v;
     A.k_ld = k_ld;
@@ -1104,5 +1298,5 @@ extern "C" int lev_attn_prompt(lev_ctx* ctx, int n_seqs, const int32_t* start, i
                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
         if (cr != CUDA_SUCCESS) return lev_fail(ctx, LEV_KERNEL_FAILED, "cuTensorMapEncodeTiled failed (%d)", (int)cr);
     }
-    return tc_run(ctx, kmap, vmap, A, P, head_dim);
+    return tc_run(ctx, enc, kmap, vmap, A, P, head_dim);
 }

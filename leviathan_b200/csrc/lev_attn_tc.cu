@@ -347,44 +347,63 @@ __device__ void tc_row_again(const TcArgs& A, const TcUnit& U, int64_t q_at, int
 template <int HD, int BATCH>
 __device__ __forceinline__ void tc_load_q(const TcArgs& A, const TcUnit& U, unsigned smem, int first_tok, int tiles, int me, int warps, int lane) {
     constexpr int kPieces = HD / 8, kRows = 32 / kPieces;   // 16-byte pieces of a row; rows of a warp's step
-    const int piece = lane % kPieces, sub = lane / kPieces, rows = tiles * 128;
-    auto source = [&](int r) -> int64_t {   // element offset of this lane's piece; negative: no such row
-        const int rr = r & 127, tok = rr / A.group, at = first_tok + (r >> 7) * A.tpt + tok;
-        if (r >= rows || tok >= A.tpt || at >= U.tokens) return -1;
-        return (int64_t)(U.row0 + U.t0 + at) * A.q_ld + (int64_t)(U.kvh * A.group + rr - tok * A.group) * HD + piece * 8;
-    };
-    auto put = [&](int r, uint4 v) {
-        if (r >= rows) return;
-        if (A.negate) v = make_uint4(v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
-        const unsigned dst = smem + (unsigned)(r >> 7) * (128u * HD * 2) + (unsigned)(piece >> 3) * 16384u + (unsigned)(r & 127) * 128u +
-                             (unsigned)(((piece & 7) ^ (r & 7)) << 4);
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-    };
-    const int step = warps * kRows;
+    const int piece = lane % kPieces, step = warps * kRows, first = me * kRows + lane / kPieces;
+    const int size = A.q_type == TC_F32 ? 4 : 2;
+    // from row to row the token and the head go up by these, and the address with them (divisions and products for each row
+    // took longer than the loads)
+    const int tok_step = step / A.group, head_step = step - tok_step * A.group;
+    const int64_t move = (tok_step * A.q_ld + (int64_t)head_step * HD) * size, wrap = (A.q_ld - (int64_t)A.group * HD) * size;
 #pragma unroll 1
-    for (int r0 = me * kRows + sub; r0 < rows + sub; r0 += BATCH * step) {
-        if (A.q_type == TC_F32) {
-            float4 a[BATCH], b[BATCH];
-#pragma unroll
-            for (int k = 0; k < BATCH; k++) {
-                const int64_t at = source(r0 + k * step);
-                const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(A.q) + at);
-                a[k] = at >= 0 ? src[0] : make_float4(0.f, 0.f, 0.f, 0.f);
-                b[k] = at >= 0 ? src[1] : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int tile = 0; tile < tiles; tile++) {
+        int tok = first / A.group, head = first - tok * A.group;
+        const int from = first_tok + tile * A.tpt, end = U.tokens - from < A.tpt ? U.tokens - from : A.tpt;   // tokens of this tile
+        const char* src = static_cast<const char*>(A.q) + ((int64_t)(U.row0 + U.t0 + from + tok) * A.q_ld + (int64_t)(U.kvh * A.group + head) * HD + piece * 8) * size;
+        const unsigned dst = smem + (unsigned)tile * (128u * HD * 2) + (unsigned)(piece >> 3) * 16384u;
+        auto put = [&](int r, uint4 v) {
+            if (r >= 128) return;
+            if (A.negate) v = make_uint4(v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst + (unsigned)r * 128u + (unsigned)(((piece & 7) ^ (r & 7)) << 4)), "r"(v.x),
+                         "r"(v.y), "r"(v.z), "r"(v.w)
+                         : "memory");
+        };
+        auto next = [&]() {
+            tok += tok_step;
+            head += head_step;
+            src += move;
+            if (head >= A.group) {
+                head -= A.group;
+                tok++;
+                src += wrap;
             }
+        };
+#pragma unroll 1
+        for (int r0 = first; r0 < 128; r0 += BATCH * step) {
+            if (A.q_type == TC_F32) {
+                float4 a[BATCH], b[BATCH];
 #pragma unroll
-            for (int k = 0; k < BATCH; k++)
-                put(r0 + k * step, make_uint4(pack16(a[k].x, a[k].y, TC_F16), pack16(a[k].z, a[k].w, TC_F16), pack16(b[k].x, b[k].y, TC_F16),
-                                              pack16(b[k].z, b[k].w, TC_F16)));
-        } else {
-            uint4 v[BATCH];
+                for (int k = 0; k < BATCH; k++) {
+                    a[k] = b[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (tok < end && r0 + k * step < 128) {
+                        a[k] = reinterpret_cast<const float4*>(src)[0];
+                        b[k] = reinterpret_cast<const float4*>(src)[1];
+                    }
+                    next();
+                }
 #pragma unroll
-            for (int k = 0; k < BATCH; k++) {
-                const int64_t at = source(r0 + k * step);
-                v[k] = at >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(A.q) + at) : make_uint4(0u, 0u, 0u, 0u);
+                for (int k = 0; k < BATCH; k++)
+                    put(r0 + k * step, make_uint4(pack16(a[k].x, a[k].y, TC_F16), pack16(a[k].z, a[k].w, TC_F16), pack16(b[k].x, b[k].y, TC_F16),
+                                                  pack16(b[k].z, b[k].w, TC_F16)));
+            } else {
+                uint4 v[BATCH];
+#pragma unroll
+                for (int k = 0; k < BATCH; k++) {
+                    v[k] = make_uint4(0u, 0u, 0u, 0u);
+                    if (tok < end && r0 + k * step < 128) v[k] = *reinterpret_cast<const uint4*>(src);
+                    next();
+                }
+#pragma unroll
+                for (int k = 0; k < BATCH; k++) put(r0 + k * step, v[k]);
             }
-#pragma unroll
-            for (int k = 0; k < BATCH; k++) put(r0 + k * step, v[k]);
         }
     }
     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");   // the tensor core reads through the async proxy
@@ -648,12 +667,11 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                     asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
                     for (int q = 0; q < 32; q++) probe = fmaf(__uint_as_float(o[q]), 0.f, probe);
-                    if (OUT == TC_F32) {   // partial sums for the merge
+                    if constexpr (OUT == TC_F32) {   // partial sums for the merge
 #pragma unroll
                         for (int q = 0; q < 32; q += 4)
                             *reinterpret_cast<uint4*>(part_o + t * HD + (((c + q) >> 2 ^ (t & 7)) << 2)) = make_uint4(o[q], o[q + 1], o[q + 2], o[q + 3]);
-                        continue;
-                    }
+                    } else {
                     uint4 v[4];
 #pragma unroll
                     for (int q = 0; q < 4; q++)
@@ -669,6 +687,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
 #pragma unroll
                     for (int q = 0; q < 4; q++)
                         if (quad_out[q] >= 0) *reinterpret_cast<uint4*>(static_cast<unsigned short*>(A.out) + quad_out[q] + c + (lane & 3) * 8) = v[q];
+                    }
                 }
             };
             if (A.splits > 1) rows_out(std::integral_constant<int, TC_F32>());

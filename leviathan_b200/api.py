@@ -40,36 +40,52 @@ def _ptr(a):
     return a.ctypes.data
 
 
-_ELEM = {}
+def _dp(t):
+    return None if t is None else t.data_ptr()
 
 
-def _elem(t, what: str, allowed: str) -> int:
-    """LEV_ELEM_* of a CUDA tensor's type, one of `allowed` (names separated by spaces)."""
-    if not _ELEM:
+_T = None      # torch, once a call has been given its tensors (this module does not import it by itself)
+_ELEM = {}     # dtype -> LEV_ELEM_*
+
+
+def _torch():
+    global _T
+    if _T is None:
         import torch
 
-        _ELEM.update({torch.float32: (L.ELEM_F32, "float32"), torch.float16: (L.ELEM_F16, "float16"), torch.bfloat16: (L.ELEM_BF16, "bfloat16")})
-    code, name = _ELEM.get(t.dtype, (None, str(t.dtype)))
-    if name not in allowed:
-        raise TypeError(f"{what} is {name}: {allowed.replace(' ', ' or ')} is wanted")
+        _ELEM.update({torch.float32: L.ELEM_F32, torch.float16: L.ELEM_F16, torch.bfloat16: L.ELEM_BF16})
+        _T = torch
+    return _T
+
+
+def _elem(t, what: str, allowed) -> int:
+    """LEV_ELEM_* of a tensor's type, one of `allowed`."""
+    code = _ELEM.get(t.dtype, -1)
+    if code not in allowed:
+        names = {v: str(k) for k, v in _ELEM.items()}
+        raise TypeError(f"{what} is {t.dtype}: {' or '.join(names[a] for a in allowed)} is wanted")
     return code
 
 
+_F32_F16, _ANY16, _ANY = (L.ELEM_F32, L.ELEM_F16), (L.ELEM_F16, L.ELEM_BF16), (L.ELEM_F32, L.ELEM_F16, L.ELEM_BF16)
+
+
 def _head_rows(t, what: str):
-    """[rows][heads][head_dim] with heads and dims contiguous, as the parts of a fused projection output lie: its row stride."""
-    if t.ndim != 3 or t.stride(2) != 1 or t.stride(1) != t.shape[2]:
-        raise ValueError(f"{what}: [rows][heads][head_dim] with contiguous heads is wanted, got shape {tuple(t.shape)}, strides {t.stride()}")
-    return t.stride(0)
+    """[rows][heads][head_dim] with heads and dims contiguous, as the parts of a fused projection output lie: shape and row stride."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or stride[2] != 1 or stride[1] != shape[2]:
+        raise ValueError(f"{what}: [rows][heads][head_dim] with contiguous heads is wanted, got shape {tuple(shape)}, strides {stride}")
+    return shape, stride[0]
 
 
 def _i32(t, n: int, what: str):
-    if t.numel() != n or str(t.dtype) != "torch.int32" or not t.is_contiguous():
+    if t.dtype is not _T.int32 or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{what}: {n} contiguous int32 values are wanted, got {t.numel()} of {t.dtype}")
 
 
 def _on(device: int, *tensors):
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device.index != device):
+        if t is not None and t.get_device() != device:
             raise ValueError(f"a tensor lies on {t.device}, the context on cuda:{device}")
 
 
@@ -124,6 +140,7 @@ class Context:
         ordering rules hold between this library's kernels and torch's."""
         self.follow_torch_stream = follow_torch_stream
         self._stream_seen = None
+        self._like = None
         self.lib, self.host = L.load(), L.host()
         h = C.c_void_p()
         st = self.lib.lev_cuda_init(device, C.byref(h))
@@ -320,56 +337,62 @@ class Context:
         """lev_norm_residual: (out, h) with out = scale * (residual + alpha * gate * rmsnorm(x) * post) and h = rmsnorm(out) * pre.
         x and residual are f32 [rows][n]; the norm behind the block runs when `post` is given (or norm_post=True: without a scale);
         gate is [n] or [rows][n]; h is f32 or of `dtype` (float16, bfloat16).  out may be residual or x; h=False leaves h out."""
-        import torch
-
-        rows, n = x.shape
-        out = torch.empty_like(residual) if out is None else out
+        torch = _T or _torch()
+        f32, shape = torch.float32, x.shape
+        rows, n = shape
+        if x.dtype is not f32 or residual.dtype is not f32 or residual.shape != shape or not x.is_contiguous() or not residual.is_contiguous():
+            raise ValueError(f"x {tuple(shape)} of {x.dtype}, residual {tuple(residual.shape)} of {residual.dtype}: contiguous float32 of one shape is wanted")
+        if out is None:
+            out = torch.empty_like(residual)
+        elif out.dtype is not f32 or out.shape != shape or not out.is_contiguous():
+            raise ValueError(f"out: contiguous float32 {tuple(shape)} is wanted, got {tuple(out.shape)} of {out.dtype}")
+        ht = L.ELEM_F32
         if h is None:
-            h = torch.empty((rows, n), dtype=dtype or torch.float32, device=x.device)
+            h = torch.empty(shape, dtype=dtype or f32, device=x.device)
         elif h is False:
             h = None
-        _on(self.device, x, residual, post, pre, gate, out, h)
-        for what, t, shape in (("x", x, (rows, n)), ("residual", residual, (rows, n)), ("out", out, (rows, n)), ("post", post, (n,)), ("pre", pre, (n,))):
-            if t is not None and (t.shape != shape or t.dtype is not torch.float32 or not t.is_contiguous()):
-                raise ValueError(f"{what}: contiguous float32 {shape} is wanted, got {tuple(t.shape)} of {t.dtype}")
+        if h is not None:
+            ht = _elem(h, "h", _ANY)
+            if h.shape != shape or not h.is_contiguous():
+                raise ValueError(f"h: contiguous {tuple(shape)} is wanted, got {tuple(h.shape)}")
+        for w in (post, pre):
+            if w is not None and (w.dtype is not f32 or w.numel() != n or not w.is_contiguous()):
+                raise ValueError(f"norm weights: {n} contiguous float32 values are wanted, got {tuple(w.shape)} of {w.dtype}")
         gate_ld = 0
         if gate is not None:
-            if gate.dtype is not torch.float32 or gate.stride(-1) != 1 or tuple(gate.shape) not in ((n,), (rows, n)):
+            if gate.dtype is not f32 or gate.stride(-1) != 1 or tuple(gate.shape) not in ((n,), (rows, n)):
                 raise ValueError(f"gate: float32 ({n},) or ({rows}, {n}) is wanted, got {tuple(gate.shape)} of {gate.dtype}")
             gate_ld = gate.stride(0) if gate.ndim == 2 and rows > 1 else 0
-        ht = L.ELEM_F32
-        if h is not None:
-            ht = _elem(h, "h", "float32 float16 bfloat16")
-            if h.shape != (rows, n) or not h.is_contiguous():
-                raise ValueError(f"h: contiguous {(rows, n)} is wanted, got {tuple(h.shape)}")
+        _on(self.device, x, residual, post, pre, gate, out, h)
         self._flags(False, False)
-        self._check(self.host.norm_residual(self._h, _ptr(x), _ptr(residual), rows, n, int(post is not None if norm_post is None else norm_post),
-                                            _ptr(post), _ptr(gate), gate_ld, alpha, scale, _ptr(pre), eps, _ptr(out), _ptr(h), ht))
+        self._check(self.host.norm_residual(self._h, _dp(x), _dp(residual), rows, n, int(post is not None if norm_post is None else norm_post),
+                                            _dp(post), _dp(gate), gate_ld, alpha, scale, _dp(pre), eps, _dp(out), _dp(h), ht))
         return out, h
 
     def logprobs(self, logits, tokens=None, top: int = 0, softcap: float = 0.0):
         """lev_logprobs over the rows of logits [rows][n] (f32, f16 or bf16; rows may be a stride apart): (logprob of tokens int32 [rows],
         entropy, top_index [rows][top], top_logprob [rows][top]); logprob is None without tokens, the last two without `top`."""
-        import torch
-
+        torch = _T or _torch()
         rows, n = logits.shape
-        if logits.stride(1) != 1:
+        ld, one = logits.stride()
+        if one != 1 and n > 1:
             raise ValueError("logits: rows of contiguous values are wanted")
-        ty = _elem(logits, "logits", "float32 float16 bfloat16")
+        ty = _elem(logits, "logits", _ANY)
         _on(self.device, logits, tokens)
+        if self._like is None:   # makes outputs: new_empty of a tensor costs half of torch.empty with a device
+            self._like = torch.empty(0, device=logits.device), torch.empty(0, dtype=torch.int32, device=logits.device)
+        f32, i32 = self._like
         lp = ids = lps = None
         if tokens is not None:
             _i32(tokens, rows, "tokens")
-        vals = torch.empty((2, rows), dtype=torch.float32, device=logits.device)
-        if tokens is not None:
-            lp = vals[0]
+            lp = f32.new_empty(rows)
+        entropy = f32.new_empty(rows)
         if top > 0:
-            ids = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
-            lps = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
+            ids, lps = i32.new_empty((rows, top)), f32.new_empty((rows, top))
         self._flags(False, False)
-        self._check(self.host.logprobs(self._h, _ptr(logits), ty, rows, n, logits.stride(0) if rows > 1 else n, softcap, _ptr(tokens), top, _ptr(lp),
-                                       _ptr(vals[1]), _ptr(ids), _ptr(lps)))
-        return lp, vals[1], ids, lps
+        self._check(self.host.logprobs(self._h, logits.data_ptr(), ty, rows, n, ld if rows > 1 else n, softcap, _dp(tokens), top, _dp(lp),
+                                       entropy.data_ptr(), _dp(ids), _dp(lps)))
+        return lp, entropy, ids, lps
 
     def qkv_norm_rope(self, qkv, q_heads: int, kv_heads: int, head_dim: int, q_weight=None, k_weight=None, eps: float = 1e-6,
                       inv_freq=None, pos=None):
@@ -541,44 +564,43 @@ class Context:
         """lev_attn_chunk: rows start[c] ... start[c + 1] - 1 of q [rows][q_heads][head_dim] (f32 or f16; rows may be a stride apart)
         are new tokens of sequence slot[c] from position pos[c] on, whose K and V rows are in the cache already -> out of q's
         shape in bf16 (or `dtype` float16); start, slot and pos are int32 device tensors."""
-        import torch
-
+        torch = _T or _torch()
         n = slot.numel()
         if out is None:
             out = torch.empty(q.shape, dtype=dtype or torch.bfloat16, device=q.device)
         _on(self.device, q, out, start, slot, pos, cache.k)
-        q_ld, out_ld = _head_rows(q, "q"), _head_rows(out, "out")
-        if out.shape != q.shape or q.shape[2] != cache.layout.head_dim:
-            raise ValueError(f"q {tuple(q.shape)}, out {tuple(out.shape)}, head dimension {cache.layout.head_dim} of the cache")
+        (shape, q_ld), (out_shape, out_ld) = _head_rows(q, "q"), _head_rows(out, "out")
+        if out_shape != shape or shape[2] != cache.layout.head_dim:
+            raise ValueError(f"q {tuple(shape)}, out {tuple(out_shape)}, head dimension {cache.layout.head_dim} of the cache")
         _i32(start, n + 1, "start")
         _i32(slot, n, "slot")
         _i32(pos, n, "pos")
-        qt, ot = _elem(q, "q", "float32 float16"), _elem(out, "out", "float16 bfloat16")
+        qt, ot = _elem(q, "q", _F32_F16), _elem(out, "out", _ANY16)
         self._flags(False, False)
-        self._check(self.host.attn_chunk(self._h, C.addressof(cache.layout), _ptr(cache.k), _ptr(cache.v), _ptr(cache.table), n, _ptr(start),
-                                         _ptr(slot), _ptr(pos), q.shape[0], q.shape[1], _ptr(q), qt, q_ld, window, scale, _ptr(out), ot, out_ld))
+        self._check(self.host.attn_chunk(self._h, C.addressof(cache.layout), _dp(cache.k), _dp(cache.v), _dp(cache.table), n, _dp(start),
+                                         _dp(slot), _dp(pos), shape[0], shape[1], _dp(q), qt, q_ld, window, scale, _dp(out), ot, out_ld))
         return out
 
     def attn_prompt(self, q, k, v, start, window: int = 0, scale: float = 1.0, out=None):
         """lev_attn_prompt: causal attention of whole prompts packed behind one another; q [rows][q_heads][head_dim], k and v
         [rows][kv_heads][head_dim] of one 16-bit type, rows may be a stride apart (views of a fused projection output);
         start int32 [sequences + 1] on the device."""
-        import torch
-
+        torch = _T or _torch()
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         _on(self.device, q, k, v, out, start)
         n = start.numel() - 1
-        q_ld, k_ld, v_ld, out_ld = _head_rows(q, "q"), _head_rows(k, "k"), _head_rows(v, "v"), _head_rows(out, "out")
-        if out.shape != q.shape or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
-            raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, out {tuple(out.shape)}")
+        (shape, q_ld), (kv_shape, k_ld), (v_shape, v_ld), (out_shape, out_ld) = _head_rows(q, "q"), _head_rows(k, "k"), _head_rows(v, "v"), _head_rows(out, "out")
+        rows, q_heads, hd = shape
+        if out_shape != shape or kv_shape != v_shape or kv_shape[0] != rows or kv_shape[2] != hd:
+            raise ValueError(f"q {tuple(shape)}, k {tuple(kv_shape)}, v {tuple(v_shape)}, out {tuple(out_shape)}")
         _i32(start, n + 1, "start")
-        ty = _elem(q, "q", "float16 bfloat16")
-        if not (q.dtype == k.dtype == v.dtype == out.dtype):
+        ty = _elem(q, "q", _ANY16)
+        if not (q.dtype is k.dtype is v.dtype is out.dtype):
             raise TypeError(f"q, k, v and out are of one type: got {q.dtype}, {k.dtype}, {v.dtype}, {out.dtype}")
         self._flags(False, False)
-        self._check(self.host.attn_prompt(self._h, n, _ptr(start), q.shape[0], q.shape[1], k.shape[1], q.shape[2], ty, _ptr(q), q_ld, _ptr(k), k_ld,
-                                          _ptr(v), v_ld, window, scale, _ptr(out), out_ld))
+        self._check(self.host.attn_prompt(self._h, n, _dp(start), rows, q_heads, kv_shape[1], hd, ty, _dp(q), q_ld, _dp(k), k_ld, _dp(v), v_ld,
+                                          window, scale, _dp(out), out_ld))
         return out
 
     def _matvec_host(self, fn, blocks, out_dim, in_dim, x):

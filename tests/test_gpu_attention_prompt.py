@@ -184,3 +184,217 @@ def test_prompt_windows(ctx, window, heads):
 @pytest.mark.parametrize("heads", [(16, 8, 256), (8, 2, 128)])
 def test_one_long_prompt(ctx, heads):
     run_prompt(ctx, [2500], heads, torch.bfloat16)
+
+
+# ---- values that nothing attends to, indices outside the layout ----
+@pytest.mark.parametrize("junk", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("heads,n,at,window,page", [((16, 8, 256), 70, 300, 0, 16), ((8, 2, 128), 5, 900, 0, 16), ((16, 8, 256), 700, 100, 200, 16),
+                                                    ((8, 2, 128), 700, 130, 100, 16), ((8, 2, 128), 9, 40, 0, 7)])
+def test_unattended_cache_may_hold_anything(ctx, junk, heads, n, at, window, page):
+    """Positions behind the last row and in front of every window, pages no entry names: NaN and infinities there change nothing.  A NaN among
+    the new tokens reaches the rows from its own on (as far as the window), and only those."""
+    qh, kvh, hd = heads
+    P = Paged([at + n], page, kvh, hd, 5)
+    k, v = (t.clone() for t in P.rows(0, at + n))
+    used = P.table[0, :P.need[0]].long()
+    mark = torch.ones(P.k.shape[0], dtype=torch.bool, device=DEV)
+    mark[used] = False
+    for pool in (P.k, P.v):
+        pool[mark] = junk
+        e = int(P.table[0, (at + n - 1) // page])
+        pool[e, (at + n - 1) % page + 1:] = junk          # behind the last position, in its page
+        for p in range(max(0, at + 1 - window) if window else 0):
+            pool[int(P.table[0, p // page]), p % page] = junk
+    q = torch.randn((n, qh, hd), generator=torch.Generator(device=DEV).manual_seed(3), device=DEV)
+    args = (i32([0, n]), i32([0]), i32([at]), q, window, hd ** -0.5)
+    got = ctx.attn_chunk(P.cache, *args)
+    ctx.synchronize()
+    ref, mag = reference(q.half(), k, v, at, window, hd ** -0.5)
+    check(got, ref, mag, torch.float16)
+    first = n // 2
+    pool_v = P.v[int(P.table[0, (at + first) // page])]
+    pool_v[(at + first) % page, 0, 3] = junk
+    got2 = ctx.attn_chunk(P.cache, *args)
+    ctx.synchronize()
+    g = qh // kvh
+    last = min(n, first + window) if window else n
+    hit = got2[first:last, :g, 3].float()
+    assert (hit.isnan() if math.isnan(junk) else hit == junk).all()
+    clean = torch.ones_like(got2, dtype=torch.bool)
+    clean[first:last, :g, 3] = False
+    assert got2[clean].isfinite().all()
+    check(torch.where(clean, got2, got), ref, mag, torch.float16)
+
+
+@pytest.mark.parametrize("heads", [(16, 8, 256), (8, 2, 128)])
+def test_other_prompts_may_hold_anything(ctx, heads):
+    qh, kvh, hd = heads
+    g = torch.Generator(device=DEV).manual_seed(8)
+    x = torch.randn((600, qh + 2 * kvh, hd), generator=g, device=DEV).to(torch.bfloat16)
+    x[200:410] = math.nan
+    q, k, v = x[:, :qh], x[:, qh:qh + kvh], x[:, qh + kvh:]
+    got = ctx.attn_prompt(q, k, v, i32([0, 200, 410, 600]), 0, hd ** -0.5)
+    ctx.synchronize()
+    for a, b in ((0, 200), (410, 600)):
+        ref, mag = reference(q[a:b], k[a:b], v[a:b], 0, 0, hd ** -0.5)
+        check(got[a:b], ref, mag, torch.bfloat16)
+    assert got[200:410].isnan().all()
+
+
+@pytest.mark.parametrize("page", [16, 7])
+@pytest.mark.parametrize("heads", [(16, 8, 256), (8, 2, 128)])
+@pytest.mark.parametrize("kind", ["slot", "slot_negative", "pos", "pos_negative", "entry", "entry_negative"])
+def test_bad_indices_are_reported_and_not_followed(ctx, heads, page, kind):
+    qh, kvh, hd = heads
+    lens, ctxs = [40, 300, 3], [200, 50, 77]
+    P = Paged([a + b for a, b in zip(lens, ctxs)], page, kvh, hd, 9)
+    slot, pos = [0, 1, 2], list(ctxs)
+    if kind == "slot":
+        slot[1] = 3
+    elif kind == "slot_negative":
+        slot[1] = -1
+    elif kind == "pos":
+        pos[1] = P.table.shape[1] * page - 299
+    elif kind == "pos_negative":
+        pos[1] = -1
+    else:
+        P.table[1, 2] = P.k.shape[0] if kind == "entry" else -1
+    q = torch.randn((343, qh, hd), generator=torch.Generator(device=DEV).manual_seed(3), device=DEV)
+    got = ctx.attn_chunk(P.cache, i32([0, 40, 340, 343]), i32(slot), i32(pos), q, 0, hd ** -0.5)
+    with pytest.raises(lev.LevError, match="badDimensions"):
+        ctx.synchronize()
+    ctx.synchronize()   # reported once
+    assert got[40:340].isnan().all()
+    for c, (a, b) in ((0, (0, 40)), (2, (340, 343))):
+        k, v = P.rows(c, lens[c] + ctxs[c])
+        ref, mag = reference(q[a:b].half(), k, v, ctxs[c], 0, hd ** -0.5)
+        check(got[a:b], ref, mag, torch.float16)
+
+
+@pytest.mark.parametrize("starts", [[0, 9, 5, 20], [0, 9, 25, 20], [-1, 9, 9, 20], [0, 9, 9, 21]])
+def test_bad_ranges_are_reported_and_left_out(ctx, starts):
+    x = torch.randn((20, 4, 128), device=DEV).to(torch.float16)
+    out = torch.full((20, 2, 128), 7.0, dtype=torch.float16, device=DEV)
+    ctx.attn_prompt(x[:, :2], x[:, 2:3], x[:, 3:], i32(starts), out=out)
+    with pytest.raises(lev.LevError, match="badDimensions"):
+        ctx.synchronize()
+    good = [(a, b) for a, b in zip(starts, starts[1:]) if 0 <= a <= b <= 20]
+    for r in range(20):
+        assert bool((out[r] == 7.0).all()) == (not any(a <= r < b for a, b in good)), r
+
+
+def test_all_chunks_empty_or_rows_outside(ctx):
+    out = torch.full((30, 2, 128), 7.0, dtype=torch.float16, device=DEV)
+    x = torch.randn((30, 4, 128), device=DEV).to(torch.float16)
+    ctx.attn_prompt(x[:, :2], x[:, 2:3], x[:, 3:], i32([5, 5, 5]), out=out)
+    ctx.synchronize()
+    assert (out == 7.0).all()
+    ctx.attn_prompt(x[:, :2], x[:, 2:3], x[:, 3:], i32([5, 12]), out=out)
+    ctx.synchronize()
+    assert (out[:5] == 7.0).all() and (out[12:] == 7.0).all() and (out[5:12] != 7.0).any(-1).all()
+
+
+@pytest.mark.parametrize("seqs", [33, 150, 1000])
+def test_many_sequences(ctx, seqs):
+    lens = [1 + (7 * i) % 13 for i in range(seqs)]
+    run_prompt(ctx, lens, (8, 2, 128), torch.float16)
+
+
+def test_output_rows_a_stride_apart(ctx):
+    g = torch.Generator(device=DEV).manual_seed(2)
+    x = torch.randn((150, 6, 128), generator=g, device=DEV).to(torch.bfloat16)
+    wide = torch.full((150, 7, 128), 7.0, dtype=torch.bfloat16, device=DEV)
+    got = ctx.attn_prompt(x[:, :4], x[:, 4:5], x[:, 5:], i32([0, 150]), 0, 0.1, out=wide[:, 1:5])
+    ctx.synchronize()
+    ref, mag = reference(x[:, :4], x[:, 4:5], x[:, 5:], 0, 0, 0.1)
+    check(got, ref, mag, torch.bfloat16)
+    assert (wide[:, 0] == 7.0).all() and (wide[:, 5:] == 7.0).all()
+
+
+def test_long_offsets(ctx):
+    """a pool of more than 2^32 bytes: rows of its last blocks"""
+    hd, kvh, page = 256, 8, 64
+    blocks = (5 << 30) // (page * kvh * hd * 2)
+    k = torch.zeros((blocks, page, kvh, hd), dtype=torch.float16, device=DEV)
+    v = torch.zeros_like(k)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    table = i32([[blocks - 1, 3, blocks - 2, blocks - 9]])
+    for e in table[0].tolist():
+        k[e].normal_(generator=g)
+        v[e].normal_(generator=g)
+    q = torch.randn((20, 16, hd), generator=g, device=DEV)
+    got = ctx.attn_chunk(lev.PagedKV.over(k, v, table), i32([0, 20]), i32([0]), i32([230]), q, 0, 1 / 16)
+    ctx.synchronize()
+    e = table[0].long()
+    ref, mag = reference(q.half(), k[e].flatten(0, 1)[:250], v[e].flatten(0, 1)[:250], 230, 0, 1 / 16)
+    check(got, ref, mag, torch.float16)
+
+
+def test_repeats_captures_and_streams(ctx):
+    """the same bits eager, captured and replayed, and from two contexts at once on two streams"""
+    P = Paged([700, 1300], 16, 8, 256, 4)
+    q = torch.randn((300, 16, 256), generator=torch.Generator(device=DEV).manual_seed(3), device=DEV)
+    args = (i32([0, 100, 300]), i32([0, 1]), i32([600, 1100]), q, 0, 1 / 16)
+    few = (i32([0, 2, 5]), i32([0, 1]), i32([690, 1290]), q[:5], 0, 1 / 16)   # merged over a cluster
+    want, want_few = ctx.attn_chunk(P.cache, *args), ctx.attn_chunk(P.cache, *few)
+    for _ in range(3):
+        assert torch.equal(ctx.attn_chunk(P.cache, *args), want) and torch.equal(ctx.attn_chunk(P.cache, *few), want_few)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            a, b = ctx.attn_chunk(P.cache, *args), ctx.attn_chunk(P.cache, *few)
+        a.zero_(), b.zero_()
+        g.replay()
+        g.replay()
+    s.synchronize()
+    assert torch.equal(a, want) and torch.equal(b, want_few)
+    other = lev.Context(0)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    outs = []
+    for _ in range(5):
+        with torch.cuda.stream(s1):
+            outs.append((ctx.attn_chunk(P.cache, *args), want))
+        with torch.cuda.stream(s2):
+            outs.append((other.attn_chunk(P.cache, *few), want_few))
+            outs.append((other.attn_chunk(P.cache, *args), want))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in outs)
+    other.close()
+
+
+def test_agrees_with_the_single_query_form(ctx):
+    P = Paged([400], 16, 8, 256, 11)
+    q = torch.randn((9, 16, 256), generator=torch.Generator(device=DEV).manual_seed(3), device=DEV)
+    one = ctx.attn_decode(P.cache, i32([0] * 9), i32(list(range(391, 400))), q, 0, 1 / 16)
+    got = ctx.attn_chunk(P.cache, i32([0, 9]), i32([0]), i32([391]), q, 0, 1 / 16, dtype=torch.float16)
+    ctx.synchronize()
+    # queries and weights rounded to f16 on one side only: 2^-11 of each score's terms and of each weight
+    assert (got.float() - one).abs().max() <= 6e-3 * one.abs().max()
+
+
+def test_refusals(ctx):
+    P = Paged([64], 16, 2, 128, 1)
+    st, sl, ps = i32([0, 8]), i32([0]), i32([5])
+    q = torch.randn((8, 4, 128), device=DEV)
+    half = q.half()
+    ok = ctx.attn_chunk(P.cache, st, sl, ps, q)
+    assert ok.dtype is torch.bfloat16
+    for e, call in [(TypeError, lambda: ctx.attn_chunk(P.cache, st, sl, ps, q.to(torch.bfloat16))), (TypeError, lambda: ctx.attn_chunk(P.cache, st, sl, ps, q, out=q.clone())),
+                    (ValueError, lambda: ctx.attn_chunk(P.cache, st.long(), sl, ps, q)), (ValueError, lambda: ctx.attn_chunk(P.cache, sl, sl, ps, q)),
+                    (ValueError, lambda: ctx.attn_chunk(P.cache, st, sl, ps, q.transpose(0, 1))), (ValueError, lambda: ctx.attn_chunk(P.cache, st, sl, ps, q[..., :64])),
+                    (ValueError, lambda: ctx.attn_chunk(P.cache, st, sl, ps, q.cpu())), (lev.LevError, lambda: ctx.attn_chunk(P.cache, st, sl, ps, q[:, :3].contiguous())),
+                    (lev.LevError, lambda: ctx.attn_chunk(P.cache, st, sl, ps, q, window=-1)), (lev.LevError, lambda: ctx.attn_chunk(P.cache, st, sl, ps, q, scale=math.inf)),
+                    (lev.LevError, lambda: ctx.attn_chunk(P.cache, st, sl, ps, torch.randn((8, 34, 128), device=DEV))),
+                    (lev.LevError, lambda: ctx.attn_chunk(P.cache, st, sl, ps, half, out=half)),
+                    (lev.LevError, lambda: ctx.attn_chunk(P.cache, st, sl, ps, torch.randn(8 * 512 + 1, device=DEV)[1:].view(8, 4, 128))),
+                    (lev.LevError, lambda: ctx.attn_chunk(P.cache, st, sl, ps, torch.randn((8, 513), device=DEV)[:, :512].unflatten(1, (4, 128)))),
+                    (TypeError, lambda: ctx.attn_prompt(half, half[:, :2], half[:, :2].to(torch.bfloat16), st)), (TypeError, lambda: ctx.attn_prompt(q, q[:, :2], q[:, :2], st)),
+                    (ValueError, lambda: ctx.attn_prompt(half, half[:7, :2], half[:7, :2], st)), (lev.LevError, lambda: ctx.attn_prompt(half, half[:, :3], half[:, :3], st)),
+                    (lev.LevError, lambda: ctx.attn_prompt(half[..., :64].contiguous(), half[:, :2, :64].contiguous(), half[:, :2, :64].contiguous(), st)),
+                    (lev.LevError, lambda: ctx.attn_prompt(half, half[:, :2], half[:, 2:], st, out=half)),
+                    (ValueError, lambda: lev.PagedKV.over(P.k, P.v[:, :8], P.table)), (TypeError, lambda: lev.PagedKV.over(P.k.to(torch.bfloat16), P.v.to(torch.bfloat16), P.table)),
+                    (ValueError, lambda: lev.PagedKV.over(P.k, P.v, P.table.long()))]:
+        with pytest.raises(e):
+            call()
+    ctx.synchronize()

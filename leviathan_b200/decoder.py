@@ -9,6 +9,10 @@ to the host every layer (Gemma4.swift:3796-3809, :3637-3641), every step here st
 token ids, positions and slots are device tensors, so the whole step is captured as one CUDA graph and
 a replay is one decoded token per sequence with the next token id already in place.
 
+Prompts go through the same layers many rows at a time (`prompts=True`): `prefill` takes new tokens of several sequences into their
+caches, whole or piece by piece, and leaves the next token's logits; `score` gives the log probability of every token of whole prompts
+without a cache.
+
 Weights are random (seeded SplitMix64 normals, sigma 0.02, quantized with this package's encoders);
 caches are filled with N(0, 1) values up to the last position.  torch holds the buffers and the
 graph; every arithmetic step is a kernel of libleviathan_cuda.so.
@@ -89,15 +93,21 @@ class SyntheticDecoder:
     `batch` sequences (their caches differ by rank, the weights do not), attention and the head are local, and
     the experts are sharded -- rank r keeps experts [r * E / world, (r + 1) * E / world) -- so the MoE of a step
     is the expert-parallel layer: tokens go to the ranks that hold their experts and the expert rows come back
-    to be combined in slot order on the token's rank."""
+    to be combined in slot order on the token's rank.
+
+    `prompts=True` keeps what prompts need beside the decode step: the tensors' GGUF-order copies (lev_gemm_prefill wants them) and, for
+    narrow batches, a fused [q | k | v] tensor; one GPU only."""
 
     def __init__(self, ctx: Context, cfg: DecoderConfig, batch: int = 1, device="cuda", norm_sigma: float = 0.02,
-                 keep_host_copies: bool = False, gemm_from: int = 16, rank: int = 0, world: int = 1):
+                 keep_host_copies: bool = False, gemm_from: int = 16, rank: int = 0, world: int = 1, prompts: bool = False):
         import torch
 
         self.ctx, self.cfg, self.batch, self.dev = ctx, cfg, batch, device
         self.wide = batch >= gemm_from
         self.rank, self.world = rank, world
+        if prompts and world > 1:
+            raise ValueError("prompts run on one GPU")
+        self.prompts = prompts
         if cfg.experts % world:
             raise ValueError(f"{cfg.experts} experts do not split over {world} ranks")
         H, QH, KVH, HD = cfg.hidden, cfg.q_heads, cfg.kv_heads, cfg.head_dim
@@ -115,12 +125,14 @@ class SyntheticDecoder:
                 wqkv = ctx.upload(torch.cat(parts), cfg.weight_type, (QH + 2 * KVH) * HD, H)
                 del parts
             else:
-                wq = self._tensor(f"blk.{l}.attn_q", cfg.weight_type, QH * HD, H)
-                wk = self._tensor(f"blk.{l}.attn_k", cfg.weight_type, KVH * HD, H)
-                wv = self._tensor(f"blk.{l}.attn_v", cfg.weight_type, KVH * HD, H)
+                parts = [self._blocks(f"blk.{l}.attn_{n}", cfg.weight_type, h * HD, H) for n, h in (("q", QH), ("k", KVH), ("v", KVH))]
+                wq, wk, wv = (ctx.upload(b, cfg.weight_type, h * HD, H) for b, h in zip(parts, (QH, KVH, KVH)))
+                if prompts:
+                    wqkv = ctx.upload(torch.cat(parts), cfg.weight_type, (QH + 2 * KVH) * HD, H)
+                del parts
             wo = self._tensor(f"blk.{l}.attn_output", cfg.weight_type, H, QH * HD)
             if not self.wide:
-                for w in (wq, wk, wv, wo):
+                for w in (wq, wk, wv) if prompts else (wq, wk, wv, wo):
                     w.release_gguf()   # only the decode kernels read these: one resident copy instead of two
             moe = self._experts(l)
             cache = PagedKV(batch * blocks_per_seq + 1, cfg.page, KVH, HD, slots=batch, max_blocks=blocks_per_seq, dtype="f16", device=device)
@@ -199,7 +211,7 @@ class SyntheticDecoder:
             self.host[f"blk.{l}.ffn_down_exps"] = dn.cpu().numpy()
             self.host[f"blk.{l}.ffn_gate_inp"] = router.cpu().numpy()
         moe = self.ctx.moe_upload(router, gu, dn, E, H, I, first, per)
-        if self.batch * self.world * c.top_k < 512:
+        if self.batch * self.world * c.top_k < 512 and not self.prompts:
             moe.release_gguf()   # decode-sized calls read the repacked experts only: one resident copy
         return moe
 
@@ -273,6 +285,74 @@ class SyntheticDecoder:
                 ctx.matvec_fused(self.head, x[a:b], "rmsnorm", self.out_norm, c.eps, out=self.logits[a:b])
         ctx.softcap(self.logits, c.softcap)
         ctx.argmax_into(self.logits, self.tok)
+
+    # ---- prompts ----
+    def _rows_of(self, start, n: int):
+        """for each of n rows: its chunk and its number inside the chunk"""
+        import torch
+
+        row = torch.arange(n, device=self.dev)
+        chunk = torch.bucketize(row, start[1:].long(), right=True)
+        return chunk, (row - start.long()[chunk]).to(torch.int32)
+
+    def _layers_of_prompt(self, tokens, attend):
+        """Embedding rows, all layers and the final norm over rows of tokens -> bf16 [rows][hidden].  `attend(layer, qkv)` gives a
+        layer's attention output, bf16 [rows][q_heads][head_dim], from the fused projection's f32 rows."""
+        import torch
+
+        c, ctx, n = self.cfg, self.ctx, tokens.numel()
+        if not self.prompts:
+            raise ValueError("the decoder was made without prompts=True")
+        bf16 = torch.bfloat16
+        x = ctx.embed_rows(self.head, tokens, math.sqrt(c.hidden))
+        h = ctx.act_bf16(ctx.rmsnorm(x, self.layers[0].attn_norm, c.eps))
+        nexts = [L.attn_norm for L in self.layers[1:]] + [self.out_norm]
+        for L, norm in zip(self.layers, nexts):
+            a = attend(L, ctx.gemm_prefill(L.wqkv, h))
+            o = ctx.gemm_prefill(L.wo, a.view(n, c.q_heads * c.head_dim))
+            x, f = ctx.norm_residual(o, x, pre=L.ffn_norm, eps=c.eps, out=x)
+            o = ctx.moe_layer(L.moe, f, c.top_k)
+            x, h = ctx.norm_residual(o, x, pre=norm, eps=c.eps, out=x, dtype=bf16)
+        return h
+
+    def prefill(self, tokens, start, slot, pos):
+        """Takes new tokens into the caches: rows start[i] ... start[i + 1] - 1 of `tokens` (int32) continue sequence slot[i] at position
+        pos[i] (int32 device tensors; at least one token each).  Returns (next tokens int32 [chunks], softcapped logits [chunks][vocab]) behind
+        each chunk's last token: what the Rust runtime's prefill_advance leaves (rust/crates/lev-model/src/gpu.rs:1346)."""
+        import torch
+
+        c, ctx = self.cfg, self.ctx
+        chunk, within = self._rows_of(start, tokens.numel())
+        row_slot, row_pos = slot[chunk].contiguous(), pos[chunk] + within
+
+        def attend(L, qkv):
+            ctx.qkv_norm_rope_append(qkv, c.q_heads, L.cache, row_slot, row_pos, L.q_norm, L.k_norm, c.eps, self.inv_freq)
+            q = qkv.view(-1, c.q_heads + 2 * c.kv_heads, c.head_dim)[:, :c.q_heads]
+            return ctx.attn_chunk(L.cache, start, slot, pos, q, 0, c.attn_scale)
+
+        h = self._layers_of_prompt(tokens, attend)
+        logits = ctx.softcap(ctx.gemm_prefill(self.head, h.index_select(0, start[1:].long() - 1)), c.softcap)
+        return ctx.argmax(logits), logits
+
+    def score(self, tokens, start, top: int = 0, rows: int = 512):
+        """Whole prompts packed behind one another, no cache: for every row the log probability of the next token of its prompt (0 behind a
+        prompt's last token), the entropy of the prediction and its `top` alternatives (see Context.logprobs).  Logits are made `rows` rows at a time."""
+        import torch
+
+        c, ctx, n = self.cfg, self.ctx, tokens.numel()
+        _, within = self._rows_of(start, n)
+
+        def attend(L, qkv):
+            ctx.qkv_norm_rope(qkv, c.q_heads, c.kv_heads, c.head_dim, L.q_norm, L.k_norm, c.eps, self.inv_freq, within)
+            b = ctx.act_bf16(qkv).view(n, c.q_heads + 2 * c.kv_heads, c.head_dim)
+            return ctx.attn_prompt(b[:, :c.q_heads], b[:, c.q_heads:c.q_heads + c.kv_heads], b[:, c.q_heads + c.kv_heads:], start, 0, c.attn_scale)
+
+        h = self._layers_of_prompt(tokens, attend)
+        given = torch.full_like(tokens, -1)
+        given[:-1] = tokens[1:]
+        given[start[1:].long() - 1] = -1   # nothing follows a prompt's last token
+        parts = [ctx.logprobs(ctx.gemm_prefill(self.head, h[a:a + rows]), given[a:a + rows], top=top, softcap=c.softcap) for a in range(0, n, rows)]
+        return tuple(None if p[0] is None else torch.cat(p) for p in zip(*parts))
 
     def capture(self, advance: bool = False):
         """Records `step` as one CUDA graph on the context's stream; `replay()` then decodes a token."""

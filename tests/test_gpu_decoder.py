@@ -124,3 +124,89 @@ def test_decoder_step_against_the_f64_oracle_eager_and_as_one_graph(ctx, batch):
         ctx.synchronize()
         assert np.array_equal(dec.tok.cpu().numpy(), second)
         dec.free()
+
+
+# ---- prompts: the operators together, as a serving loop runs them ----
+PROMPT = dict(SMALL, top_k=8, positions=176)   # every expert takes part: no near-tie of the router falls the other way
+
+
+def _walk(dec, cfg, tokens):
+    """the oracle's steps over a prompt from an empty cache: one dict per token"""
+    kc = [np.zeros((cfg.positions, cfg.kv_heads, cfg.head_dim), np.float16) for _ in dec.layers]
+    vc = [np.zeros_like(k) for k in kc]
+    return [O.decode_step_f64(cfg, dec.host, int(t), p, kc, vc) for p, t in enumerate(tokens)]
+
+
+def _near(got, want):
+    # projections and experts' inputs in bf16, as in a wide decode step: the same bar
+    err = np.max(np.abs(got - want)) / max(1.0, float(np.max(np.abs(want))))
+    assert err < 2e-2, err
+
+
+@pytest.mark.parametrize("batch", [2, 17])
+def test_prompt_pieces_and_decode_steps_against_the_f64_oracle(ctx, batch):
+    """two prompts taken in by pieces (one whole, one in three pieces, pieces of both in one call), then a decode step on top"""
+    cfg = DecoderConfig(**PROMPT)
+    dec = SyntheticDecoder(ctx, cfg, batch=batch, keep_host_copies=True, prompts=True)
+    rng = np.random.default_rng(3)
+    prompts = [rng.integers(0, cfg.vocab, 23), rng.integers(0, cfg.vocab, 61)]
+    refs = [_walk(dec, cfg, p) for p in prompts]
+    i32 = lambda v: torch.tensor(np.asarray(v), dtype=torch.int32, device="cuda")  # noqa: E731
+    pieces = [[(1, 0, 20)], [(0, 0, 23), (1, 20, 59)], [(1, 59, 61)]]   # (sequence, from, to) of each call
+    for call in pieces:
+        toks = np.concatenate([prompts[s][a:b] for s, a, b in call])
+        start = np.concatenate([[0], np.cumsum([b - a for _, a, b in call])])
+        nxt, logits = dec.prefill(i32(toks), i32(start), i32([s for s, _, _ in call]), i32([a for _, a, _ in call]))
+        ctx.synchronize()
+        for i, (s, a, b) in enumerate(call):
+            _near(logits[i].cpu().numpy(), refs[s][b - 1]["logits"])
+            assert int(nxt[i]) == int(torch.argmax(logits[i]))
+    # a decode step continues both sequences from the caches that the prompts left
+    dec.tok[:2] = i32([5, 9])
+    dec.pos[:2] = i32([23, 61])
+    want = [_walk(dec, cfg, list(prompts[s]) + [t])[-1]["logits"] for s, t in ((0, 5), (1, 9))]
+    dec.step()
+    ctx.synchronize()
+    for s in range(2):
+        _near(dec.logits[s].cpu().numpy(), want[s])
+    dec.free()
+
+
+def test_scored_prompts_against_the_f64_oracle(ctx):
+    cfg = DecoderConfig(**PROMPT)
+    dec = SyntheticDecoder(ctx, cfg, batch=1, keep_host_copies=True, prompts=True)
+    rng = np.random.default_rng(4)
+    prompts = [rng.integers(0, cfg.vocab, n) for n in (1, 37, 18)]
+    toks = torch.tensor(np.concatenate(prompts), dtype=torch.int32, device="cuda")
+    start = torch.tensor(np.concatenate([[0], np.cumsum([len(p) for p in prompts])]), dtype=torch.int32, device="cuda")
+    lp, ent, ids, lps = dec.score(toks, start, top=3, rows=40)
+    ctx.synchronize()
+    row = 0
+    for p in prompts:
+        for i, r in enumerate(_walk(dec, cfg, p)):
+            want = torch.log_softmax(torch.from_numpy(r["logits"]), 0)
+            # a log probability moves by at most twice what the logits are off by (2e-2 of the largest)
+            tol = 2 * 2e-2 * max(1.0, float(np.max(np.abs(r["logits"]))))
+            if i + 1 < len(p):
+                assert abs(float(lp[row]) - float(want[int(p[i + 1])])) <= tol
+            else:
+                assert float(lp[row]) == 0.0
+            assert torch.all((lps[row].cpu() - want[ids[row].cpu().long()]).abs() <= tol)
+            assert abs(float(ent[row]) + float((want.exp() * want).sum())) <= 2 * tol * float(want.abs().max())
+            row += 1
+    # the same rows through the caches: log probabilities of the last rows agree
+    _, logits = dec.prefill(toks[1:38], torch.tensor([0, 37], dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda"),
+                            torch.zeros(1, dtype=torch.int32, device="cuda"))
+    again = ctx.logprobs(logits, None, top=3)
+    ctx.synchronize()
+    # f16 cache and queries on one side, bf16 on the other: 2^-8 of a logit's size through two layers
+    assert (again[3][0] - lps[37]).abs().max() <= 4e-2 * max(1.0, float(logits.abs().max()))
+    dec.free()
+
+
+def test_prompts_are_refused_without_their_tensors(ctx):
+    dec = SyntheticDecoder(ctx, DecoderConfig(**SMALL), batch=1)
+    one = torch.zeros(1, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="prompts=True"):
+        dec.prefill(one, torch.tensor([0, 1], dtype=torch.int32, device="cuda"), one, one)
+    dec.free()

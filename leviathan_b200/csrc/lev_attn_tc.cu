@@ -18,7 +18,7 @@
 // f16, and both operands of an MMA have one type), P (11 bits for f16, 8 for bf16 prompts), the output.
 //
 // Roles of a CTA: one (two) softmax warpgroup(s), one warp that issues MMAs, one that issues TMA boxes; where the cache
-// cannot be boxed (f32 pools, page sizes that neither divide 128 nor are multiples of it) the last three warps of the
+// cannot be boxed (f32 pools, pages that are no whole groups of eight rows) the last three warps of the
 // CTA copy and convert rows instead.  Every wait is bounded (about a second, then LEV_TIMEOUT).
 //
 // Places that a row does not attend to may hold anything, NaN included.  Scores there are replaced, but 0 * NaN is NaN
@@ -242,10 +242,10 @@ __device__ bool tc_find(const TcArgs& A, int u, int per, int lane, TcUnit* U) {
 }
 
 // layout of a stage of `rows` x `cols`: boxes of pages are whole rows of atoms, boxes of packed rows and copied rows slabs
-__device__ __forceinline__ TcLayout tc_layout(const TcArgs& A, int rows, int cols) {
+__device__ __forceinline__ TcLayout tc_layout(bool pages, int rows, int cols) {
     TcLayout L;
-    L.group = A.box_k > 0 && A.table ? (unsigned)cols * 16u : 1024u;
-    L.slab = A.box_k > 0 && A.table ? 1024u : (unsigned)rows * 128u;
+    L.group = pages ? (unsigned)cols * 16u : 1024u;
+    L.slab = pages ? 1024u : (unsigned)rows * 128u;
     return L;
 }
 
@@ -410,6 +410,11 @@ __device__ __forceinline__ void tc_load_q(const TcArgs& A, const TcUnit& U, unsi
     __syncwarp();
 }
 
+// where a step's rows lie (see `entries` in the kernel)
+struct TcRows {
+    int64_t off[4];
+};
+
 // The hardware hands a running cluster the next one of the grid that has not started: `request` asks (the answer, 16 bytes, arrives
 // at `bar`), `taken` reads it: the first CTA's index in x, or -1 when all have started.  Not to be asked again after that.
 __device__ __forceinline__ void tc_next_request(unsigned answer, unsigned bar) {
@@ -439,10 +444,11 @@ struct TcDims {
     static constexpr size_t kSmem = 1024 + TILES * kQTile + (size_t)kStages * TC_STAGE;
 };
 
-// HD: head dimension.  TYPE: what the tensor core multiplies (LEV_ELEM_F16 or LEV_ELEM_BF16).  TILES: 128-row tiles of a CTA, each with a softmax warpgroup; one tile has two S buffers, two
+// HD: head dimension.  TYPE: what the tensor core multiplies (LEV_ELEM_F16 or LEV_ELEM_BF16).  COPY: K and V rows are copied by
+// warps (kernels of their own: with both ways in one, 32 heads of 128 lost 5 % to the registers of the one not taken).  TILES: 128-row tiles of a CTA, each with a softmax warpgroup; one tile has two S buffers, two
 // tiles have one each.  CG = 2: a pair of CTAs (cta_group::2) with one tile each that share K and V.  splits > 1: the
 // CTAs of a cluster take parts of the positions and merge through distributed shared memory.
-template <int HD, int TILES, int CG, int TYPE>
+template <int HD, int TILES, int CG, int TYPE, bool COPY>
 __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
     k_attn_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap,
               const __grid_constant__ TcArgs A) {
@@ -467,12 +473,11 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
     const int split = (int)in_cluster / CG, per = A.tpt * TILES * CG;
     const unsigned smem = (smem_u32(smem_dyn) + 1023u) & ~1023u;
     const unsigned ring = smem + TILES * D::kQTile;
-    const int tma = A.box_k > 0;
     if (threadIdx.x == 0) {
         abort_s = 0;
         bad_s[0] = bad_s[1] = 0;
         for (int s = 0; s < NS; s++) {
-            mbar_init(smem_u32(&full[s]), tma ? 1 : TC_LOAD_WARPS);
+            mbar_init(smem_u32(&full[s]), COPY ? TC_LOAD_WARPS : 1);
             mbar_init(smem_u32(&empty[s]), 1);
         }
         for (int s = 0; s < 2; s++) {
@@ -745,7 +750,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
             const unsigned m_field = (unsigned)((128 * CG) >> 4) << 24;
             const unsigned id_qk = (1u << 4) | fmt | ((128u >> 3) << 17) | m_field;
             const unsigned id_pv = (1u << 4) | fmt | (1u << 16) | ((unsigned)((CG == 2 ? HD : 128) >> 3) << 17) | m_field;   // B is N-major
-            const TcLayout kl = tc_layout(A, 128 / CG, HD / KV_STAGES), vl = tc_layout(A, 128, 128);
+            const TcLayout kl = tc_layout(!COPY && A.table, 128 / CG, HD / KV_STAGES), vl = tc_layout(!COPY && A.table, 128, 128);
             Ring kr(NS), vr(NS);   // stages of the next K and of the next V tile
             auto qk = [&](int tile, int slot_i, bool release) {   // S[slot] = Q[tile] K^T
                 Ring st = kr;
@@ -843,34 +848,49 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         const unsigned full_c = CG == 2 ? map_to_rank(smem_u32(&full[0]), lead) : smem_u32(&full[0]);
         Ring st(NS);
         const bool more = A.splits == 1;   // a cluster that merges has one unit
-        int units = 0;
+        int units = 0, under_way = 0;   // under_way: stages whose copies have not been handed over, from `landed` on
+        Ring landed(NS);
         if (more && have && w == 0 && rank == 0 && lane == 0) tc_next_request(smem_u32(answer_s), smem_u32(&answer_bar));
         for (int k = 0; have; k++) {
             units++;
             const int n = U.n, jb = U.jb, p_last = U.p_last();
             const int32_t* trow = A.table ? A.table + (int64_t)U.slot * A.max_blocks : nullptr;
             const int page_lo = trow ? U.lo / A.page : 0, page_hi = trow ? p_last / A.page : 0;
-            // Lane l: the table entry of the step's page l.  Pages that no row attends to are filled with zeros, not read.
+            auto entry_of = [&](int pg) {   // of a page that some row attends to; A.blocks where it lies outside the pool
+                const int e = trow[pg];
+                if (e >= 0 && e < A.blocks) return e;
+                atomicOr(A.status, LEV_DEV_BAD_INDEX);
+                bad_s[k & 1] = k + 1;
+                return (int)A.blocks;
+            };
+            // Where a step's rows lie.  Boxes: lane l has box l's block and first group of eight rows; pages that no row attends to are
+            // filled with zeros, not read.  Copies: lane l has the byte offsets of rows l, l + 32, ... (negative: zeros).
             auto entries = [&](int i) {
-                int e = (int)A.blocks;
-                if (tma && trow && i < n) {
-                    const int pg = (jb + i) * TC_KV / A.page + lane;
-                    if (lane * A.box_v < TC_KV && pg >= page_lo && pg <= page_hi) {
-                        e = trow[pg];
-                        if (e < 0 || e >= A.blocks) {
-                            atomicOr(A.status, LEV_DEV_BAD_INDEX);
-                            bad_s[k & 1] = k + 1;
-                            e = (int)A.blocks;
+                TcRows R;
+#pragma unroll
+                for (int q = 0; q < 4; q++) R.off[q] = -1;
+                if (trow && i < n) {
+                    const int c0 = (jb + i) * TC_KV;
+                    if (!COPY) {
+                        const int at = c0 + lane * A.box_v, pg = at / A.page;
+                        R.off[0] = A.blocks;
+                        if (lane * A.box_v < TC_KV && pg >= page_lo && pg <= page_hi) R.off[0] = (int64_t)((at - pg * A.page) >> 3) << 32 | (unsigned)entry_of(pg);
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            const int at = c0 + 32 * q + lane, pg = at / A.page;
+                            if (at < U.lo || at > p_last) continue;
+                            const int e = entry_of(pg);
+                            if (e < A.blocks) R.off[q] = LEV_KV_ROW(e, at - pg * A.page, U.kvh, A.page, A.kv_heads) * (int64_t)(HD * (A.kv_type == TC_F32 ? 4 : 2));
                         }
                     }
                 }
                 __syncwarp();
-                return e;
+                return R;
             };
             // boxes of a step's K or V; three warps share a stage's
-            auto boxes = [&](int i, bool is_v, int entry) {
+            auto boxes = [&](int i, bool is_v, const TcRows& R) {
                 const CUtensorMap* map = is_v ? &vmap : &kmap;
-                const int c0 = (jb + i) * TC_KV;
                 const int r_first = CG == 2 && !is_v ? (int)rank * 64 : 0, r_n = CG == 2 && !is_v ? 64 : 128;   // rows of this CTA
                 constexpr int kSlabsV = 2, kSlabsK = CG == 2 ? HD / 64 : 2;
                 const int box = is_v ? A.box_v : A.box_k;
@@ -883,67 +903,89 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                     const int x0 = CG == 2 ? (is_v ? (int)rank * 128 : 0) : h * 128;
                     if (trow) {
                         const int slab = (U.kvh * HD + x0) >> 6;
-                        const int in_page = A.page >= TC_KV ? (c0 + r_first) % A.page >> 3 : 0;   // first group of eight rows
-                        for (int r = w * box; r < r_n; r += TC_LOAD_WARPS * box)
-                            tc_box_page<CG>(dst + (unsigned)r * row_bytes, map, slab, in_page, __shfl_sync(0xffffffffu, entry, (r_first + r) / A.box_v), bar, elected);
+                        for (int r = w * box; r < r_n; r += TC_LOAD_WARPS * box) {
+                            const int at = r_first + r, l = at / A.box_v;
+                            const int block = (int)__shfl_sync(0xffffffffu, (unsigned)R.off[0], l), group = __shfl_sync(0xffffffffu, (int)(R.off[0] >> 32), l);
+                            tc_box_page<CG>(dst + (unsigned)r * row_bytes, map, slab, group + ((at - l * A.box_v) >> 3), block, bar, elected);
+                        }
                     } else {
                         for (int b = w; b < (is_v ? kSlabsV : kSlabsK); b += TC_LOAD_WARPS)
-                            tc_box_rows<CG>(dst + (unsigned)(b * r_n) * 128u, map, x0 + 64 * b, U.kvh, U.row0 + c0 + r_first, bar, elected);
+                            tc_box_rows<CG>(dst + (unsigned)(b * r_n) * 128u, map, x0 + 64 * b, U.kvh, U.row0 + (jb + i) * TC_KV + r_first, bar, elected);
                     }
                     st.step(1);
                 }
             };
-            // rows copied (and converted): pages of any size, f32 pools (never in pairs)
-            auto copies = [&](int i, bool is_v) {
-                const int c0 = (jb + i) * TC_KV;
+            // Rows copied by warps: pages that are no whole groups of eight rows, f32 pools (never in pairs).  f16 rows by asynchronous
+            // copies, three stages under way: a stage is handed over when its copies have landed, two stages later.
+            auto hand_over = [&]() {
+                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&full[landed.s]));
+                landed.step(1);
+                under_way--;
+            };
+            auto copies = [&](bool is_v, const TcRows& R) {
+                const int piece = lane & 15, sub = lane >> 4;   // two rows of 16 pieces (8 values each) per step of a warp
+                const char* pool = static_cast<const char*>(is_v ? A.v : A.k);
                 for (int h = 0; h < KV_STAGES; h++) {
                     pk_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
-                    const unsigned dst = ring + (unsigned)st.s * TC_STAGE;
-                    // two rows of 16 pieces (8 values each) per step of a warp
-                    const int piece = lane & 15, sub = lane >> 4;
-                    for (int r0 = 2 * w; r0 < 128; r0 += 2 * TC_LOAD_WARPS * 4) {
-                        uint4 v[4];
+                    const unsigned dst = ring + (unsigned)st.s * TC_STAGE + (unsigned)(piece >> 3) * 16384u;
+                    auto row = [&](int r, int64_t* off) {
+                        const int64_t v = (r >> 5) == 0 ? R.off[0] : (r >> 5) == 1 ? R.off[1] : (r >> 5) == 2 ? R.off[2] : R.off[3];
+                        *off = __shfl_sync(0xffffffffu, v, (r & 30) + sub);   // r is even: both rows are in one group of 32
+                        return dst + (unsigned)(r + sub) * 128u + (unsigned)(((piece & 7) ^ ((r + sub) & 7)) << 4);
+                    };
+                    if (A.kv_type != TC_F32) {
+                        for (int r = 2 * w; r < 128; r += 2 * TC_LOAD_WARPS) {
+                            int64_t off;
+                            const unsigned to = row(r, &off);
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to), "l"(pool + (off < 0 ? 0 : off + (h * 16 + piece) * 16)),
+                                         "r"(off < 0 ? 0 : 16)
+                                         : "memory");
+                        }
+                        asm volatile("cp.async.commit_group;\n" ::: "memory");
+                        under_way++;
+                        if (under_way == 3) {
+                            asm volatile("cp.async.wait_group 2;\n" ::: "memory");
+                            hand_over();
+                        }
+                    } else {
+                        constexpr int kRowsAtOnce = 4;
+                        for (int r0 = 2 * w; r0 < 128; r0 += 2 * TC_LOAD_WARPS * kRowsAtOnce) {
+                            float4 a[kRowsAtOnce], b[kRowsAtOnce];
+                            unsigned to[kRowsAtOnce];
 #pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            const int r = r0 + q * 2 * TC_LOAD_WARPS + sub, at = c0 + r;
-                            v[q] = make_uint4(0u, 0u, 0u, 0u);
-                            if (r < 128 && at >= U.lo && at <= p_last) {
-                                const unsigned char* src = tc_row(A, U, HD, at, is_v);
-                                if (!src) {
-                                    atomicOr(A.status, LEV_DEV_BAD_INDEX);
-                                    bad_s[k & 1] = k + 1;
-                                } else if (A.kv_type == TC_F32) {
-                                    const float4* f = reinterpret_cast<const float4*>(src) + (h * 16 + piece) * 2;
-                                    const float4 a = f[0], b = f[1];
-                                    v[q] = make_uint4(pack16(a.x, a.y, TC_F16), pack16(a.z, a.w, TC_F16), pack16(b.x, b.y, TC_F16), pack16(b.z, b.w, TC_F16));
-                                } else {
-                                    v[q] = *(reinterpret_cast<const uint4*>(src) + h * 16 + piece);
+                            for (int q = 0; q < kRowsAtOnce; q++) {
+                                const int r = r0 + q * 2 * TC_LOAD_WARPS;
+                                int64_t off = -1;
+                                to[q] = row(r < 128 ? r : 0, &off);
+                                a[q] = b[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+                                if (r < 128 && off >= 0) {
+                                    const float4* f = reinterpret_cast<const float4*>(pool + off) + (h * 16 + piece) * 2;
+                                    a[q] = f[0];
+                                    b[q] = f[1];
                                 }
                             }
-                        }
 #pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            const int r = r0 + q * 2 * TC_LOAD_WARPS + sub;
-                            if (r < 128)
-                                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst + (unsigned)(piece >> 3) * 16384u + (unsigned)r * 128u +
-                                                                                                (unsigned)(((piece & 7) ^ (r & 7)) << 4)),
-                                             "r"(v[q].x), "r"(v[q].y), "r"(v[q].z), "r"(v[q].w)
-                                             : "memory");
+                            for (int q = 0; q < kRowsAtOnce; q++)
+                                if (r0 + q * 2 * TC_LOAD_WARPS < 128)
+                                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(to[q]), "r"(pack16(a[q].x, a[q].y, TC_F16)), "r"(pack16(a[q].z, a[q].w, TC_F16)),
+                                                 "r"(pack16(b[q].x, b[q].y, TC_F16)), "r"(pack16(b[q].z, b[q].w, TC_F16))
+                                                 : "memory");
                         }
+                        under_way++;
+                        hand_over();
                     }
-                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&full[st.s]));
                     st.step(1);
                 }
             };
-            auto load = [&](int i, bool is_v, int entry) {
-                if (tma) boxes(i, is_v, entry);
-                else copies(i, is_v);
+            auto load = [&](int i, bool is_v, const TcRows& R) {
+                if constexpr (COPY) copies(is_v, R);
+                else boxes(i, is_v, R);
             };
-            int e_now = entries(0), e_before = 0;
+            TcRows e_now = entries(0), e_before = e_now;
             for (int i = 0; i <= n; i++) {
-                const int e_next = entries(i + 1);   // read a step ahead
+                const TcRows e_next = entries(i + 1);   // read a step ahead
                 if (i < n) load(i, false, e_now);
                 if (i == 0) {
                     // This unit's queries, when the last product that read the ones before is done.  The first K tile has been asked
@@ -974,6 +1016,10 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 }
                 e_before = e_now;
                 e_now = e_next;
+            }
+            if (COPY && under_way) {
+                asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+                while (under_way) hand_over();
             }
             if (!more) break;
             // ---- the next unit ----
@@ -1129,12 +1175,12 @@ TcPlan tc_plan(const lev_ctx* ctx, int64_t rows, int seqs, int kv_heads, int tpt
     return P;
 }
 
-template <int HD, int TILES, int CG, int TYPE>
+template <int HD, int TILES, int CG, int TYPE, bool COPY = false>
 int tc_launch(lev_ctx* ctx, const CUtensorMap& kmap, const CUtensorMap& vmap, const CUtensorMap& qmap, const TcArgs& A, int64_t units) {
     using D = TcDims<HD, TILES>;
     static bool configured[16] = {};
     if (!configured[ctx->device & 15]) {
-        LEV_CUDA(ctx, cudaFuncSetAttribute(k_attn_tc<HD, TILES, CG, TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)D::kSmem));
+        LEV_CUDA(ctx, cudaFuncSetAttribute(k_attn_tc<HD, TILES, CG, TYPE, COPY>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)D::kSmem));
         configured[ctx->device & 15] = true;
     }
     const int cluster = CG * A.splits;
@@ -1151,7 +1197,7 @@ int tc_launch(lev_ctx* ctx, const CUtensorMap& kmap, const CUtensorMap& vmap, co
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
-    LEV_CUDA(ctx, cudaLaunchKernelEx(&cfg, k_attn_tc<HD, TILES, CG, TYPE>, kmap, vmap, qmap, A));
+    LEV_CUDA(ctx, cudaLaunchKernelEx(&cfg, k_attn_tc<HD, TILES, CG, TYPE, COPY>, kmap, vmap, qmap, A));
     ctx->launches++;
     return lev_cuda_check(ctx, cudaGetLastError(), "k_attn_tc");
 }
@@ -1174,6 +1220,10 @@ int tc_run(lev_ctx* ctx, EncodeTiledFn enc, const CUtensorMap& kmap, const CUten
             return P.cg == 2 ? tc_launch<256, 1, 2, TYPE>(ctx, kmap, vmap, qmap, A, P.units) : tc_launch<256, 1, 1, TYPE>(ctx, kmap, vmap, qmap, A, P.units);
         return P.tiles == 2 ? tc_launch<128, 2, 1, TYPE>(ctx, kmap, vmap, qmap, A, P.units) : tc_launch<128, 1, 1, TYPE>(ctx, kmap, vmap, qmap, A, P.units);
     };
+    if (!A.box_k) {
+        if (hd == 256) return tc_launch<256, 1, 1, TC_F16, true>(ctx, kmap, vmap, qmap, A, P.units);
+        return P.tiles == 2 ? tc_launch<128, 2, 1, TC_F16, true>(ctx, kmap, vmap, qmap, A, P.units) : tc_launch<128, 1, 1, TC_F16, true>(ctx, kmap, vmap, qmap, A, P.units);
+    }
     return A.kv_type == TC_BF16 ? launch(std::integral_constant<int, TC_BF16>()) : launch(std::integral_constant<int, TC_F16>());
 }
 
@@ -1251,14 +1301,16 @@ extern "C" int lev_attn_chunk(lev_ctx* ctx, const lev_kv_layout* L, const void* 
     A.page = L->page;
     A.max_blocks = L->max_blocks;
     A.slots = L->slots;
-    // pages that make up whole steps of 128 positions out of whole swizzle atoms go by TMA, others are copied by warps
-    const bool boxes = A.kv_type == TC_F16 && LEV_KV_ROW(0, 0, 1, L->page, L->kv_heads) == 1 && L->page % 8 == 0 && (TC_KV % L->page == 0 || L->page % TC_KV == 0) && L->blocks < (1ll << 31);
+    // pages of whole groups of eight rows go by TMA (a box is what pages and steps of 128 positions have in common), others are copied by warps
+    const bool boxes = A.kv_type == TC_F16 && LEV_KV_ROW(0, 0, 1, L->page, L->kv_heads) == 1 && L->page % 8 == 0 && L->blocks < (1ll << 31);
     const int64_t cap = (int64_t)L->max_blocks * L->page, span = window > 0 && window < cap ? window : cap;
     const TcPlan P = tc_plan(ctx, n_rows, n_chunks, L->kv_heads, A.tpt, hd, span, boxes);
     A.splits = P.splits;
     CUtensorMap kmap = {}, vmap = {};
     if (boxes) {
-        const int box_v = L->page < TC_KV ? L->page : TC_KV, box_k = box_v > TC_KV / P.cg ? TC_KV / P.cg : box_v;
+        int box_v = TC_KV;
+        while (L->page % box_v) box_v /= 2;
+        const int box_k = box_v > TC_KV / P.cg ? TC_KV / P.cg : box_v;
         // an atom's 64 columns and eight rows, then slabs of 64 columns over all heads, groups of eight rows, blocks
         const int64_t row = LEV_KV_ROW(0, 1, 0, L->page, L->kv_heads) * hd * 2;
         const cuuint64_t dims[5] = {64, 8, (cuuint64_t)L->kv_heads * hd / 64, (cuuint64_t)L->page / 8, (cuuint64_t)L->blocks};

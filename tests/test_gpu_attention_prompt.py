@@ -115,10 +115,11 @@ def test_several_sequences(ctx, heads, q_type, out_type):
     run_chunk(ctx, [1, 0, 37, 130, 64, 1, 257], [500, 3, 0, 1000, 63, 0, 129], 16, heads, q_type=q_type, out_type=out_type, order=[3, 0, 6, 1, 2, 5, 4])
 
 
-@pytest.mark.parametrize("page", [1, 5, 8, 16, 24, 32, 64, 128, 256, 384])
+@pytest.mark.parametrize("page", [1, 3, 5, 8, 16, 24, 32, 40, 48, 64, 96, 100, 128, 160, 256, 384])
 @pytest.mark.parametrize("heads", [(16, 8, 256), (8, 2, 128)])
 def test_page_sizes(ctx, page, heads):
     run_chunk(ctx, [70, 3], [333, 150], page, heads, seed=page)
+    run_chunk(ctx, [1, 200, 1, 1, 5, 300], [1200, 30, 700, 1, 128, 0], page, heads, seed=page)
 
 
 @pytest.mark.parametrize("window", [1, 2, 100, 128, 129, 1000])
@@ -128,8 +129,10 @@ def test_windows(ctx, window, heads):
 
 
 @pytest.mark.parametrize("page", [16, 7])
-def test_f32_cache(ctx, page):
-    run_chunk(ctx, [150, 2], [200, 31], page, (8, 2, 128), kv_type=torch.float32)
+@pytest.mark.parametrize("heads", [(16, 8, 256), (8, 2, 128)])
+def test_f32_cache(ctx, page, heads):
+    run_chunk(ctx, [150, 2], [200, 31], page, heads, kv_type=torch.float32)
+    run_chunk(ctx, [300, 2, 500], [500, 900, 0], page, heads, kv_type=torch.float32, window=333)
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.07, 1.0])

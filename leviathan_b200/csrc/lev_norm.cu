@@ -9,6 +9,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "lev_stream.h"
 #include "lev_stream_math.cuh"
 
@@ -105,19 +107,22 @@ __global__ void __launch_bounds__(kNormThreads) k_rmsnorm(const float* x, int n,
 
 // The norm behind a block, its gate, the residual sum and scale and the norm before the next block in one pass:
 //   b = x * inv_rms(x) * post,  r = scale * (residual + alpha * gate * b),  h = r * inv_rms(r) * pre
-// One CTA per row; both statistics are reduced in the order of k_rmsnorm.  Rows of up to kMixRegs * 1024 elements on
-// 16-byte boundaries stay in registers between the steps, and everything that does not wait for a statistic is requested up
-// front, so x and residual are read once and out and h written once.  Longer or unaligned rows are read again (r from out,
-// which every thread wrote itself).  out may be residual or x: a thread touches only its own elements.
+// Rows of up to kMixMost elements stay in registers between the steps, so x and residual are read once, out and h written
+// once.  A few CTAs per SM walk the rows with the weights in registers (read again for every row they cost as much of L2 as the
+// rows themselves: 4096 x 2816 took 33 us) and the next row on its way while this one is reduced: 29.5 us = 5.5 TB/s, 0.83 of the
+// copy bandwidth; what is left are the two block reductions of a row.  Statistics are f32 sums in a fixed order.  Longer rows are read
+// again (r from out, which every thread wrote itself).  out may be residual or x: a thread touches only its own elements.
 struct MixArgs {
     const float *x, *residual, *post, *gate, *pre;
     int64_t gate_ld;
     float alpha, scale, eps;
     float* out;
     void* h;
-    int n, norm_post, h_type, vec;
+    int n, norm_post, h_type;
+    int64_t rows;
 };
-constexpr int kMixRegs = 4;
+constexpr int kMixMost = 16 * 512;   // elements of a row that registers hold
+template <int THREADS>
 __device__ __forceinline__ float mix_block_sum(float v, float* part) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -125,7 +130,7 @@ __device__ __forceinline__ float mix_block_sum(float v, float* part) {
     __syncthreads();
     float tot = 0.f;
 #pragma unroll
-    for (int k = 0; k < kNormThreads / 32; k++) tot += part[k];
+    for (int k = 0; k < THREADS / 32; k++) tot += part[k];
     return tot;
 }
 __device__ __forceinline__ void mix_store(const MixArgs& A, int64_t at, float v) {
@@ -133,72 +138,128 @@ __device__ __forceinline__ void mix_store(const MixArgs& A, int64_t at, float v)
     else if (A.h_type == LEV_ELEM_BF16) static_cast<__nv_bfloat16*>(A.h)[at] = __float2bfloat16_rn(v);
     else static_cast<__half*>(A.h)[at] = __float2half_rn(v);
 }
-__global__ void __launch_bounds__(kNormThreads) k_norm_residual(MixArgs A) {
+// VEC consecutive elements of row memory; on 16-byte boundaries four, else one (neighbouring threads then take neighbours)
+template <int VEC>
+__device__ __forceinline__ void mix_load(float* v, const float* p, bool in, float other) {
+    if (VEC == 4) {
+        const float4 a = in ? __ldcs(reinterpret_cast<const float4*>(p)) : make_float4(other, other, other, other);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+    } else {
+        v[0] = in ? __ldcs(p) : other;
+    }
+}
+// CTAs per SM that the registers allow without spilling: 4096 x 2816 29.5 us with two (three: 32.4), x 1024 12.5 with four (three: 13.7)
+constexpr int mix_ctas(int threads, int elems) { return threads == 512 ? 1 : threads == 128 ? 8 : elems <= 4 ? 4 : elems <= 8 ? 3 : 2; }
+// GATES: every row has a gate of its own
+template <int THREADS, int ELEMS, int VEC, bool GATES>
+__global__ void __launch_bounds__(THREADS, mix_ctas(THREADS, ELEMS)) k_norm_residual(MixArgs A) {
+    __shared__ float part[2][2][THREADS / 32];   // [parity of the row][statistic]
+    constexpr int PIECES = ELEMS / VEC;
+    const int n = A.n;
+    pdl_wait();
+    pdl_launch_dependents();
+    float x[ELEMS], r[ELEMS], g[ELEMS], w[ELEMS];
+    auto fetch = [&](int64_t row, float* xv, float* rv) {
+#pragma unroll
+        for (int k = 0; k < PIECES; k++) {
+            const int i = (threadIdx.x + k * THREADS) * VEC;
+            mix_load<VEC>(xv + k * VEC, A.x + row * n + i, i < n, 0.f);
+            mix_load<VEC>(rv + k * VEC, A.residual + row * n + i, i < n, 0.f);
+        }
+    };
+    fetch(blockIdx.x, x, r);
+#pragma unroll
+    for (int k = 0; k < PIECES; k++) {
+        const int i = (threadIdx.x + k * THREADS) * VEC;
+        mix_load<VEC>(g + k * VEC, A.post + i, i < n && A.norm_post && A.post, 1.f);
+        if (!GATES && A.gate) {
+            float v[VEC];
+            mix_load<VEC>(v, A.gate + i, i < n, 0.f);
+#pragma unroll
+            for (int q = 0; q < VEC; q++) g[k * VEC + q] *= v[q];
+        }
+        mix_load<VEC>(w + k * VEC, A.pre + i, i < n && A.h && A.pre, 1.f);
+    }
+    int odd = 0;
+    for (int64_t row = blockIdx.x; row < A.rows; row += gridDim.x, odd ^= 1) {
+        const int64_t base = row * n;
+        float nx[ELEMS], nr[ELEMS], gv[GATES ? ELEMS : 1];
+        if (GATES)
+#pragma unroll
+            for (int k = 0; k < PIECES; k++) {
+                const int i = (threadIdx.x + k * THREADS) * VEC;
+                mix_load<VEC>(gv + k * VEC, A.gate + row * A.gate_ld + i, i < n, 0.f);
+            }
+        if (row + gridDim.x < A.rows) fetch(row + gridDim.x, nx, nr);
+        float mul = A.alpha;
+        if (A.norm_post) {
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < ELEMS; e++) ss = fmaf(x[e], x[e], ss);
+            mul *= 1.0f / sqrtf(mix_block_sum<THREADS>(ss, part[odd][0]) / (float)n + A.eps);
+        }
+        float ss = 0.f;
+#pragma unroll
+        for (int k = 0; k < PIECES; k++) {
+            const int i = (threadIdx.x + k * THREADS) * VEC;
+#pragma unroll
+            for (int q = 0; q < VEC; q++) {
+                const int e = k * VEC + q;
+                r[e] = A.scale * fmaf(GATES ? mul * g[e] * gv[e] : mul * g[e], x[e], r[e]);
+                ss = fmaf(r[e], r[e], ss);
+            }
+            if (i < n) {
+                if (VEC == 4) *reinterpret_cast<float4*>(A.out + base + i) = make_float4(r[k * VEC], r[k * VEC + 1], r[k * VEC + 2], r[k * VEC + 3]);
+                else A.out[base + i] = r[k];
+            }
+        }
+        if (A.h) {
+            const float inv = 1.0f / sqrtf(mix_block_sum<THREADS>(ss, part[odd][1]) / (float)n + A.eps);
+#pragma unroll
+            for (int k = 0; k < PIECES; k++) {
+                const int i = (threadIdx.x + k * THREADS) * VEC;
+                if (i >= n) continue;
+                float h[4] = {};
+#pragma unroll
+                for (int q = 0; q < VEC; q++) h[q] = r[k * VEC + q] * inv * w[k * VEC + q];
+                if (VEC == 1) {
+                    mix_store(A, base + i, h[0]);
+                } else if (A.h_type == LEV_ELEM_F32) {
+                    *reinterpret_cast<float4*>(static_cast<float*>(A.h) + base + i) = make_float4(h[0], h[1], h[2], h[3]);
+                } else if (A.h_type == LEV_ELEM_BF16) {
+                    const __nv_bfloat162 a = __floats2bfloat162_rn(h[0], h[1]), b = __floats2bfloat162_rn(h[2], h[3]);
+                    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(A.h) + base + i) =
+                        make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
+                } else {
+                    const __half2 a = __floats2half2_rn(h[0], h[1]), b = __floats2half2_rn(h[2], h[3]);
+                    *reinterpret_cast<uint2*>(static_cast<__half*>(A.h) + base + i) =
+                        make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < ELEMS; e++) {
+            x[e] = nx[e];
+            r[e] = nr[e];
+        }
+    }
+}
+// rows that are too long for registers: one CTA per row, read again between the steps
+__global__ void __launch_bounds__(kNormThreads) k_norm_residual_any(MixArgs A) {
     __shared__ float part[2][kNormThreads / 32];
     const int n = A.n;
     pdl_wait();
     pdl_launch_dependents();
     const int64_t row = blockIdx.x, base = row * n;
     const float *x = A.x + base, *res = A.residual + base, *gate = A.gate ? A.gate + row * A.gate_ld : nullptr;
-    if (A.vec) {
-        float4 xv[kMixRegs], rv[kMixRegs], gv[kMixRegs], pv[kMixRegs];
-        const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int k = 0; k < kMixRegs; k++) {
-            const int i = (threadIdx.x + k * kNormThreads) * 4;
-            const bool in = i < n;
-            xv[k] = in ? *reinterpret_cast<const float4*>(x + i) : none;
-            rv[k] = in ? *reinterpret_cast<const float4*>(res + i) : none;
-            gv[k] = in && gate ? *reinterpret_cast<const float4*>(gate + i) : make_float4(1.f, 1.f, 1.f, 1.f);
-            if (in && A.norm_post && A.post) {
-                const float4 w = __ldg(reinterpret_cast<const float4*>(A.post + i));
-                gv[k] = make_float4(gv[k].x * w.x, gv[k].y * w.y, gv[k].z * w.z, gv[k].w * w.w);
-            }
-            pv[k] = in && A.h && A.pre ? __ldg(reinterpret_cast<const float4*>(A.pre + i)) : make_float4(1.f, 1.f, 1.f, 1.f);
-        }
-        float mul = A.alpha;
-        if (A.norm_post) {
-            float ss = 0.f;
-#pragma unroll
-            for (int k = 0; k < kMixRegs; k++) ss = fmaf(xv[k].w, xv[k].w, fmaf(xv[k].z, xv[k].z, fmaf(xv[k].y, xv[k].y, fmaf(xv[k].x, xv[k].x, ss))));
-            mul *= 1.0f / sqrtf(mix_block_sum(ss, part[0]) / (float)n + A.eps);
-        }
-        float ss = 0.f;
-#pragma unroll
-        for (int k = 0; k < kMixRegs; k++) {
-            const int i = (threadIdx.x + k * kNormThreads) * 4;
-            float4 r = make_float4(A.scale * fmaf(mul * gv[k].x, xv[k].x, rv[k].x), A.scale * fmaf(mul * gv[k].y, xv[k].y, rv[k].y),
-                                   A.scale * fmaf(mul * gv[k].z, xv[k].z, rv[k].z), A.scale * fmaf(mul * gv[k].w, xv[k].w, rv[k].w));
-            rv[k] = r;
-            if (i < n) *reinterpret_cast<float4*>(A.out + base + i) = r;
-            ss = fmaf(r.w, r.w, fmaf(r.z, r.z, fmaf(r.y, r.y, fmaf(r.x, r.x, ss))));
-        }
-        if (!A.h) return;
-        const float inv = 1.0f / sqrtf(mix_block_sum(ss, part[1]) / (float)n + A.eps);
-#pragma unroll
-        for (int k = 0; k < kMixRegs; k++) {
-            const int i = (threadIdx.x + k * kNormThreads) * 4;
-            if (i >= n) continue;
-            const float4 h = make_float4(rv[k].x * inv * pv[k].x, rv[k].y * inv * pv[k].y, rv[k].z * inv * pv[k].z, rv[k].w * inv * pv[k].w);
-            if (A.h_type == LEV_ELEM_F32) {
-                *reinterpret_cast<float4*>(static_cast<float*>(A.h) + base + i) = h;
-            } else if (A.h_type == LEV_ELEM_BF16) {
-                const __nv_bfloat162 a = __floats2bfloat162_rn(h.x, h.y), b = __floats2bfloat162_rn(h.z, h.w);
-                *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(A.h) + base + i) = make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
-            } else {
-                const __half2 a = __floats2half2_rn(h.x, h.y), b = __floats2half2_rn(h.z, h.w);
-                *reinterpret_cast<uint2*>(static_cast<__half*>(A.h) + base + i) = make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
-            }
-        }
-        return;
-    }
     float mul = A.alpha;
     if (A.norm_post) {
         float ss = 0.f;
         for (int i = threadIdx.x; i < n; i += kNormThreads) ss = fmaf(x[i], x[i], ss);
-        mul *= 1.0f / sqrtf(mix_block_sum(ss, part[0]) / (float)n + A.eps);
+        mul *= 1.0f / sqrtf(mix_block_sum<kNormThreads>(ss, part[0]) / (float)n + A.eps);
     }
     float ss = 0.f;
+#pragma unroll 4
     for (int i = threadIdx.x; i < n; i += kNormThreads) {
         float g = mul * (gate ? gate[i] : 1.f);
         if (A.norm_post && A.post) g *= A.post[i];
@@ -207,7 +268,8 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_residual(MixArgs A) {
         ss = fmaf(r, r, ss);
     }
     if (!A.h) return;
-    const float inv = 1.0f / sqrtf(mix_block_sum(ss, part[1]) / (float)n + A.eps);
+    const float inv = 1.0f / sqrtf(mix_block_sum<kNormThreads>(ss, part[1]) / (float)n + A.eps);
+#pragma unroll 4
     for (int i = threadIdx.x; i < n; i += kNormThreads) mix_store(A, base + i, A.out[base + i] * inv * (A.pre ? A.pre[i] : 1.f));
 }
 
@@ -309,10 +371,31 @@ extern "C" int lev_norm_residual(lev_ctx* ctx, const float* x, const float* resi
                                                                   (gate && overlap(h, h_bytes, gate, gate_bytes)))))
         return lev_fail(ctx, LEV_BAD_ARGUMENT, "an output overlaps another argument");
     LEV_CUDA(ctx, cudaSetDevice(ctx->device));
-    MixArgs A = {x, residual, post, gate, pre, gate_ld, alpha, scale, eps, out, h, (int)n, norm_post != 0, h_type, 0};
+    MixArgs A = {x, residual, post, gate, pre, gate_ld, alpha, scale, eps, out, h, (int)n, norm_post != 0, h_type, rows};
     const uintptr_t all = (uintptr_t)x | (uintptr_t)residual | (uintptr_t)out | (uintptr_t)post | (uintptr_t)gate | (uintptr_t)pre | (uintptr_t)h;
-    A.vec = n % 4 == 0 && n <= kMixRegs * 4 * kNormThreads && (all & 15) == 0 && gate_ld % 4 == 0;
-    LEV_CUDA(ctx, launch_pdl(k_norm_residual, dim3((unsigned)rows), dim3(kNormThreads), 0, ctx->stream, A));
+    if (n > kMixMost) {
+        LEV_CUDA(ctx, launch_pdl(k_norm_residual_any, dim3((unsigned)rows), dim3(kNormThreads), 0, ctx->stream, A));
+    } else {
+        const bool gates = gate && gate_ld != 0, quads = n % 4 == 0 && (all & 15) == 0 && (!gates || gate_ld % 4 == 0);
+        auto run = [&](auto threads_tag, auto elems_tag) {
+            constexpr int THREADS = decltype(threads_tag)::value, ELEMS = decltype(elems_tag)::value;
+            const int64_t most = mix_ctas(THREADS, ELEMS) * (int64_t)ctx->prop.multiProcessorCount, waves = (rows + most - 1) / most;
+            const dim3 grid((unsigned)((rows + waves - 1) / waves));   // rows spread evenly
+            if (quads)
+                return gates ? launch_pdl(k_norm_residual<THREADS, ELEMS, 4, true>, grid, dim3(THREADS), 0, ctx->stream, A)
+                             : launch_pdl(k_norm_residual<THREADS, ELEMS, 4, false>, grid, dim3(THREADS), 0, ctx->stream, A);
+            return gates ? launch_pdl(k_norm_residual<THREADS, ELEMS, 1, true>, grid, dim3(THREADS), 0, ctx->stream, A)
+                         : launch_pdl(k_norm_residual<THREADS, ELEMS, 1, false>, grid, dim3(THREADS), 0, ctx->stream, A);
+        };
+        typedef std::integral_constant<int, 128> narrow;
+        typedef std::integral_constant<int, 256> usual;
+        typedef std::integral_constant<int, 512> wide;
+        LEV_CUDA(ctx, n <= 4 * 128    ? run(narrow(), std::integral_constant<int, 4>())
+                      : n <= 4 * 256  ? run(usual(), std::integral_constant<int, 4>())
+                      : n <= 8 * 256  ? run(usual(), std::integral_constant<int, 8>())
+                      : n <= 16 * 256 ? run(usual(), std::integral_constant<int, 16>())
+                                      : run(wide(), std::integral_constant<int, 16>()));
+    }
     ctx->launches++;
     return LEV_OK;
 }

@@ -11,10 +11,10 @@
 // batch's maximum in shared memory (with keys pushed under a running threshold in every round, 512 rows of 262144 took a
 // third longer).  The `top` largest values lie in the `top` batches with the largest best values: were a value's batch not
 // among them, `top` other batches would each hold a larger one.  So, behind the pass: a threshold that at least `top` values reach
-// (the least of the maxima of as many groups of threads); the batches that reach it, some hundred, are read again for the index of
-// their best value, go to a buffer as 64-bit keys (value in order, then index) and are sorted; then the values of the best `top`
-// batches that reach the last of these keys are.  Where the buffer would overflow (long ties) it is sorted in between and the threshold
-// rises.  The result is that of a full sort: keys are distinct, so the order in which threads append does not matter.
+// (the top-th largest of 128 groups' maxima); the batches that reach it, a few more than `top`, are sorted by their maxima; then the
+// values of those that reach the top-th maximum are read again and sorted as 64-bit keys (value in order, then index).  Where too many
+// batches tie with the top-th, their best values' indices decide, and where the buffer would overflow it is sorted in between and the
+// threshold rises.  The result is that of a full sort: keys are distinct, so the order in which threads append does not matter.
 //
 // A row belongs to a cluster of up to eight thread blocks, whose partial results the first one joins through distributed
 // shared memory: no work buffer, no second launch.
@@ -37,7 +37,7 @@ struct LpArgs {
     int64_t n, ld;
     const int32_t* tokens;
     float cap_k, cap2;      // 2 log2(e) / cap, cap log2(e)
-    int top, group, keep;   // group: lanes whose maximum counts as one in the first threshold; keep: keys that the buffer may hold after a round
+    int top, keep;          // keep: keys that the buffer may hold after a round
     float *logprob, *entropy, *top_logprob;
     int32_t* top_index;
     int* status;
@@ -164,7 +164,8 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) k_logprobs(LpArgs A, in
     extern __shared__ float batch_max[];   // [round][thread]
     __shared__ LpStats warp_stats[NT / 32], block_stats;
     __shared__ unsigned long long thr_key;
-    __shared__ float thr_value, group_low[NT / 32], lse_s[2];
+    __shared__ float thr_value, lse_s[2];
+    __shared__ __align__(16) float group_max[128];
     __shared__ int count;
     __shared__ unsigned batch_s[kLpKeys / kLpRound];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) k_logprobs(LpArgs A, in
     auto append = [&](unsigned long long k) {
         const int at = atomicAdd(&count, 1);
         over |= at >= A.keep;
-        if (at < kLpKeys) cand[at] = k;   // always: the buffer is looked after in time
+        if (at < kLpKeys) cand[at] = k;
     };
     auto push = [&](unsigned long long k) {
         if (k > thr_key) append(k);
@@ -295,19 +296,24 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) k_logprobs(LpArgs A, in
     }
     if (lane == 0) warp_stats[warp] = s;
     if (A.top) {
-        // a threshold that at least `top` values reach: each group of threads has one that reaches the least of their maxima
+        // a threshold that at least `top` values reach: the top-th largest of the maxima of 128 groups of threads
         float g = raw_max;
-        for (int o = 1; o < A.group; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) g = fminf(g, __shfl_xor_sync(0xffffffffu, g, o));
-        if (lane == 0) group_low[warp] = g;
+        for (int o = 1; o < NT / 128; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+        if (t % (NT / 128) == 0) group_max[t / (NT / 128)] = g;
         __syncthreads();
-        if (t == 0) {
-            float low = group_low[0];
-            for (int w = 1; w < NT / 32; w++) low = fminf(low, group_low[w]);
-            if (low > -INFINITY) {
-                thr_value = low;
-                thr_key = ((unsigned long long)lp_order(low) << 32) - 1;
+        if (t < 128) {
+            const float mine = group_max[t];
+            int larger = 0;
+#pragma unroll 8
+            for (int i = 0; i < 128; i += 4) {
+                const float4 o = *reinterpret_cast<const float4*>(group_max + i);
+                larger += (o.x > mine || (o.x == mine && i < t)) + (o.y > mine || (o.y == mine && i + 1 < t)) + (o.z > mine || (o.z == mine && i + 2 < t)) +
+                          (o.w > mine || (o.w == mine && i + 3 < t));
+            }
+            if (larger == A.top - 1 && mine > -INFINITY) {
+                thr_value = mine;
+                thr_key = ((unsigned long long)lp_order(mine) << 32) - 1;
             }
         }
         __syncthreads();
@@ -340,11 +346,23 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) k_logprobs(LpArgs A, in
             known = count;
             over = 0;
         };
-        for (int r = 0; r < round; r++) {
-            if (ub + r * per_round + t < ue && !(batch_max[r * NT + t] < thr_value))
-                append((unsigned long long)lp_order(batch_max[r * NT + t]) << 32 | (unsigned)(r * NT + t));
-            if (r % kEvery == kEvery - 1)
-                if (__syncthreads_or(over)) look();
+        auto enter = [&](int r) {
+            const float mx = batch_max[r * NT + t];
+            if (ub + r * per_round + t < ue && !(mx < thr_value)) append((unsigned long long)lp_order(mx) << 32 | (unsigned)(r * NT + t));
+        };
+#pragma unroll 4
+        for (int r = 0; r < round; r++) enter(r);
+        __syncthreads();
+        if (count > kLpKeys) {   // ties without end: again, with the buffer sorted whenever it has filled up
+            __syncthreads();
+            if (t == 0) count = 0;
+            over = 0;
+            __syncthreads();
+            for (int r = 0; r < round; r++) {
+                enter(r);
+                if (r % kEvery == kEvery - 1)
+                    if (__syncthreads_or(over)) look();
+            }
         }
         // Nearly always the maxima alone decide: all batches that reach the top-th maximum, if they are few enough.  Otherwise
         // (ties without end, or nothing above -inf) their best values' indices do.
@@ -492,13 +510,10 @@ int lp_launch(lev_ctx* ctx, const LpArgs& A, int64_t rows, int splits) {
 
 template <typename T>
 int lp_run(lev_ctx* ctx, const LpArgs& A, int64_t rows, int splits) {
-    LpArgs B = A;
-    if (rows * splits < ctx->prop.multiProcessorCount) {   // few blocks: wide ones, so that a row's loads are in flight together
-        B.group = A.top <= 32 ? 32 : 16;                   // 32 or 64 groups
-        return A.cap2 > 0.f ? lp_launch<T, 1024, true>(ctx, B, rows, splits) : lp_launch<T, 1024, false>(ctx, B, rows, splits);
-    }
-    B.group = A.top <= 8 ? 32 : A.top <= 32 ? 8 : 4;       // 8, 32 or 64 groups
-    return A.cap2 > 0.f ? lp_launch<T, 256, true>(ctx, B, rows, splits) : lp_launch<T, 256, false>(ctx, B, rows, splits);
+    // few blocks: wide ones, so that a row's loads are in flight together
+    if (rows * splits < ctx->prop.multiProcessorCount)
+        return A.cap2 > 0.f ? lp_launch<T, 1024, true>(ctx, A, rows, splits) : lp_launch<T, 1024, false>(ctx, A, rows, splits);
+    return A.cap2 > 0.f ? lp_launch<T, 256, true>(ctx, A, rows, splits) : lp_launch<T, 256, false>(ctx, A, rows, splits);
 }
 
 }  // namespace

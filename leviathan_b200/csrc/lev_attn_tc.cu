@@ -377,7 +377,7 @@ __device__ __forceinline__ void tc_load_q(const TcArgs& A, const TcUnit& U, unsi
             }
         };
 #pragma unroll 1
-        for (int r0 = first; r0 < 128; r0 += BATCH * step) {
+        for (int r0 = first; r0 < 128; r0 += BATCH * step) {   // (rows of no token are zeros: with what lay there their references would run away)
             if (A.q_type == TC_F32) {
                 float4 a[BATCH], b[BATCH];
 #pragma unroll
@@ -505,7 +505,6 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         }
     }
     pdl_wait();
-    pdl_launch_dependents();
     TcUnit U;   // the first unit: the same answer in every warp and every CTA of the cluster
     bool have = tc_unit(A, (int)blockIdx.x / cluster, per, split, lane, &U);
     if (!have) U.tokens = 0;
@@ -1065,6 +1064,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
             st.step(1);
         }
     }
+    pdl_launch_dependents();   // what follows finds no room on an SM before (40 packed prompts: 73 us with the launch at the start, 71 here)
     pk_finish(abort_flag, A.status, LEV_DEV_TIMEOUT);
     if (A.splits > 1) {
         const int tokens = U0.tokens;

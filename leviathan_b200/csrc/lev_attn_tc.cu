@@ -36,6 +36,7 @@
 namespace {
 
 constexpr int TC_KV = 128;                 // positions per step
+constexpr int TC_MAX_SPLITS = 8;   // CTAs of a cluster that share a unit's positions
 constexpr unsigned TC_STAGE = 32768;       // 128 rows x 128 columns of 16 bits: two slabs of 64 columns
 constexpr int TC_MAX_STAGES = 6;
 constexpr int TC_LOAD_WARPS = 3;           // copying warps where TMA boxes do not apply
@@ -433,6 +434,15 @@ __device__ __forceinline__ int tc_next_taken(unsigned answer) {
     return ok ? x : -1;
 }
 
+// four lanes hand their rows' four 16-byte pieces round, so that a store writes 64 bytes of a row: v[q] is then piece (lane & 3) of the
+// row of the quad's lane q
+__device__ __forceinline__ void quad_turn(uint4* v, int lane) {
+    swap_pieces(v[0], v[1], 1, lane);
+    swap_pieces(v[2], v[3], 1, lane);
+    swap_pieces(v[0], v[2], 2, lane);
+    swap_pieces(v[1], v[3], 2, lane);
+}
+
 template <int HD, int TILES>
 struct TcDims {
     static constexpr int kWarps = 4 * TILES + 4;
@@ -448,7 +458,7 @@ struct TcDims {
 // warps (kernels of their own: with both ways in one, 32 heads of 128 lost 5 % to the registers of the one not taken).  TILES: 128-row tiles of a CTA, each with a softmax warpgroup; one tile has two S buffers, two
 // tiles have one each.  CG = 2: a pair of CTAs (cta_group::2) with one tile each that share K and V.  splits > 1: the
 // CTAs of a cluster take parts of the positions and merge through distributed shared memory.
-template <int HD, int TILES, int CG, int TYPE, bool COPY>
+template <int HD, int TILES, int CG, int TYPE, bool COPY, bool SPLIT>
 __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
     k_attn_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap,
               const __grid_constant__ TcArgs A) {
@@ -467,7 +477,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
     __shared__ float again_w[TILES][128];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // a cluster is a unit: the pair (one CTA without pairs) of split 0, then that of split 1, ...
-    const int cluster = CG * A.splits;
+    const int cluster = SPLIT ? CG * A.splits : CG;
     const unsigned in_cluster = (int)blockIdx.x % cluster;
     const unsigned rank = in_cluster % CG, lead = in_cluster - rank;
     const int split = (int)in_cluster / CG, per = A.tpt * TILES * CG;
@@ -518,7 +528,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
     volatile int* abort_flag = &abort_s;
     // Unit k (from 0) of this CTA is in unit_s[k & 1].  Ends unit k and goes on to the next one; false: there is none.
     auto next_unit = [&](int k) {
-        if (A.splits > 1) return false;   // a cluster that merges has one unit
+        if (SPLIT) return false;   // a cluster that merges has one unit
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&unit_empty[k & 1]));
         k++;
@@ -527,11 +537,16 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         U = unit_s[k & 1];
         return U.tokens > 0 && !*abort_flag;
     };
-    // splits: partial sums [tile][row][HD] where the queries and stages were, behind them 8 KB for one row's work or the
-    // merge's weights, then a row's reference and sum
+    // Splits: the CTA of split z adds up rows z * share ... of a tile.  Every CTA stores its partial sums of a row, reference and sum of
+    // weights straight into that CTA's shared memory, [tile][part][row of the share][HD] where the queries and stages were, when all
+    // CTAs of the cluster are done with theirs; stores need no answer, loads from the other CTAs (7.5 us for a tile of 256 columns)
+    // waited for theirs.
     unsigned char* const base = smem_dyn + (smem - smem_u32(smem_dyn));
-    constexpr unsigned kMergeAt = TILES * 128 * HD * 4, kStatsAt = kMergeAt + 8192;
-    float(*merge_ml)[2] = reinterpret_cast<float(*)[2]>(base + kStatsAt);
+    constexpr unsigned kPartRows = 128 + TC_MAX_SPLITS, kStatsAt = TILES * kPartRows * HD * 4, kWeightsAt = kStatsAt + TILES * kPartRows * 8;
+    auto rows_of_tile = [&](int tokens, int tile) {   // that have a token
+        const int left = tokens - (int)(rank * TILES + tile) * A.tpt;
+        return left <= 0 ? 0 : (left < A.tpt ? left : A.tpt) * A.group;
+    };
 
     if (warp < 4 * TILES) {
         // ---- softmax: thread = row of the tile ----
@@ -643,7 +658,6 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         if (n > 0) {
             const int last = TILES == 2 ? tile : (g - 1) & 1, lpar = TILES == 2 ? (g - 1) & 1 : ((g - 1) >> 1) & 1;
             pk_wait(smem_u32(&pv_done[last]), lpar, abort_flag);
-            if (TILES == 2 && A.splits > 1) pk_wait(smem_u32(&pv_done[tile ^ 1]), lpar, abort_flag);   // the partial sums go where K and V were
             __syncwarp();
             tc_after();
         }
@@ -660,7 +674,20 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         int64_t quad_out[4];   // where the four rows of this lane's quad go; negative: nowhere
 #pragma unroll
         for (int q = 0; q < 4; q++) quad_out[q] = __shfl_sync(0xffffffffu, live ? out_at : -1, (lane & 28) + q);
-        float* part_o = reinterpret_cast<float*>(base) + tile * 128 * HD;   // splits: [row][HD], 16-byte pieces swizzled
+        unsigned quad_part[4], stats_at = 0;   // splits: where the quad's partial sums (16-byte pieces swizzled) and this row's statistics go
+        const int share = SPLIT ? (rows_of_tile(V.tokens, tile) + A.splits - 1) / A.splits : 1;
+        auto part_row = [&](int r, unsigned* stats) {
+            const int owner = r / share, at = split * share + r - owner * share;
+            *stats = map_to_rank(smem + kStatsAt + (unsigned)(tile * kPartRows + at) * 8u, owner * CG + rank);
+            return map_to_rank(smem + (unsigned)(tile * kPartRows + at) * (HD * 4u), owner * CG + rank);
+        };
+        if constexpr (SPLIT) {
+            const unsigned part_at = live ? part_row(t, &stats_at) : 0u;
+#pragma unroll
+            for (int q = 0; q < 4; q++) quad_part[q] = __shfl_sync(0xffffffffu, part_at, (lane & 28) + q);
+            __syncwarp();
+            cluster_sync_all();   // every CTA's products are done
+        }
         if (n > 0) {
             auto rows_out = [&](auto type_tag) {
                 constexpr int OUT = decltype(type_tag)::value;
@@ -673,8 +700,18 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                     for (int q = 0; q < 32; q++) probe = fmaf(__uint_as_float(o[q]), 0.f, probe);
                     if constexpr (OUT == TC_F32) {   // partial sums for the merge
 #pragma unroll
-                        for (int q = 0; q < 32; q += 4)
-                            *reinterpret_cast<uint4*>(part_o + t * HD + (((c + q) >> 2 ^ (t & 7)) << 2)) = make_uint4(o[q], o[q + 1], o[q + 2], o[q + 3]);
+                        for (int half = 0; half < 32; half += 16) {
+                            uint4 v[4];
+#pragma unroll
+                            for (int q = 0; q < 4; q++) v[q] = make_uint4(o[half + 4 * q], o[half + 4 * q + 1], o[half + 4 * q + 2], o[half + 4 * q + 3]);
+                            quad_turn(v, lane);
+#pragma unroll
+                            for (int q = 0; q < 4; q++) {
+                                const unsigned to = quad_part[q] + ((unsigned)((c + half) / 4 + (lane & 3)) ^ ((lane & 4u) + q)) * 16u;
+                                if (quad_out[q] >= 0)
+                                    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(to), "r"(v[q].x), "r"(v[q].y), "r"(v[q].z), "r"(v[q].w) : "memory");
+                            }
+                        }
                     } else {
                     uint4 v[4];
 #pragma unroll
@@ -683,22 +720,18 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                                           pack16(__uint_as_float(o[8 * q + 2]) * inv, __uint_as_float(o[8 * q + 3]) * inv, OUT),
                                           pack16(__uint_as_float(o[8 * q + 4]) * inv, __uint_as_float(o[8 * q + 5]) * inv, OUT),
                                           pack16(__uint_as_float(o[8 * q + 6]) * inv, __uint_as_float(o[8 * q + 7]) * inv, OUT));
-                    // four lanes hand their rows' 16-byte pieces round, so that a store writes 64 bytes of a row
-                    swap_pieces(v[0], v[1], 1, lane);
-                    swap_pieces(v[2], v[3], 1, lane);
-                    swap_pieces(v[0], v[2], 2, lane);
-                    swap_pieces(v[1], v[3], 2, lane);
+                    quad_turn(v, lane);
 #pragma unroll
                     for (int q = 0; q < 4; q++)
                         if (quad_out[q] >= 0) *reinterpret_cast<uint4*>(static_cast<unsigned short*>(A.out) + quad_out[q] + c + (lane & 3) * 8) = v[q];
                     }
                 }
             };
-            if (A.splits > 1) rows_out(std::integral_constant<int, TC_F32>());
+            if constexpr (SPLIT) rows_out(std::integral_constant<int, TC_F32>());
             else if (A.out_type == TC_BF16) rows_out(std::integral_constant<int, TC_BF16>());
             else rows_out(std::integral_constant<int, TC_F16>());
         }
-        if (!ok && live && A.splits == 1) {
+        if (!ok && live && !SPLIT) {
             const unsigned nan = A.out_type == TC_BF16 ? 0x7FC07FC0u : 0x7E007E00u;
             uint4* dst = reinterpret_cast<uint4*>(static_cast<unsigned short*>(A.out) + out_at);
             for (int q = 0; q < HD / 8; q++) dst[q] = make_uint4(nan, nan, nan, nan);
@@ -726,8 +759,11 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
 #pragma unroll
                 for (int q = 0; q < HD / 128; q++) {
                     const int d = t + 128 * q;
-                    if (A.splits > 1) part_o[r * HD + ((((d >> 2) ^ (r & 7)) << 2) | (d & 3))] = o[q];
-                    else tc_store16(A, row * A.out_ld + rh * HD + d, o[q] / l2);
+                    if (SPLIT) {
+                        unsigned stats;
+                        const unsigned to = part_row(r, &stats) + ((unsigned)(d >> 2) ^ (r & 7u)) * 16u + (d & 3) * 4u;
+                        asm volatile("st.shared::cluster.f32 [%0], %1;\n" ::"r"(to), "f"(o[q]) : "memory");
+                    } else tc_store16(A, row * A.out_ld + rh * HD + d, o[q] / l2);
                 }
                 if (t == r) {
                     m = m2;
@@ -735,9 +771,10 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 }
             }
         }
-        if (A.splits > 1) {
-            merge_ml[tile * 128 + t][0] = bad ? 0.f : m;
-            merge_ml[tile * 128 + t][1] = bad ? NAN : l;
+        if (SPLIT) {
+            if (live)
+                asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};\n" ::"r"(stats_at), "f"(bad ? 0.f : m), "f"(bad ? NAN : l) : "memory");
+            break;   // (the cluster's only unit)
         }
         wg_sync(1 + tile);   // again_s is free for the next unit
         }
@@ -846,7 +883,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         const unsigned elected = elect_lane();
         const unsigned full_c = CG == 2 ? map_to_rank(smem_u32(&full[0]), lead) : smem_u32(&full[0]);
         Ring st(NS);
-        const bool more = A.splits == 1;   // a cluster that merges has one unit
+        const bool more = !SPLIT;   // a cluster that merges has one unit
         int units = 0, under_way = 0;   // under_way: stages whose copies have not been handed over, from `landed` on
         Ring landed(NS);
         if (more && have && w == 0 && rank == 0 && lane == 0) tc_next_request(smem_u32(answer_s), smem_u32(&answer_bar));
@@ -1064,84 +1101,56 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
             st.step(1);
         }
     }
+    if (SPLIT && (warp >= 4 * TILES || !U0.tokens)) {
+        __syncwarp();
+        cluster_sync_all();   // the softmax warps' one
+    }
     pdl_launch_dependents();   // what follows finds no room on an SM before (40 packed prompts: 73 us with the launch at the start, 71 here)
     pk_finish(abort_flag, A.status, LEV_DEV_TIMEOUT);
-    if (A.splits > 1) {
-        const int tokens = U0.tokens;
-        // ---- merge: the CTA of split z adds its share of the rows over all splits, in their order ----
-        cluster_sync_all();
+    if constexpr (SPLIT) {
+        // ---- the rows of this CTA's share: the parts in their order ----
+        cluster_sync_all();   // all parts have arrived
         const int Z = A.splits;
-        float* wts = reinterpret_cast<float*>(base + kMergeAt);   // [row][Z]: a part's share of a row
+        float* wts = reinterpret_cast<float*>(base + kWeightsAt);   // [row of the share][Z]: a part's share of a row
 #pragma unroll 1
         for (int tile = 0; tile < TILES; tile++) {
-            const int tile_tok = (int)(rank * TILES + tile) * A.tpt;
-            const int used = tokens > tile_tok ? (tokens - tile_tok < A.tpt ? tokens - tile_tok : A.tpt) * A.group : 0;   // rows
-            const int ra = used * split / Z, rb = used * (split + 1) / Z;
+            const int used = rows_of_tile(U0.tokens, tile), share = (used + Z - 1) / Z, first = split * share;
+            const int rows = used - first < share ? used - first : share;   // may be negative
+            const float2* stats = reinterpret_cast<const float2*>(base + kStatsAt) + tile * kPartRows;
             __syncthreads();   // the weights of the tile before are read
-            for (int r = ra + (int)threadIdx.x; r < rb; r += blockDim.x) {
-                float m[16], l[16], mm = -INFINITY, ll = 0.f;
-#pragma unroll
-                for (int z = 0; z < 16; z++) {
-                    m[z] = -INFINITY, l[z] = 0.f;
-                    if (z < Z)
-                        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];\n"
-                                     : "=f"(m[z]), "=f"(l[z])
-                                     : "r"(map_to_rank(smem + kStatsAt + 8u * (unsigned)(tile * 128 + r), z * CG + rank))
-                                     : "memory");
-                }
-#pragma unroll
-                for (int z = 0; z < 16; z++) mm = fmaxf(mm, m[z]);
-#pragma unroll
-                for (int z = 0; z < 16; z++) {
-                    m[z] = m[z] == -INFINITY && l[z] == 0.f ? 0.f : ex2((m[z] - mm) * A.sl);   // 0: the part attends to nothing
-                    ll = fmaf(l[z], m[z], ll);
+            for (int r = threadIdx.x; r < rows; r += blockDim.x) {
+                float mm = -INFINITY, ll = 0.f;
+                for (int z = 0; z < Z; z++) mm = fmaxf(mm, stats[z * share + r].x);
+                for (int z = 0; z < Z; z++) {
+                    const float2 v = stats[z * share + r];
+                    const float w = v.x == -INFINITY && v.y == 0.f ? 0.f : ex2((v.x - mm) * A.sl);   // 0: the part attends to nothing
+                    wts[r * Z + z] = w;
+                    ll = fmaf(v.y, w, ll);
                 }
                 const float inv = 1.f / ll;
-#pragma unroll
-                for (int z = 0; z < 16; z++)
-                    if (z < Z) wts[r * Z + z] = m[z] * inv;
+                for (int z = 0; z < Z; z++) wts[r * Z + z] *= inv;
             }
             __syncthreads();
-            constexpr int kQuads = HD / 4, kItems = 4;
-            const int first = ra * kQuads + (int)threadIdx.x, end = rb * kQuads;
-            for (int i0 = first; i0 < end; i0 += kItems * (int)blockDim.x) {
-                float4 a[kItems];
-#pragma unroll
-                for (int k = 0; k < kItems; k++) a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
+            constexpr int kQuads = HD / 4;
+            for (int item = threadIdx.x; item < rows * kQuads; item += blockDim.x) {
+                const int r = item / kQuads, qd = item - r * kQuads, row = first + r, tok = row / A.group;
+                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
                 for (int z = 0; z < Z; z++) {
-                    const unsigned part = map_to_rank(smem + (unsigned)(tile * 128 * HD) * 4u, z * CG + rank);
-                    float4 o[kItems];
-                    float w[kItems];
-#pragma unroll
-                    for (int k = 0; k < kItems; k++) {
-                        const int item = i0 + k * (int)blockDim.x, r = item / kQuads, qd = item - r * kQuads;
-                        w[k] = item < end ? wts[r * Z + z] : 0.f;
-                        o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (w[k] != 0.f)
-                            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n"
-                                         : "=f"(o[k].x), "=f"(o[k].y), "=f"(o[k].z), "=f"(o[k].w)
-                                         : "r"(part + (unsigned)(r * HD + ((qd ^ (r & 7)) << 2)) * 4u));
-                    }
-#pragma unroll
-                    for (int k = 0; k < kItems; k++) {
-                        a[k].x = fmaf(o[k].x, w[k], a[k].x);
-                        a[k].y = fmaf(o[k].y, w[k], a[k].y);
-                        a[k].z = fmaf(o[k].z, w[k], a[k].z);
-                        a[k].w = fmaf(o[k].w, w[k], a[k].w);
+                    const float w = wts[r * Z + z];
+                    const float4 o = reinterpret_cast<const float4*>(base)[(tile * kPartRows + z * share + r) * kQuads + (qd ^ (row & 7))];
+                    if (w != 0.f) {   // (a part that attends to nothing has stored nothing)
+                        a.x = fmaf(o.x, w, a.x);
+                        a.y = fmaf(o.y, w, a.y);
+                        a.z = fmaf(o.z, w, a.z);
+                        a.w = fmaf(o.w, w, a.w);
                     }
                 }
-#pragma unroll
-                for (int k = 0; k < kItems; k++) {
-                    const int item = i0 + k * (int)blockDim.x, r = item / kQuads, qd = item - r * kQuads, tok = r / A.group;
-                    if (item >= end) continue;
-                    unsigned short* dst = static_cast<unsigned short*>(A.out) + (int64_t)(U0.row0 + U0.t0 + tile_tok + tok) * A.out_ld +
-                                          (int64_t)(U0.kvh * A.group + r - tok * A.group) * HD + 4 * qd;
-                    *reinterpret_cast<uint2*>(dst) = make_uint2(pack16(a[k].x, a[k].y, A.out_type), pack16(a[k].z, a[k].w, A.out_type));
-                }
+                unsigned short* dst = static_cast<unsigned short*>(A.out) + (int64_t)(U0.row0 + U0.t0 + (int)(rank * TILES + tile) * A.tpt + tok) * A.out_ld +
+                                      (int64_t)(U0.kvh * A.group + row - tok * A.group) * HD + 4 * qd;
+                *reinterpret_cast<uint2*>(dst) = make_uint2(pack16(a.x, a.y, A.out_type), pack16(a.z, a.w, A.out_type));
             }
         }
-        cluster_sync_all();   // a CTA's shared memory stays until its peers have read it
     }
     if (CG == 2) cluster_sync_all();
     tc_after();
@@ -1167,20 +1176,31 @@ TcPlan tc_plan(const lev_ctx* ctx, int64_t rows, int seqs, int kv_heads, int tpt
         if (hd == 128) P.tiles = 2;
         else if (boxes) P.cg = 2;
     }
-    // few units: the CTAs of a cluster share the positions of one
-    const int64_t ctas = (mean + tpt * P.tiles * P.cg - 1) / (tpt * P.tiles * P.cg) * P.cg * seqs * kv_heads;
-    while (2 * P.splits * P.cg <= 8 && 2 * P.splits * ctas <= sms && 2 * P.splits * TC_KV <= span) P.splits *= 2;
     const int64_t per = (int64_t)tpt * P.tiles * P.cg;
-    P.units = rows / per + seqs < rows ? rows / per + seqs : rows;
+    P.units = rows > seqs ? (rows - seqs) / per + seqs : rows;   // at most, whatever the lengths
+    // Few units: the CTAs of a cluster share the positions of one, where that takes fewer steps (of about 1.4 us; the merge takes about
+    // two), counting that larger clusters find less room: with a whole SM to each CTA, 74, 33 or 15 of 2, 4 or 8 CTAs on 148 SMs run at
+    // once.  (14 units of 2 heads with 99 to 288 tokens: 16 us with clusters of 2 that all run at once, 34 with one of 4 too many.)
+    const int64_t steps = (span + TC_KV - 1) / TC_KV, clusters = P.units * kv_heads;
+    int64_t least = INT64_MAX;
+    for (int z = 1; z * P.cg <= TC_MAX_SPLITS; z *= 2) {
+        const int size = z * P.cg;
+        const int64_t fit = size == 1 ? sms : size == 2 ? sms / 2 : size == 4 ? sms * 33 / 148 : sms * 15 / 148;
+        const int64_t t = (clusters + fit - 1) / fit * ((steps + z - 1) / z + (z > 1 ? 2 : 0));
+        if (t < least) {
+            least = t;
+            P.splits = z;
+        }
+    }
     return P;
 }
 
-template <int HD, int TILES, int CG, int TYPE, bool COPY = false>
-int tc_launch(lev_ctx* ctx, const CUtensorMap& kmap, const CUtensorMap& vmap, const CUtensorMap& qmap, const TcArgs& A, int64_t units) {
+template <int HD, int TILES, int CG, int TYPE, bool COPY, bool SPLIT>
+int tc_launch_one(lev_ctx* ctx, const CUtensorMap& kmap, const CUtensorMap& vmap, const CUtensorMap& qmap, const TcArgs& A, int64_t units) {
     using D = TcDims<HD, TILES>;
     static bool configured[16] = {};
     if (!configured[ctx->device & 15]) {
-        LEV_CUDA(ctx, cudaFuncSetAttribute(k_attn_tc<HD, TILES, CG, TYPE, COPY>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)D::kSmem));
+        LEV_CUDA(ctx, cudaFuncSetAttribute(k_attn_tc<HD, TILES, CG, TYPE, COPY, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)D::kSmem));
         configured[ctx->device & 15] = true;
     }
     const int cluster = CG * A.splits;
@@ -1197,9 +1217,15 @@ int tc_launch(lev_ctx* ctx, const CUtensorMap& kmap, const CUtensorMap& vmap, co
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
-    LEV_CUDA(ctx, cudaLaunchKernelEx(&cfg, k_attn_tc<HD, TILES, CG, TYPE, COPY>, kmap, vmap, qmap, A));
+    LEV_CUDA(ctx, cudaLaunchKernelEx(&cfg, k_attn_tc<HD, TILES, CG, TYPE, COPY, SPLIT>, kmap, vmap, qmap, A));
     ctx->launches++;
     return lev_cuda_check(ctx, cudaGetLastError(), "k_attn_tc");
+}
+
+template <int HD, int TILES, int CG, int TYPE, bool COPY = false>
+int tc_launch(lev_ctx* ctx, const CUtensorMap& kmap, const CUtensorMap& vmap, const CUtensorMap& qmap, const TcArgs& A, int64_t units) {
+    return A.splits > 1 ? tc_launch_one<HD, TILES, CG, TYPE, COPY, true>(ctx, kmap, vmap, qmap, A, units)
+                        : tc_launch_one<HD, TILES, CG, TYPE, COPY, false>(ctx, kmap, vmap, qmap, A, units);
 }
 
 int tc_run(lev_ctx* ctx, EncodeTiledFn enc, const CUtensorMap& kmap, const CUtensorMap& vmap, TcArgs A, const TcPlan& P, int hd) {

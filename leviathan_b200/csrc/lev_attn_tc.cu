@@ -17,13 +17,22 @@
 // one.  Sums of weights are f32, O is f32 in tensor memory.  Rounded to 16 bits: q where it comes as f32 (the cache is
 // f16, and both operands of an MMA have one type), P (11 bits for f16, 8 for bf16 prompts), the output.
 //
-// Roles of a CTA: one (two) softmax warpgroup(s), one warp that issues MMAs, one that issues TMA boxes; where the cache
-// cannot be boxed (f32 pools, pages that are no whole groups of eight rows) the last three warps of the
-// CTA copy and convert rows instead.  Every wait is bounded (about a second, then LEV_TIMEOUT).
+// Roles of a CTA: one (two) softmax warpgroup(s), one warp that issues MMAs, three that request TMA boxes or, where the cache cannot be
+// boxed (f32 pools, pages that are no whole groups of eight rows), copy rows.  A CTA keeps its tensor memory and barriers from unit to
+// unit: the hardware hands it the next one of the grid, longest first (24 sequences of mixed lengths: 207 us with a CTA per unit, 176 so).
+// Every wait is bounded (about a second, then LEV_TIMEOUT).
 //
-// Places that a row does not attend to may hold anything, NaN included.  Scores there are replaced, but 0 * NaN is NaN
-// in the product with V: a row whose sums come out non-finite is computed once more, position by position, over the
-// places that it does attend to (tc_row_again; never taken where all values are finite).
+// Places that a row does not attend to may hold anything, NaN included.  Scores there are replaced, but 0 * NaN is NaN in the product
+// with V.  Behind the last position of a unit V becomes zeros in shared memory (100 tokens of 8 sequences with NaN in the unfilled part
+// of their last pages: 34 us, 70 ms without); elsewhere (above the diagonal, before the window) a row whose sums come out non-finite
+// is computed once more, position by position, over the places that it does attend to (tc_row_again; slow, and never taken where all
+// values are finite).
+//
+// What bounds it: for 16 heads of 256 on 8, a prompt of 4096 takes 104 us = 1.32 PFLOP/s (0.80 of a library product's burst rate; the
+// tensor pipe is active 70 % of the cycles, the rest is the diagonal's half steps and the softmax between two products).  For 32 heads of
+// 128 (two tiles) the warps that make the weights bound it: 24 chunks of mixed lengths 176 us = 0.74 PFLOP/s, the tensor pipe active 45 %;
+// an exponential costs as much as 8 of a tile's multiply-adds there.  Few tokens on a long cache: 26 sequences of 5 tokens, 33.6 MB, 20 us =
+// 1.7 TB/s, a chain of latencies (start, table, K, scores, weights, V, merge) of which the bytes take 5.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -36,7 +45,7 @@
 namespace {
 
 constexpr int TC_KV = 128;                 // positions per step
-constexpr int TC_MAX_SPLITS = 8;   // CTAs of a cluster that share a unit's positions
+constexpr int TC_MAX_SPLITS = 8;           // CTAs of a cluster that share a unit's positions
 constexpr unsigned TC_STAGE = 32768;       // 128 rows x 128 columns of 16 bits: two slabs of 64 columns
 constexpr int TC_MAX_STAGES = 6;
 constexpr int TC_LOAD_WARPS = 3;           // copying warps where TMA boxes do not apply
@@ -129,23 +138,30 @@ __device__ __forceinline__ void tc_qk(unsigned d, unsigned a_lo, unsigned b_lo, 
 #undef LEV_QK
     }
 }
-// O[128 x N] += P[128 x 128] V[128 x N]: P from tensor memory (64 columns of packed pairs), V N-major in shared memory.
-// Eight MMAs of 16 positions: P steps by 8 columns, V by two atoms of rows.  The descriptor's low word holds the address
-// and the distance between slabs.
+// O[128 x N] += P[128 x 16] V[16 x N]: P from tensor memory (packed pairs), V N-major in shared memory.  The descriptor's low word
+// holds the address and the distance between slabs.
 template <int CG>
-__device__ __forceinline__ void tc_pv(unsigned d, unsigned p, unsigned b_lo, unsigned b_hi, unsigned step, unsigned idesc, unsigned acc, unsigned elected) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
+__device__ __forceinline__ void tc_pv16(unsigned d, unsigned p, unsigned b_lo, unsigned b_hi, unsigned idesc, unsigned acc, unsigned elected) {
 #define LEV_PV(GROUP)                                                                                          \
     asm volatile(                                                                                              \
         "{\n .reg .pred p, q;\n .reg .b64 db;\n setp.ne.b32 p, %5, 0;\n setp.ne.b32 q, %6, 0;\n"               \
         " mov.b64 db, {%2, %4};\n"                                                                             \
         " @q tcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d),                 \
-        "r"(p + 8u * i), "r"(b_lo + step * i), "r"(idesc), "r"(b_hi), "r"(i ? 1u : acc), "r"(elected)          \
+        "r"(p), "r"(b_lo), "r"(idesc), "r"(b_hi), "r"(acc), "r"(elected)                                       \
         : "memory")
-        if (CG == 2) LEV_PV("2");
-        else LEV_PV("1");
+    if (CG == 2) LEV_PV("2");
+    else LEV_PV("1");
 #undef LEV_PV
+}
+// `steps` groups of 16 positions: P steps by 8 columns, V by two atoms of rows (`step`)
+template <int CG>
+__device__ __forceinline__ void tc_pv(unsigned d, unsigned p, unsigned b_lo, unsigned b_hi, unsigned step, int steps, unsigned idesc, unsigned acc, unsigned elected) {
+    if (steps == 8) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) tc_pv16<CG>(d, p + 8u * i, b_lo + step * i, b_hi, idesc, i ? 1u : acc, elected);
+    } else {
+#pragma unroll 1
+        for (int i = 0; i < steps; i++) tc_pv16<CG>(d, p + 8u * i, b_lo + step * i, b_hi, idesc, i ? 1u : acc, elected);
     }
 }
 // Packed rows: one box of 64 columns (column, head, row).  Cache pages: one box of whole atoms, all columns that the stage
@@ -184,6 +200,11 @@ struct TcUnit {
     int p_first, lo;    // position of its first row, lowest position that the unit attends to
     int jb, n;          // steps of 128 positions: the first one of this CTA's split and how many
     __device__ __forceinline__ int p_last() const { return p_first + tokens - 1; }
+    // of the last step's positions, those up to the last one that some row attends to
+    __device__ __forceinline__ int last_used() const {
+        const int left = p_last() + 1 - (jb + n - 1) * TC_KV;
+        return left < TC_KV ? left : TC_KV;
+    }
 };
 
 // Unit u of all sequences' units (each sequence has ceil(tokens / per)), those with most work first: of every 32 sequences the ones
@@ -455,9 +476,10 @@ struct TcDims {
 };
 
 // HD: head dimension.  TYPE: what the tensor core multiplies (LEV_ELEM_F16 or LEV_ELEM_BF16).  COPY: K and V rows are copied by
-// warps (kernels of their own: with both ways in one, 32 heads of 128 lost 5 % to the registers of the one not taken).  TILES: 128-row tiles of a CTA, each with a softmax warpgroup; one tile has two S buffers, two
-// tiles have one each.  CG = 2: a pair of CTAs (cta_group::2) with one tile each that share K and V.  splits > 1: the
-// CTAs of a cluster take parts of the positions and merge through distributed shared memory.
+// warps (kernels of their own: with both ways in one, 32 heads of 128 lost 5 % to the registers of the one not taken).  TILES: 128-row
+// tiles of a CTA, each with a softmax warpgroup; one tile has two S buffers, two tiles have one each.  CG = 2: a pair of CTAs
+// (cta_group::2) with one tile each that share K and V.  SPLIT: the CTAs of a cluster take parts of the positions and add up through
+// distributed shared memory (kernels of their own: 40 packed prompts 72 us with the runtime choice, 65 without).
 template <int HD, int TILES, int CG, int TYPE, bool COPY, bool SPLIT>
 __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
     k_attn_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap,
@@ -467,7 +489,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
     constexpr int KV_STAGES = CG == 2 ? 1 : HD / 128;   // stages of a K (or V) tile of this CTA
     constexpr int O_COL = 256;                          // tensor memory: S slots at 0 and 128, then O
     extern __shared__ unsigned char smem_dyn[];
-    __shared__ __align__(8) unsigned long long full[NS], empty[NS], s_full[2], p_full[2], pv_done[2], q_first, q_full, q_empty;
+    __shared__ __align__(8) unsigned long long full[NS], empty[NS], s_full[2], p_full[2], pv_done[2], q_first, q_full, q_empty, v_last, v_clean;
     __shared__ __align__(8) unsigned long long unit_full[2], unit_empty[2], answer_bar, told_bar[2];
     __shared__ __align__(16) unsigned answer_s[4];
     __shared__ unsigned tmem_base_s;
@@ -502,6 +524,8 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         mbar_init(smem_u32(&q_first), 4 * TILES * CG);   // without boxes: the softmax warps load the first unit's queries
         mbar_init(smem_u32(&q_empty), 1);
         mbar_init(smem_u32(&answer_bar), 1);
+        mbar_init(smem_u32(&v_last), 1);
+        mbar_init(smem_u32(&v_clean), 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
     }
@@ -738,7 +762,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         }
         tc_before();
         // rows that met a non-finite value where they do not attend (or where they do: the answer is then the same)
-        const unsigned again_warp = __ballot_sync(0xffffffffu, live && n > 0 && !bad && probe != 0.f);
+        const unsigned again_warp = __ballot_sync(0xffffffffu, live && n > 0 && !bad && probe != 0.f && l == l);   // (a sum of weights that is NaN: so is every column)
         if (lane == 0) again_s[tile * 4 + w4] = again_warp;
         wg_sync(1 + tile);
         unsigned again[4];
@@ -780,6 +804,23 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         }
     } else if (warp == D::kMma) {
         // ---- MMA issue (of a pair: the leader): the whole warp walks the loop, one elected lane issues ----
+        // A unit's last step takes whole groups of 16 positions.  V rows of the last group that no row attends to (pages that are not
+        // filled yet, rows behind the last prompt) become zeros once they have landed, while the softmax warps are at the step's weights:
+        // 0 times a NaN there would send every row to tc_row_again.  `steps`: of all units so far.
+        auto zeros = [&](int steps, int used) {
+            const TcLayout vl = tc_layout(A.table, 128, 128);
+            const int pieces = (16 - (used & 15)) * 2 * KV_STAGES * 8;   // 16 bytes each
+            for (int item = lane; item < pieces; item += 32) {
+                const int line = item >> 3, r = used + line / (2 * KV_STAGES), c = line % (2 * KV_STAGES);
+                const unsigned at = (unsigned)((2 * steps - 1) * KV_STAGES + (c >> 1)) % NS * TC_STAGE + (unsigned)(r >> 3) * vl.group + (unsigned)(c & 1) * vl.slab;
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};\n" ::"r"(ring + at + (unsigned)(r & 7) * 128u + (item & 7) * 16u), "r"(0) : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            __syncwarp();
+        };
+        // (of packed prompts, the last one's: behind the others lie rows in use)
+        auto cleaned = [&](const TcUnit& W) { return !COPY && (A.table || W.seq == A.seqs - 1); };
+        unsigned tails = 0;   // units that had to be cleaned
         if (rank == 0) {
             const unsigned elected = elect_lane();
             const unsigned fmt = TYPE == TC_BF16 ? (1u << 7) | (1u << 10) : 0u;
@@ -805,7 +846,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 }
                 tc_commit<CG>(smem_u32(&s_full[slot_i]), lead, elected);
             };
-            auto pv = [&](int tile, int slot_i, bool first, bool release) {   // O[tile] += P[slot] V
+            auto pv = [&](int tile, int slot_i, bool first, bool release, int steps) {   // O[tile] += P[slot] V
                 Ring st = vr;
 #pragma unroll
                 for (int h = 0; h < KV_STAGES; h++) {
@@ -813,8 +854,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                     tc_after();
                     const unsigned vb = ring + (unsigned)st.s * TC_STAGE;
                     const unsigned b_lo = ((vb >> 4) & 0x3FFFu) | ((vl.slab >> 4) << 16);
-                    tc_pv<CG>(tmem + O_COL + (TILES == 2 ? tile * 128u : h * 128u), tmem + (unsigned)slot_i * 128u, b_lo, vl.hi(), vl.group >> 3, id_pv,
-                              first ? 0u : 1u, elected);
+                    tc_pv<CG>(tmem + O_COL + (TILES == 2 ? tile * 128u : h * 128u), tmem + (unsigned)slot_i * 128u, b_lo, vl.hi(), vl.group >> 3, steps, id_pv, first ? 0u : 1u, elected);
                     if (release) tc_commit<CG>(smem_u32(&empty[st.s]), lead, elected);
                     st.step(1);
                 }
@@ -823,7 +863,19 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
             int g = 0;   // steps of all units so far
             Ring st(NS);
             for (int k = 0; have; have = next_unit(k++)) {
-                const int n = U.n;
+                const int n = U.n, used = n > 0 ? U.last_used() : 0, dirty = used & 15 && cleaned(U) ? used : 0;
+                auto tail = [&]() {
+                    if (!dirty) return;
+                    Ring at = vr;
+                    for (int h = 0; h < KV_STAGES; h++) {
+                        pk_wait(smem_u32(&full[at.s]), at.ph, abort_flag);
+                        at.step(1);
+                    }
+                    __syncwarp();
+                    if (CG == 2 && lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&v_last), lead + 1));
+                    zeros(g + 1, used);
+                    if (CG == 2) pk_wait(smem_u32(&v_clean), tails++ & 1, abort_flag);
+                };
                 if (A.q_boxes) pk_wait(smem_u32(&q_full), k & 1, abort_flag);
                 else if (k == 0) pk_wait(smem_u32(&q_first), 0, abort_flag);
                 else pk_wait(smem_u32(&q_full), (k - 1) & 1, abort_flag);
@@ -841,9 +893,10 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                     for (int i = 0; i < n; i++, g++) {
 #pragma unroll
                         for (int tile = 0; tile < 2; tile++) {
+                            if (tile == 0 && i == n - 1) tail();
                             pk_wait(smem_u32(&p_full[tile]), g & 1, abort_flag);
                             tc_after();
-                            pv(tile, tile, i == 0, tile == 1);
+                            pv(tile, tile, i == 0, tile == 1, i == n - 1 ? (used + 15) >> 4 : 8);
                             if (i + 1 < n) qk(tile, tile, tile == 1);
                         }
                         if (i + 2 == n) tc_commit<CG>(smem_u32(&q_empty), lead, elected);   // the unit's last use of its queries
@@ -866,16 +919,26 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                             st.step(KV_STAGES);
                             if (i + 2 == n) tc_commit<CG>(smem_u32(&q_empty), lead, elected);
                         }
+                        vr = st;
+                        if (i == n - 1) tail();
                         pk_wait(smem_u32(&p_full[g & 1]), (g >> 1) & 1, abort_flag);
                         tc_after();
-                        vr = st;
-                        pv(0, g & 1, i == 0, true);
+                        pv(0, g & 1, i == 0, true, i == n - 1 ? (used + 15) >> 4 : 8);
                         st.step(KV_STAGES);
                     }
                 }
             }
         } else {
-            for (int k = 0; have; have = next_unit(k++)) {}   // of a pair's second CTA: keeps the units' slots moving
+            int g = 0;   // of a pair's second CTA: cleans its columns of V and keeps the units' slots moving
+            for (int k = 0; have; have = next_unit(k++)) {
+                const int n = U.n, used = n > 0 ? U.last_used() : 0, dirty = used & 15 && cleaned(U) ? used : 0;
+                g += n;
+                if (dirty) {
+                    pk_wait(smem_u32(&v_last), tails++ & 1, abort_flag);
+                    zeros(g, used);
+                    if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&v_clean), lead));
+                }
+            }
         }
     } else {
         // ---- loads, by three warps, in the order in which the MMA warp takes the stages; the first of them also hands out units ----

@@ -229,6 +229,53 @@ def test_unattended_cache_may_hold_anything(ctx, junk, heads, n, at, window, pag
     check(torch.where(clean, got2, got), ref, mag, torch.float16)
 
 
+@pytest.mark.parametrize("heads", [(16, 8, 256), (8, 2, 128), (32, 8, 128)])
+@pytest.mark.parametrize("new,page", [(3, 16), (3, 128), (90, 64), (150, 128), (11, 24)])
+def test_what_lies_behind_the_last_position_changes_no_bit(ctx, heads, new, page):
+    """Sequences that end at every remainder of 16 (and with it of a step of 128), NaN against zeros behind each of them."""
+    qh, kvh, hd = heads
+    seqs = 33
+    new_of = [new + s % 5 for s in range(seqs)]
+    at = [s * 17 for s in range(seqs)]
+    P = Paged([a + n for a, n in zip(at, new_of)], page, kvh, hd, 7)
+    rows = [0]
+    for n in new_of:
+        rows.append(rows[-1] + n)
+    q = torch.randn((rows[-1], qh, hd), generator=torch.Generator(device=DEV).manual_seed(3), device=DEV).half()
+    outs = []
+    for junk in (0.0, math.nan):
+        for s in range(seqs):
+            end = at[s] + new_of[s]
+            for pool in (P.k, P.v):
+                if end % page:
+                    pool[int(P.table[s, end // page]), end % page:] = junk
+        outs.append(ctx.attn_chunk(P.cache, i32(rows), i32(list(range(seqs))), i32(at), q, 0, hd ** -0.5))
+        ctx.synchronize()
+    assert outs[0].isfinite().all()
+    assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("heads", [(16, 8, 256), (8, 2, 128), (32, 8, 128)])
+@pytest.mark.parametrize("lens", [[1], [130, 15], [700], [40] * 37 + [129]])
+def test_rows_behind_the_last_prompt_change_no_bit(ctx, heads, lens):
+    qh, kvh, hd = heads
+    rows = sum(lens)
+    start = i32([sum(lens[:i]) for i in range(len(lens) + 1)])
+    g = torch.Generator(device=DEV).manual_seed(9)
+    outs = []
+    q, k, v = (torch.randn((rows + 200, h, hd), generator=g, device=DEV).bfloat16() for h in (qh, kvh, kvh))
+    for junk in (0.0, math.nan):
+        for t in (q, k, v):
+            t[rows:] = junk
+        out = torch.full_like(q, 7.0)
+        ctx.attn_prompt(q, k, v, start, 0, hd ** -0.5, out=out)
+        ctx.synchronize()
+        assert (out[rows:] == 7.0).all()
+        outs.append(out[:rows])
+    assert outs[0].isfinite().all()
+    assert torch.equal(*outs)
+
+
 @pytest.mark.parametrize("heads", [(16, 8, 256), (8, 2, 128)])
 def test_other_prompts_may_hold_anything(ctx, heads):
     qh, kvh, hd = heads

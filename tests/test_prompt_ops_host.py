@@ -1,0 +1,71 @@
+"""What the many-row entry points refuse before any GPU work: arguments that are missing, tensors of the wrong type, layout or device."""
+import ctypes
+
+import pytest
+import torch
+
+from leviathan_b200 import _lib as L
+from leviathan_b200 import api
+
+
+@pytest.fixture(scope="module")
+def lib():
+    import os
+
+    if not os.path.exists(L.LIB_PATH):
+        from leviathan_b200.build import build_library
+
+        build_library()
+    return L.load()
+
+
+@pytest.mark.parametrize("name", ["lev_attn_chunk", "lev_attn_prompt", "lev_logprobs", "lev_norm_residual"])
+def test_null_arguments_are_an_error_code(lib, name):
+    f = getattr(lib, name)
+    args = [t() if t in (ctypes.c_int, ctypes.c_int32, ctypes.c_int64) else (t(0.0) if t is ctypes.c_float else None) for t in f.argtypes]
+    assert lib.lev_status_name(f(*args)) == b"badArgument"
+
+
+def test_head_rows():
+    api._torch()
+    fused = torch.zeros(5, 10, 128)
+    assert api._head_rows(fused[:, :6], "q") == (torch.Size([5, 6, 128]), 1280)
+    assert api._head_rows(fused[1:, 8:], "v") == (torch.Size([4, 2, 128]), 1280)
+    for bad in (torch.zeros(5, 128), fused[:, ::2], fused[..., ::2], fused.transpose(0, 1), fused[..., :64]):
+        with pytest.raises(ValueError, match="q: "):
+            api._head_rows(bad, "q")
+
+
+def test_element_types():
+    api._torch()
+    assert [api._elem(torch.zeros(1, dtype=t), "x", api._ANY) for t in (torch.float32, torch.float16, torch.bfloat16)] == [L.ELEM_F32, L.ELEM_F16, L.ELEM_BF16]
+    for t, allowed in ((torch.bfloat16, api._F32_F16), (torch.float32, api._ANY16), (torch.float64, api._ANY), (torch.int32, api._ANY)):
+        with pytest.raises(TypeError, match="x is "):
+            api._elem(torch.zeros(1, dtype=t), "x", allowed)
+
+
+def test_index_vectors():
+    api._torch()
+    api._i32(torch.zeros(3, dtype=torch.int32), 3, "start")
+    for bad in (torch.zeros(3, dtype=torch.int64), torch.zeros(4, dtype=torch.int32), torch.zeros(6, dtype=torch.int32)[::2]):
+        with pytest.raises(ValueError, match="start: 3"):
+            api._i32(bad, 3, "start")
+    with pytest.raises(ValueError, match="cuda:0"):
+        api._on(0, None, torch.zeros(1))
+
+
+def test_cache_over_pools_of_the_caller():
+    k = torch.zeros(4, 16, 2, 128, dtype=torch.float16)
+    table = torch.zeros(2, 3, dtype=torch.int32)
+    c = api.PagedKV.over(k, torch.zeros_like(k), table)
+    l = c.layout
+    assert (l.kv_type, l.page, l.kv_heads, l.head_dim, l.blocks, l.max_blocks, l.slots) == (L.KV_F16, 16, 2, 128, 4, 3, 2)
+    assert c.k is k and c.table is table
+    with pytest.raises(ValueError):
+        api.PagedKV.over(k, torch.zeros(4, 16, 2, 64, dtype=torch.float16), table)
+    with pytest.raises(ValueError):
+        api.PagedKV.over(k, torch.zeros(4, 2, 16, 128, dtype=torch.float16).transpose(1, 2), table)
+    with pytest.raises(ValueError):
+        api.PagedKV.over(k, torch.zeros_like(k), table.long())
+    with pytest.raises(TypeError):
+        api.PagedKV.over(k.bfloat16(), k.bfloat16(), table)

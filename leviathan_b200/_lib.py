@@ -182,15 +182,27 @@ def load() -> C.CDLL:
     return lib
 
 
+class _CtypesRows:
+    """The same for the calls over many rows."""
+
+    def __init__(self, lib: C.CDLL):
+        self._lib = lib
+        for name in ("attn_prompt", "norm_residual", "logprobs"):
+            setattr(self, name, getattr(lib, "lev_" + name))
+
+    def attn_chunk(self, ctx, layout, *args):
+        return self._lib.lev_attn_chunk(ctx, C.cast(layout, C.POINTER(KVLayout)), *args)
+
+
 class _CtypesHost:
     """The calls of csrc/lev_pyhost.c through ctypes, for an interpreter it is not built for: the same arguments, a
     microsecond or two more per call."""
 
     def __init__(self, lib: C.CDLL):
         self._lib = lib
-        for name in ("matvec", "rmsnorm", "axpy", "act_bf16", "gemm_prefill", "moe_layer", "moe_layer_residual", "attn_prompt",
-                     "norm_residual", "logprobs"):
+        for name in ("matvec", "rmsnorm", "axpy", "act_bf16", "gemm_prefill", "moe_layer", "moe_layer_residual"):
             setattr(self, name, getattr(lib, "lev_" + name))
+        self._rows = _CtypesRows(lib)
 
     def matvec_fused(self, ctx, w, row0, rows, x, x_count, n_cols, prologue, norm_weight, eps, residual, alpha, y, cap):
         f = Fusion(prologue, norm_weight, eps, residual, alpha)
@@ -201,9 +213,6 @@ class _CtypesHost:
 
     def kv_append(self, ctx, layout, *args):
         return self._lib.lev_kv_append(ctx, C.cast(layout, C.POINTER(KVLayout)), *args)
-
-    def attn_chunk(self, ctx, layout, *args):
-        return self._lib.lev_attn_chunk(ctx, C.cast(layout, C.POINTER(KVLayout)), *args)
 
     def attn_decode(self, ctx, layout, *args):
         return self._lib.lev_attn_decode(ctx, C.cast(layout, C.POINTER(KVLayout)), *args)

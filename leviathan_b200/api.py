@@ -142,6 +142,7 @@ class Context:
         self._stream_seen = None
         self._like = None
         self.lib, self.host = L.load(), L.host()
+        self._rows = self.host._rows   # the calls over many rows
         h = C.c_void_p()
         st = self.lib.lev_cuda_init(device, C.byref(h))
         if st != L.OK:
@@ -365,7 +366,7 @@ class Context:
             gate_ld = gate.stride(0) if gate.ndim == 2 and rows > 1 else 0
         _on(self.device, x, residual, post, pre, gate, out, h)
         self._flags(False, False)
-        self._check(self.host.norm_residual(self._h, _dp(x), _dp(residual), rows, n, int(post is not None if norm_post is None else norm_post),
+        self._check(self._rows.norm_residual(self._h, _dp(x), _dp(residual), rows, n, int(post is not None if norm_post is None else norm_post),
                                             _dp(post), _dp(gate), gate_ld, alpha, scale, _dp(pre), eps, _dp(out), _dp(h), ht))
         return out, h
 
@@ -390,7 +391,7 @@ class Context:
         if top > 0:
             ids, lps = i32.new_empty((rows, top)), f32.new_empty((rows, top))
         self._flags(False, False)
-        self._check(self.host.logprobs(self._h, logits.data_ptr(), ty, rows, n, ld if rows > 1 else n, softcap, _dp(tokens), top, _dp(lp),
+        self._check(self._rows.logprobs(self._h, logits.data_ptr(), ty, rows, n, ld if rows > 1 else n, softcap, _dp(tokens), top, _dp(lp),
                                        entropy.data_ptr(), _dp(ids), _dp(lps)))
         return lp, entropy, ids, lps
 
@@ -577,7 +578,7 @@ class Context:
         _i32(pos, n, "pos")
         qt, ot = _elem(q, "q", _F32_F16), _elem(out, "out", _ANY16)
         self._flags(False, False)
-        self._check(self.host.attn_chunk(self._h, C.addressof(cache.layout), _dp(cache.k), _dp(cache.v), _dp(cache.table), n, _dp(start),
+        self._check(self._rows.attn_chunk(self._h, C.addressof(cache.layout), _dp(cache.k), _dp(cache.v), _dp(cache.table), n, _dp(start),
                                          _dp(slot), _dp(pos), shape[0], shape[1], _dp(q), qt, q_ld, window, scale, _dp(out), ot, out_ld))
         return out
 
@@ -599,7 +600,7 @@ class Context:
         if not (q.dtype is k.dtype is v.dtype is out.dtype):
             raise TypeError(f"q, k, v and out are of one type: got {q.dtype}, {k.dtype}, {v.dtype}, {out.dtype}")
         self._flags(False, False)
-        self._check(self.host.attn_prompt(self._h, n, _dp(start), rows, q_heads, kv_shape[1], hd, ty, _dp(q), q_ld, _dp(k), k_ld, _dp(v), v_ld,
+        self._check(self._rows.attn_prompt(self._h, n, _dp(start), rows, q_heads, kv_shape[1], hd, ty, _dp(q), q_ld, _dp(k), k_ld, _dp(v), v_ld,
                                           window, scale, _dp(out), out_ld))
         return out
 

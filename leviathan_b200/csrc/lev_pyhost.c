@@ -85,7 +85,14 @@ HOST_FN(logprobs, 13, lev_ctx* c = P(a[0]); void* x = P(a[1]); long long ty = I(
 #define ENTRY(NAME) {#NAME, (PyCFunction)(void (*)(void))NAME, METH_FASTCALL, NULL}
 static PyMethodDef methods[] = {ENTRY(matvec), ENTRY(matvec_fused), ENTRY(matvec_chain), ENTRY(rmsnorm), ENTRY(axpy),
                                 ENTRY(act_bf16), ENTRY(gemm_prefill), ENTRY(moe_layer), ENTRY(moe_layer_residual), ENTRY(kv_append),
-                                ENTRY(attn_decode), ENTRY(attn_chunk), ENTRY(attn_prompt),
-                                ENTRY(norm_residual), ENTRY(logprobs), {NULL, NULL, 0, NULL}};
+                                ENTRY(attn_decode), {NULL, NULL, 0, NULL}};
+/* the calls over many rows: the module's _rows */
+static PyMethodDef row_methods[] = {ENTRY(attn_chunk), ENTRY(attn_prompt), ENTRY(norm_residual), ENTRY(logprobs), {NULL, NULL, 0, NULL}};
+static struct PyModuleDef rows_module = {PyModuleDef_HEAD_INIT, "_pyhost._rows", NULL, -1, row_methods, NULL, NULL, NULL, NULL};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pyhost", NULL, -1, methods, NULL, NULL, NULL, NULL};
-PyMODINIT_FUNC PyInit__pyhost(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__pyhost(void) {
+    PyObject *m = PyModule_Create(&module), *rows = m ? PyModule_Create(&rows_module) : NULL;
+    if (m && (!rows || PyModule_AddObjectRef(m, "_rows", rows) < 0)) Py_CLEAR(m);
+    Py_XDECREF(rows);
+    return m;
+}

@@ -69,3 +69,25 @@ def test_cache_over_pools_of_the_caller():
         api.PagedKV.over(k, torch.zeros_like(k), table.long())
     with pytest.raises(TypeError):
         api.PagedKV.over(k.bfloat16(), k.bfloat16(), table)
+
+
+# the arguments each native call over many rows takes, handles NULL
+ROW_CALLS = {
+    "attn_chunk": (None, None, None, None, None, 1, None, None, None, 1, 8, None, 0, 1024, 0, 1.0, None, 2, 1024),
+    "attn_prompt": (None, 1, None, 1, 8, 2, 128, 2, None, 1024, None, 256, None, 256, 0, 1.0, None, 1024),
+    "norm_residual": (None, None, None, 1, 32, 0, None, None, 0, 1.0, 1.0, None, 1e-6, None, None, 0),
+    "logprobs": (None, None, 0, 1, 32, 32, 0.0, None, 0, None, None, None, None),
+}
+
+
+def test_row_calls_native_and_through_ctypes(lib, monkeypatch, tmp_path):
+    native = L.host()._rows
+    assert sorted(n for n in dir(native) if not n.startswith("_")) == sorted(ROW_CALLS)
+    monkeypatch.setattr(L, "_host", None)
+    monkeypatch.setattr(L, "HOST_PATH", str(tmp_path / "missing.so"))
+    through_ctypes = L.host()._rows
+    for name, args in ROW_CALLS.items():
+        for form in (native, through_ctypes):
+            assert L.STATUS[getattr(form, name)(*args)] == "badArgument", name
+            with pytest.raises(TypeError):
+                getattr(form, name)(*args[:-1])

@@ -429,10 +429,10 @@ int lev_qkv_norm_rope_append_split(lev_ctx* ctx, float* q, float* k, float* v, i
  *   q f32 (rounded to f16: magnitudes above 65504 are not served) or f16, out f16 or bf16 (what lev_gemm_prefill reads);
  *   rows q_ld and out_ld elements apart (whole 16-byte steps, 16-byte aligned), heads contiguous: q may be the leading part of
  *   each row of a fused projection output.  out must not overlap q.  f32 caches are rounded to f16 in the same way.
- *   head_dim 128 or 256; up to 16 query heads per KV head; any page size (powers of two from 8 on are fastest).
+ *   head_dim 128 or 256; up to 16 query heads per KV head; any page size (multiples of 8 are fastest).
  * A slot or position outside the layout, or a table entry outside the pool, is not followed: rows of that chunk are NaN; start entries
  * that are no range leave their chunk out; both are reported by the next status read.  Cached values that a row does not attend to may
- * be anything, NaN included.  No work buffers: captured graphs and streams share nothing.  Repeat runs give the same bits. */
+ * be anything, NaN included (in front of a window or among the new tokens they cost a second, slow pass over the rows concerned).  No work buffers: captured graphs and streams share nothing.  Repeat runs give the same bits. */
 int lev_attn_chunk(lev_ctx* ctx, const lev_kv_layout* layout, const void* k_pool, const void* v_pool,
                    const int32_t* block_table, int n_chunks, const int32_t* start, const int32_t* slot,
                    const int32_t* pos, int64_t n_rows, int q_heads, const void* q, int q_type,

@@ -31,8 +31,8 @@
 // What bounds it: for 16 heads of 256 on 8, a prompt of 4096 takes 104 us = 1.32 PFLOP/s (0.80 of a library product's burst rate; the
 // tensor pipe is active 70 % of the cycles, the rest is the diagonal's half steps and the softmax between two products).  For 32 heads of
 // 128 (two tiles) the warps that make the weights bound it: 24 chunks of mixed lengths 176 us = 0.74 PFLOP/s, the tensor pipe active 45 %;
-// an exponential costs as much as 8 of a tile's multiply-adds there.  Few tokens on a long cache: 26 sequences of 5 tokens, 33.6 MB, 20 us =
-// 1.7 TB/s, a chain of latencies (start, table, K, scores, weights, V, merge) of which the bytes take 5.
+// an exponential costs as much as 8 of a tile's multiply-adds there.  Few tokens on a long cache: 5 tokens behind 4091
+// positions, 33.6 MB, 20 us = 1.7 TB/s, a chain of latencies (start, table, K, scores, weights, V, merge) of which the bytes take 5.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

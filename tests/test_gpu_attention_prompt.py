@@ -146,6 +146,20 @@ def test_long_cache_is_split(ctx, heads, n):
     run_chunk(ctx, [n], [2900], 16, heads, seed=n)
 
 
+@pytest.mark.parametrize("heads", [(14, 2, 128), (5, 1, 256), (16, 1, 128), (11, 1, 128), (16, 8, 256)])
+@pytest.mark.parametrize("lens,ctxs,window,page", [([1], [1500], 0, 16), ([3, 70, 0, 19], [700, 1290, 5, 1], 0, 16), ([200], [1900], 0, 32),
+                                                   ([40, 9], [2100, 300], 900, 16), ([17, 2], [1000, 1500], 0, 5), ([129], [3], 0, 16)])
+def test_parts_of_uneven_tiles(ctx, heads, lens, ctxs, window, page):
+    """few units, so that clusters share their positions: rows that no number of parts divides, parts that some units have none of"""
+    run_chunk(ctx, lens, ctxs, page, heads, window, seed=sum(lens))
+
+
+@pytest.mark.parametrize("heads", [(7, 1, 128), (3, 1, 256), (4, 2, 128)])
+@pytest.mark.parametrize("lens", [[600], [90, 1, 300]])
+def test_parts_of_prompts(ctx, heads, lens):
+    run_prompt(ctx, lens, heads, torch.float16)
+
+
 @pytest.mark.parametrize("heads", HEADS)
 def test_full_grid(ctx, heads):
     """enough tiles that nothing is split: CTA pairs, two tiles per CTA"""
@@ -187,6 +201,10 @@ def test_prompt_windows(ctx, window, heads):
 @pytest.mark.parametrize("heads", [(16, 8, 256), (8, 2, 128)])
 def test_one_long_prompt(ctx, heads):
     run_prompt(ctx, [2500], heads, torch.bfloat16)
+
+
+def test_a_prompt_of_9000(ctx):
+    run_prompt(ctx, [9000], (2, 1, 128), torch.bfloat16)
 
 
 # ---- values that nothing attends to, indices outside the layout ----

@@ -107,3 +107,27 @@ def test_refusals(ctx):
         kw = dict(dict(x=x, residual=res, pre=w), **kw)
         with pytest.raises((ValueError, TypeError)):
             ctx.norm_residual(**kw)
+
+
+@pytest.mark.parametrize("rows,n", [(1, 2816), (300, 2816), (5, 9001)])
+def test_captured_replayed_and_on_another_stream(ctx, rows, n):
+    x, res, w1, w2 = (torch.randn(s, device=DEV) for s in ((rows, n), (rows, n), (n,), (n,)))
+    out, h = ctx.norm_residual(x, res, post=w1, pre=w2, dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    out2, h2 = torch.zeros_like(out), torch.zeros_like(h)
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(g, stream=s):
+        a, b = ctx.norm_residual(x, res, post=w1, pre=w2, dtype=torch.bfloat16)
+        out2.copy_(a)
+        h2.copy_(b)
+    for _ in range(2):
+        out2.zero_()
+        h2.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out2, out) and torch.equal(h2, h)
+    with torch.cuda.stream(s):
+        a, b = ctx.norm_residual(x, res, post=w1, pre=w2, dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    assert torch.equal(a, out) and torch.equal(b, h)

@@ -20,7 +20,7 @@
 // Roles of a CTA: one (two) softmax warpgroup(s), one warp that issues MMAs, three that request TMA boxes or, where the cache cannot be
 // boxed (f32 pools, pages that are no whole groups of eight rows), copy rows.  A CTA keeps its tensor memory and barriers from unit to
 // unit: the hardware hands it the next one of the grid, longest first (24 sequences of mixed lengths: 207 us with a CTA per unit, 176 so).
-// Every wait is bounded (about a second, then LEV_TIMEOUT).
+// Every wait is bounded (about 16 seconds, then LEV_TIMEOUT).
 //
 // Places that a row does not attend to may hold anything, NaN included.  Scores there are replaced, but 0 * NaN is NaN in the product
 // with V.  Behind the last position of a unit V becomes zeros in shared memory (100 tokens of 8 sequences with NaN in the unfilled part
@@ -98,6 +98,11 @@ __device__ __forceinline__ void swap_pieces(uint4& a, uint4& b, int bit, int lan
     got.w = __shfl_xor_sync(0xffffffffu, send.w, bit);
     if (up) a = got;
     else b = got;
+}
+// Bounded, with patience: a tile whose rows meet NaN among the values they attend to goes over its positions again row by row (30 us
+// for each of them and 128 positions: a second at 33000 positions), and everybody else waits.
+__device__ __forceinline__ bool tc_wait(unsigned bar, unsigned parity, volatile int* abort_flag) {
+    return pk_try(bar, parity) || pk_wait_slow<16>(bar, parity, abort_flag);
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
@@ -556,7 +561,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&unit_empty[k & 1]));
         k++;
-        pk_wait(smem_u32(&unit_full[k & 1]), ((k - 1) >> 1) & 1, abort_flag);
+        tc_wait(smem_u32(&unit_full[k & 1]), ((k - 1) >> 1) & 1, abort_flag);
         __syncwarp();
         U = unit_s[k & 1];
         return U.tokens > 0 && !*abort_flag;
@@ -598,7 +603,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         for (int i = 0; i < n; i++, g++) {
             const int slot_i = TILES == 2 ? tile : g & 1, par = TILES == 2 ? g & 1 : (g >> 1) & 1;
             const unsigned s_addr = lane_base + (unsigned)slot_i * 128u;
-            pk_wait(smem_u32(&s_full[slot_i]), par, abort_flag);
+            tc_wait(smem_u32(&s_full[slot_i]), par, abort_flag);
             __syncwarp();
             tc_after();
             unsigned s[128];
@@ -626,7 +631,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
             }
             if (i > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
                 const int prev = TILES == 2 ? tile : (g - 1) & 1, ppar = TILES == 2 ? (g - 1) & 1 : ((g - 1) >> 1) & 1;
-                pk_wait(smem_u32(&pv_done[prev]), ppar, abort_flag);
+                tc_wait(smem_u32(&pv_done[prev]), ppar, abort_flag);
                 __syncwarp();
                 tc_after();
                 sum = fma_2(sum, two(corr, corr), two(0.f, 0.f));
@@ -681,7 +686,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         }
         if (n > 0) {
             const int last = TILES == 2 ? tile : (g - 1) & 1, lpar = TILES == 2 ? (g - 1) & 1 : ((g - 1) >> 1) & 1;
-            pk_wait(smem_u32(&pv_done[last]), lpar, abort_flag);
+            tc_wait(smem_u32(&pv_done[last]), lpar, abort_flag);
             __syncwarp();
             tc_after();
         }
@@ -833,7 +838,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 Ring st = kr;
 #pragma unroll
                 for (int h = 0; h < KV_STAGES; h++) {
-                    pk_wait(smem_u32(&full[st.s]), st.ph, abort_flag);
+                    tc_wait(smem_u32(&full[st.s]), st.ph, abort_flag);
                     tc_after();
                     const unsigned kb = ring + (unsigned)st.s * TC_STAGE;
                     constexpr int kSlabs = HD / 64 / KV_STAGES;
@@ -850,7 +855,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 Ring st = vr;
 #pragma unroll
                 for (int h = 0; h < KV_STAGES; h++) {
-                    pk_wait(smem_u32(&full[st.s]), st.ph, abort_flag);
+                    tc_wait(smem_u32(&full[st.s]), st.ph, abort_flag);
                     tc_after();
                     const unsigned vb = ring + (unsigned)st.s * TC_STAGE;
                     const unsigned b_lo = ((vb >> 4) & 0x3FFFu) | ((vl.slab >> 4) << 16);
@@ -868,17 +873,17 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                     if (!dirty) return;
                     Ring at = vr;
                     for (int h = 0; h < KV_STAGES; h++) {
-                        pk_wait(smem_u32(&full[at.s]), at.ph, abort_flag);
+                        tc_wait(smem_u32(&full[at.s]), at.ph, abort_flag);
                         at.step(1);
                     }
                     __syncwarp();
                     if (CG == 2 && lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&v_last), lead + 1));
                     zeros(g + 1, used);
-                    if (CG == 2) pk_wait(smem_u32(&v_clean), tails++ & 1, abort_flag);
+                    if (CG == 2) tc_wait(smem_u32(&v_clean), tails++ & 1, abort_flag);
                 };
-                if (A.q_boxes) pk_wait(smem_u32(&q_full), k & 1, abort_flag);
-                else if (k == 0) pk_wait(smem_u32(&q_first), 0, abort_flag);
-                else pk_wait(smem_u32(&q_full), (k - 1) & 1, abort_flag);
+                if (A.q_boxes) tc_wait(smem_u32(&q_full), k & 1, abort_flag);
+                else if (k == 0) tc_wait(smem_u32(&q_first), 0, abort_flag);
+                else tc_wait(smem_u32(&q_full), (k - 1) & 1, abort_flag);
                 tc_after();
                 if (TILES == 2) {
                     // stages: K0 V0 K1 V1 ...
@@ -894,7 +899,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
 #pragma unroll
                         for (int tile = 0; tile < 2; tile++) {
                             if (tile == 0 && i == n - 1) tail();
-                            pk_wait(smem_u32(&p_full[tile]), g & 1, abort_flag);
+                            tc_wait(smem_u32(&p_full[tile]), g & 1, abort_flag);
                             tc_after();
                             pv(tile, tile, i == 0, tile == 1, i == n - 1 ? (used + 15) >> 4 : 8);
                             if (i + 1 < n) qk(tile, tile, tile == 1);
@@ -921,7 +926,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                         }
                         vr = st;
                         if (i == n - 1) tail();
-                        pk_wait(smem_u32(&p_full[g & 1]), (g >> 1) & 1, abort_flag);
+                        tc_wait(smem_u32(&p_full[g & 1]), (g >> 1) & 1, abort_flag);
                         tc_after();
                         pv(0, g & 1, i == 0, true, i == n - 1 ? (used + 15) >> 4 : 8);
                         st.step(KV_STAGES);
@@ -934,7 +939,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 const int n = U.n, used = n > 0 ? U.last_used() : 0, dirty = used & 15 && cleaned(U) ? used : 0;
                 g += n;
                 if (dirty) {
-                    pk_wait(smem_u32(&v_last), tails++ & 1, abort_flag);
+                    tc_wait(smem_u32(&v_last), tails++ & 1, abort_flag);
                     zeros(g, used);
                     if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&v_clean), lead));
                 }
@@ -996,7 +1001,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 const unsigned row_bytes = (is_v ? kSlabsV : kSlabsK) * 128u;
 #pragma unroll
                 for (int h = 0; h < KV_STAGES; h++) {
-                    pk_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
+                    tc_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
                     const unsigned bar = full_c + 8u * (unsigned)st.s, dst = ring + (unsigned)st.s * TC_STAGE;
                     if (rank == 0 && w == 0) pk_expect(smem_u32(&full[st.s]), TC_STAGE * CG, elected);
                     const int x0 = CG == 2 ? (is_v ? (int)rank * 128 : 0) : h * 128;
@@ -1027,7 +1032,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 const int piece = lane & 15, sub = lane >> 4;   // two rows of 16 pieces (8 values each) per step of a warp
                 const char* pool = static_cast<const char*>(is_v ? A.v : A.k);
                 for (int h = 0; h < KV_STAGES; h++) {
-                    pk_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
+                    tc_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
                     const unsigned dst = ring + (unsigned)st.s * TC_STAGE + (unsigned)(piece >> 3) * 16384u;
                     auto row = [&](int r, int64_t* off) {
                         const int64_t v = (r >> 5) == 0 ? R.off[0] : (r >> 5) == 1 ? R.off[1] : (r >> 5) == 2 ? R.off[2] : R.off[3];
@@ -1089,7 +1094,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 if (i == 0) {
                     // This unit's queries, when the last product that read the ones before is done.  The first K tile has been asked
                     // for: waiting any later could wait for a stage that only these queries would free.
-                    if (k > 0) pk_wait(smem_u32(&q_empty), (k - 1) & 1, abort_flag);
+                    if (k > 0) tc_wait(smem_u32(&q_empty), (k - 1) & 1, abort_flag);
                     __syncwarp();
                     if (A.q_boxes) {   // one box of 64 columns: the group's heads of a tile's tokens
                         if (w == 0) {
@@ -1125,7 +1130,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
             if (w == 0) {
                 int x;
                 if (rank == 0) {
-                    pk_wait(smem_u32(&answer_bar), k & 1, abort_flag);
+                    tc_wait(smem_u32(&answer_bar), k & 1, abort_flag);
                     x = *abort_flag ? -1 : tc_next_taken(smem_u32(answer_s));
                     __syncwarp();
                     if (lane == 0) {
@@ -1138,14 +1143,14 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                     }
                 } else {
                     if (lane == 0) mbar_expect(smem_u32(&told_bar[k & 1]), 4);
-                    pk_wait(smem_u32(&told_bar[k & 1]), (k >> 1) & 1, abort_flag);
+                    tc_wait(smem_u32(&told_bar[k & 1]), (k >> 1) & 1, abort_flag);
                     __syncwarp();
                     x = *abort_flag ? -1 : *(volatile int*)&told_s[k & 1];
                 }
                 have = x >= 0 && tc_unit(A, x / cluster, per, split, lane, &U);
                 if (have && rank == 0 && lane == 0) tc_next_request(smem_u32(answer_s), smem_u32(&answer_bar));
                 // unit k + 1 goes where unit k - 1 was
-                if (k > 0) pk_wait(smem_u32(&unit_empty[(k + 1) & 1]), ((k - 1) >> 1) & 1, abort_flag);
+                if (k > 0) tc_wait(smem_u32(&unit_empty[(k + 1) & 1]), ((k - 1) >> 1) & 1, abort_flag);
                 __syncwarp();
                 if (lane == 0) {
                     if (!have) U.tokens = 0;
@@ -1158,9 +1163,9 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 have = next_unit(k);
             }
         }
-        if (units) pk_wait(smem_u32(&q_empty), (units - 1) & 1, abort_flag);   // the tensor core's last releases have arrived
+        if (units) tc_wait(smem_u32(&q_empty), (units - 1) & 1, abort_flag);   // the tensor core's last releases have arrived
         for (int s = 0; s < NS; s++) {
-            pk_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
+            tc_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
             st.step(1);
         }
     }

@@ -247,6 +247,24 @@ def test_unattended_cache_may_hold_anything(ctx, junk, heads, n, at, window, pag
     check(torch.where(clean, got2, got), ref, mag, torch.float16)
 
 
+def test_nan_far_back_in_a_long_cache(ctx):
+    """Every row attends to a NaN: its column is NaN, the others are what they were, and no wait runs out meanwhile (128 units of 128 rows
+    that are all gone over again, about a second and a half)."""
+    P = Paged([45064], 16, 8, 256, 5, spare=0)
+    q = torch.randn((16 * 64, 16, 256), generator=torch.Generator(device=DEV).manual_seed(3), device=DEV).half()
+    args = (i32([64 * c for c in range(17)]), i32([0] * 16), i32([45000] * 16), q, 0, 1 / 16)
+    before = ctx.attn_chunk(P.cache, *args, dtype=torch.float16)
+    P.v[int(P.table[0, 0]), 5, :, 3] = math.nan
+    got = ctx.attn_chunk(P.cache, *args, dtype=torch.float16)
+    ctx.synchronize()
+    assert got[..., 3].isnan().all()
+    got[..., 3] = before[..., 3]
+    assert before.isfinite().all() and got.isfinite().all()
+    # each is as close to the exact answer as `check` asks; the sum of p |v| over so many normal values is 0.80, below 0.9
+    u = U[torch.float16]
+    assert ((got - before).float().abs() <= 2 * ((u + 5e-4) * 0.9 + u * before.float().abs() + 1e-7)).all()
+
+
 @pytest.mark.parametrize("heads", [(16, 8, 256), (8, 2, 128), (32, 8, 128)])
 @pytest.mark.parametrize("new,page", [(3, 16), (3, 128), (90, 64), (150, 128), (11, 24)])
 def test_what_lies_behind_the_last_position_changes_no_bit(ctx, heads, new, page):

@@ -38,6 +38,7 @@
 
 #include <type_traits>
 
+#include "lev_attn_ring.h"
 #include "lev_math2.cuh"
 #include "lev_stream.h"
 #include "lev_umma.cuh"
@@ -48,7 +49,6 @@ constexpr int TC_KV = 128;                 // positions per step
 constexpr int TC_MAX_SPLITS = 8;           // CTAs of a cluster that share a unit's positions
 constexpr unsigned TC_STAGE = 32768;       // 128 rows x 128 columns of 16 bits: two slabs of 64 columns
 constexpr int TC_MAX_STAGES = 6;
-constexpr int TC_LOAD_WARPS = 3;           // copying warps where TMA boxes do not apply
 constexpr float TC_LAZY = 8.0f;            // how far (log2) the maximum may run ahead of a row's reference
 enum { TC_F32 = LEV_ELEM_F32, TC_F16 = LEV_ELEM_F16, TC_BF16 = LEV_ELEM_BF16 };
 
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         abort_s = 0;
         bad_s[0] = bad_s[1] = 0;
         for (int s = 0; s < NS; s++) {
-            mbar_init(smem_u32(&full[s]), COPY ? TC_LOAD_WARPS : 1);
+            mbar_init(smem_u32(&full[s]), tc_full_count(COPY, CG));   // every warp that waits for `empty` (lev_attn_ring.h)
             mbar_init(smem_u32(&empty[s]), 1);
         }
         for (int s = 0; s < 2; s++) {
@@ -1016,6 +1016,10 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                         for (int b = w; b < (is_v ? kSlabsV : kSlabsK); b += TC_LOAD_WARPS)
                             tc_box_rows<CG>(dst + (unsigned)(b * r_n) * 128u, map, x0 + 64 * b, U.kvh, U.row0 + (jb + i) * TC_KV + r_first, bar, elected);
                     }
+                    if (tc_full_arrives(w) && lane == 0) {
+                        if (CG == 2) mbar_arrive_cluster(bar);
+                        else mbar_arrive(bar);
+                    }
                     st.step(1);
                 }
             };
@@ -1094,7 +1098,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 if (i == 0) {
                     // This unit's queries, when the last product that read the ones before is done.  The first K tile has been asked
                     // for: waiting any later could wait for a stage that only these queries would free.
-                    if (k > 0) tc_wait(smem_u32(&q_empty), (k - 1) & 1, abort_flag);
+                    if (k > 0 && tc_waits_for_queries(A.q_boxes, w)) tc_wait(smem_u32(&q_empty), (k - 1) & 1, abort_flag);
                     __syncwarp();
                     if (A.q_boxes) {   // one box of 64 columns: the group's heads of a tile's tokens
                         if (w == 0) {
@@ -1163,7 +1167,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 have = next_unit(k);
             }
         }
-        if (units) tc_wait(smem_u32(&q_empty), (units - 1) & 1, abort_flag);   // the tensor core's last releases have arrived
+        if (units && tc_waits_for_queries(A.q_boxes, w)) tc_wait(smem_u32(&q_empty), (units - 1) & 1, abort_flag);   // the tensor core's last releases have arrived
         for (int s = 0; s < NS; s++) {
             tc_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
             st.step(1);

@@ -4,8 +4,9 @@
 //   lse = log sum_i e^x_i,   logprob = x_token - lse,   entropy = lse - sum_i e^(x_i - lse) x_i
 //   alternatives: the `top` largest l_i (the cap is monotone), ties to the lowest index like lev_argmax, with x_i - lse
 //
-// The row is read once.  Each thread keeps a running maximum m, s1 = sum e^(x - m) and s2 = sum e^(x - m) (x - m) (all in units
-// of log 2), f32 over a few hundred to a few thousand values, then trees in a fixed order.
+// The row is read once.  Each thread keeps a running maximum m, s1 = sum e^(x - m) and s2 = sum e^(x - m) (x - m), f32 over a few hundred
+// to a few thousand values, then trees in a fixed order.  Without a cap the maximum is subtracted before the difference goes to units of
+// log 2: a product with log2(e) first is rounded by more than any weight can bear from 2^31 on, and infinite for a type's lowest value.
 //
 // Alternatives: a thread's values of one round make a batch, and all that the pass over the row does for them is to leave the
 // batch's maximum in shared memory (with keys pushed under a running threshold in every round, 512 rows of 262144 took a
@@ -53,24 +54,32 @@ __device__ __forceinline__ float min_nan(float a, float b) {   // NaN if one is 
     asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
-// x in units of log 2 relative to ref2: tanh from a power of two and a reciprocal, 1 - 2 / (1 + e^(2 l / cap)); from an exponent of
-// 30 on the quotient is below f32's grid at 1
+// x in units of log 2 relative to the reference, which is a logit without a cap and a capped value in units of log 2 with one: tanh from a
+// power of two and a reciprocal, 1 - 2 / (1 + e^(2 l / cap)); from an exponent of 30 on the quotient is below f32's grid at 1
 template <bool CAP>
-__device__ __forceinline__ float lp_value(const LpArgs& A, float l, float ref2) {
-    if (!CAP) return fmaf(l, kLog2e, -ref2);
-    return fmaf(-2.f * A.cap2, rcp(1.f + ex2(min_nan(l * A.cap_k, 30.f))), A.cap2 - ref2);
+__device__ __forceinline__ float lp_value(const LpArgs& A, float l, float ref) {
+    if (!CAP) return (l - ref) * kLog2e;
+    return fmaf(-2.f * A.cap2, rcp(1.f + ex2(min_nan(l * A.cap_k, 30.f))), A.cap2 - ref);
 }
+// x - ref in units of 1
+template <bool CAP>
+__device__ __forceinline__ float lp_above(const LpArgs& A, float l, float ref) {
+    return CAP ? kLn2 * lp_value<CAP>(A, l, ref) : l - ref;
+}
+// how far one reference lies above another one, in units of log 2: at least -1000, whose weight is 0 (products with -inf would be NaN)
+template <bool CAP>
+__device__ __forceinline__ float lp_step(float from, float to) { return fmaxf(CAP ? from - to : (from - to) * kLog2e, -1000.f); }
 // four at once: one reciprocal (of the product, at most 2^120) for four, because the special function unit bounds this kernel
 template <bool CAP>
-__device__ __forceinline__ void lp_values(const LpArgs& A, const float* l, float ref2, float* d) {
+__device__ __forceinline__ void lp_values(const LpArgs& A, const float* l, float ref, float* d) {
     if constexpr (!CAP) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) d[i] = fmaf(l[i], kLog2e, -ref2);
+        for (int i = 0; i < 4; i++) d[i] = (l[i] - ref) * kLog2e;
     } else {
         float a[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) a[i] = 1.f + ex2(min_nan(l[i] * A.cap_k, 30.f));
-        const float ab = a[0] * a[1], cd = a[2] * a[3], r = rcp(ab * cd) * (-2.f * A.cap2), r0 = r * cd, r1 = r * ab, at = A.cap2 - ref2;
+        const float ab = a[0] * a[1], cd = a[2] * a[3], r = rcp(ab * cd) * (-2.f * A.cap2), r0 = r * cd, r1 = r * ab, at = A.cap2 - ref;
         d[0] = fmaf(r0, a[1], at);
         d[1] = fmaf(r0, a[0], at);
         d[2] = fmaf(r1, a[3], at);
@@ -108,13 +117,14 @@ __device__ __forceinline__ float lp_from_order(unsigned o) {
 }
 __device__ __forceinline__ unsigned long long lp_key(float l, int64_t i) { return ((unsigned long long)lp_order(l) << 32) | (unsigned)~(unsigned)i; }
 
-// running statistics in units of log 2; m = -inf: no value above -inf yet (s1 is then 0, or NaN)
+// running statistics; m = -inf: no value above -inf yet (s1 is then 0, or NaN)
 struct LpStats {
-    float m, s1, s2;   // reference, sum 2^(x - m), sum 2^(x - m) (x - m)
+    float m, s1, s2;   // reference, and with x in units of log 2 relative to it sum 2^x, sum 2^x x
 };
+template <bool CAP>
 __device__ __forceinline__ LpStats lp_merge(LpStats a, LpStats b) {
     const float m = fmaxf(a.m, b.m);
-    const float da = a.m == -INFINITY ? 0.f : a.m - m, db = b.m == -INFINITY ? 0.f : b.m - m;
+    const float da = a.m == -INFINITY ? 0.f : lp_step<CAP>(a.m, m), db = b.m == -INFINITY ? 0.f : lp_step<CAP>(b.m, m);
     const float wa = ex2(da), wb = ex2(db);
     LpStats r;
     r.m = m;
@@ -184,8 +194,8 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) k_logprobs(LpArgs A, in
     const int units = (n - head) / V, rest = n - units * V;   // rest: head and tail
     const int ub = (int)((int64_t)units * z / splits), ue = (int)((int64_t)units * (z + 1) / splits);
     const uint4* body = reinterpret_cast<const uint4*>(x + head);
-    // the thread's statistics: relative to ref2, which is the value of the largest logit so far (0 before there is one)
-    float raw_max = -INFINITY, ref2 = 0.f;
+    // the thread's statistics: relative to ref, the largest logit so far or its capped value (0 before there is one)
+    float raw_max = -INFINITY, ref = 0.f;
     float s1[2] = {0.f, 0.f}, s2[2] = {0.f, 0.f};   // two chains of additions
     if (t == 0) {
         count = 0;
@@ -196,9 +206,9 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) k_logprobs(LpArgs A, in
 
     auto raise = [&](float top) {
         if (!(top > raw_max)) return;
-        const float m = lp_value<CAP>(A, top, 0.f);
+        const float m = CAP ? lp_value<CAP>(A, top, 0.f) : top;
         if (raw_max != -INFINITY) {
-            const float d = ref2 - m, w = ex2(d);
+            const float d = lp_step<CAP>(ref, m), w = ex2(d);
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 s2[c] = w * fmaf(d, s1[c], s2[c]);
@@ -206,11 +216,11 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) k_logprobs(LpArgs A, in
             }
         }
         raw_max = top;
-        ref2 = m;
+        ref = m;
     };
     auto add = [&](const float* l) {   // four values
         float d[4];
-        lp_values<CAP>(A, l, ref2, d);
+        lp_values<CAP>(A, l, ref, d);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const float e = ex2(d[i]);
@@ -251,7 +261,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) k_logprobs(LpArgs A, in
         const int i = t < head ? t : units * V + t;
         const float l = lp_load(x + i);
         raise(l);
-        float d = lp_value<CAP>(A, l, ref2);
+        float d = lp_value<CAP>(A, l, ref);
         const float e = ex2(d);
         s1[0] = e;
         s2[0] = e * fmaxf(d, -1e30f);
@@ -289,7 +299,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) k_logprobs(LpArgs A, in
     {
         s.s1 = s1[0] + s1[1];
         s.s2 = s2[0] + s2[1];
-        s.m = raw_max == -INFINITY ? -INFINITY : ref2;
+        s.m = raw_max == -INFINITY ? -INFINITY : ref;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -297,7 +307,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) k_logprobs(LpArgs A, in
         b.m = __shfl_xor_sync(0xffffffffu, s.m, o);
         b.s1 = __shfl_xor_sync(0xffffffffu, s.s1, o);
         b.s2 = __shfl_xor_sync(0xffffffffu, s.s2, o);
-        s = lp_merge(s, b);
+        s = lp_merge<CAP>(s, b);
     }
     if (lane == 0) warp_stats[warp] = s;
     if (A.top) {
@@ -429,7 +439,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) k_logprobs(LpArgs A, in
     }
     if (t == 0) {
         s = warp_stats[0];
-        for (int w = 1; w < NT / 32; w++) s = lp_merge(s, warp_stats[w]);
+        for (int w = 1; w < NT / 32; w++) s = lp_merge<CAP>(s, warp_stats[w]);
         block_stats = s;
     }
     if (splits > 1) cluster_sync_all();
@@ -443,7 +453,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) k_logprobs(LpArgs A, in
                 asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(b.m) : "r"(a) : "memory");
                 asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(b.s1) : "r"(a + 4u) : "memory");
                 asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(b.s2) : "r"(a + 8u) : "memory");
-                s = lp_merge(s, b);
+                s = lp_merge<CAP>(s, b);
             }
             // a row without a value above -inf, and one with NaN or +inf, has no distribution
             const float log_s = s.s1 > 0.f ? log2f(s.s1) : NAN;
@@ -453,7 +463,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) k_logprobs(LpArgs A, in
                 const int tok = A.tokens[row];
                 float lp = 0.f;   // LEV_NO_TOKEN
                 if (tok >= 0 && tok < A.n) {
-                    lp = kLn2 * (lp_value<CAP>(A, lp_load(x + tok), s.m) - log_s);
+                    lp = lp_above<CAP>(A, lp_load(x + tok), s.m) - kLn2 * log_s;
                 } else if (tok != LEV_NO_TOKEN) {
                     atomicOr(A.status, LEV_DEV_BAD_INDEX);
                     lp = NAN;
@@ -479,7 +489,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) k_logprobs(LpArgs A, in
                 const unsigned long long k = cand[i];
                 const float l = lp_from_order((unsigned)(k >> 32));
                 A.top_index[row * A.top + i] = (int32_t)~(unsigned)k;
-                A.top_logprob[row * A.top + i] = kLn2 * (lp_value<CAP>(A, l, lse_s[0]) - lse_s[1]);
+                A.top_logprob[row * A.top + i] = lp_above<CAP>(A, l, lse_s[0]) - kLn2 * lse_s[1];
             }
         }
     }

@@ -308,9 +308,9 @@ int lev_softcap(lev_ctx* ctx, float* x, int64_t n, float cap);
  *   entropy[r] = -sum p log p   (NULL: left out)
  *   top_index, top_logprob [rows][top]: the `top` (0 ... LEV_MAX_TOP_K) largest logits, largest first, ties to the lowest index
  *     (-0 ties with 0, NaN comes last), with their log probabilities
- * The capped value is off by up to cap * 2^-21.  Logits of -inf have probability 0 (with a cap: that of -cap).  A row with NaN or +inf, or with nothing above -inf, has no
- * distribution: its log probabilities and entropy are NaN, its top_index is still in order.  No work buffers; repeat runs give
- * the same bits. */
+ * The capped value is off by up to cap * 2^-21.  Without a cap logits of -inf have probability 0, and a row with +inf or with nothing
+ * above -inf has no distribution; with one infinities count as -cap and cap.  A row with NaN has no distribution.  Where there is none the
+ * log probabilities and the entropy are NaN and top_index is still in order.  No work buffers; repeat runs give the same bits. */
 #define LEV_NO_TOKEN (-1)
 int lev_logprobs(lev_ctx* ctx, const void* logits, int type, int64_t rows, int64_t n, int64_t ld,
                  float cap, const int32_t* tokens, int top, float* logprob, float* entropy,

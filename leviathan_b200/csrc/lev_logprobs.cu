@@ -117,7 +117,8 @@ __device__ __forceinline__ float lp_from_order(unsigned o) {
 }
 __device__ __forceinline__ unsigned long long lp_key(float l, int64_t i) { return ((unsigned long long)lp_order(l) << 32) | (unsigned)~(unsigned)i; }
 
-// running statistics; m = -inf: no value above -inf yet (s1 is then 0, or NaN)
+// running statistics; without a cap m = -inf: no value above -inf yet (s1 is then 0, or NaN).  With one the value of -inf is -cap, whose
+// weight counts like any other, and m is never below that.
 struct LpStats {
     float m, s1, s2;   // reference, and with x in units of log 2 relative to it sum 2^x, sum 2^x x
 };
@@ -194,8 +195,8 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) k_logprobs(LpArgs A, in
     const int units = (n - head) / V, rest = n - units * V;   // rest: head and tail
     const int ub = (int)((int64_t)units * z / splits), ue = (int)((int64_t)units * (z + 1) / splits);
     const uint4* body = reinterpret_cast<const uint4*>(x + head);
-    // the thread's statistics: relative to ref, the largest logit so far or its capped value (0 before there is one)
-    float raw_max = -INFINITY, ref = 0.f;
+    // the thread's statistics: relative to ref, the largest logit so far or its capped value (before there is one 0, or that of -inf)
+    float raw_max = -INFINITY, ref = CAP ? -A.cap2 : 0.f;
     float s1[2] = {0.f, 0.f}, s2[2] = {0.f, 0.f};   // two chains of additions
     if (t == 0) {
         count = 0;
@@ -207,7 +208,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) k_logprobs(LpArgs A, in
     auto raise = [&](float top) {
         if (!(top > raw_max)) return;
         const float m = CAP ? lp_value<CAP>(A, top, 0.f) : top;
-        if (raw_max != -INFINITY) {
+        if (CAP || raw_max != -INFINITY) {
             const float d = lp_step<CAP>(ref, m), w = ex2(d);
 #pragma unroll
             for (int c = 0; c < 2; c++) {
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) k_logprobs(LpArgs A, in
     {
         s.s1 = s1[0] + s1[1];
         s.s2 = s2[0] + s2[1];
-        s.m = raw_max == -INFINITY ? -INFINITY : ref;
+        s.m = !CAP && raw_max == -INFINITY ? -INFINITY : ref;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -455,7 +456,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) k_logprobs(LpArgs A, in
                 asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(b.s2) : "r"(a + 8u) : "memory");
                 s = lp_merge<CAP>(s, b);
             }
-            // a row without a value above -inf, and one with NaN or +inf, has no distribution
+            // a row with NaN has no distribution; without a cap one with +inf or without a value above -inf neither
             const float log_s = s.s1 > 0.f ? log2f(s.s1) : NAN;
             lse_s[0] = s.m;
             lse_s[1] = log_s;

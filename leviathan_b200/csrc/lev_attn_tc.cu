@@ -662,7 +662,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                     f32x2 e;
                     both(fma_2(two(__uint_as_float(s[64 * h + 2 * c]), __uint_as_float(s[64 * h + 2 * c + 1])), sl2, neg2), a, b);
                     if (c % 4 == 1) {   // a quarter on the multiply-add units
-                        both(exp2_cubic(two(max_nan(a, -126.f), max_nan(b, -126.f))), a, b);
+                        both(exp2_cubic(two(max_nan(a, -127.f), max_nan(b, -127.f))), a, b);
                     } else {
                         a = ex2(a);
                         b = ex2(b);

@@ -46,18 +46,18 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;\n" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
-// 2^x for -126 <= x <= 127 on the multiply-add units, for part of the weights where the special function unit (a quarter of their
+// 2^x for -127 <= x <= 127 on the multiply-add units, for part of the weights where the special function unit (a quarter of their
 // rate) bounds a kernel: x = n + f with |f| <= 1/2 by adding and subtracting 1.5 * 2^23, a cubic in f of least maximal relative
-// error (Remez's exchange: 7.5e-5, an eighth of f16's half step), and n added to its exponent.  NaN gives a huge number.
+// error (Remez's exchange: 7.5e-5, about a sixth of f16's half step), times 2^n from n's bits.  The product is 0 at n = -127, what callers
+// clamp lower values to: a weight of 0 is 0, not a least number that bf16 could still represent.  NaN stays NaN.
 __device__ __forceinline__ f32x2 exp2_cubic(f32x2 x) {
     const f32x2 r = add_2(x, twice(12582912.f)), f = fma_2(add_2(r, twice(-12582912.f)), twice(-1.f), x);
     f32x2 p = fma_2(f, twice(0.0551716685295105f), twice(0.2426111251115799f));
     p = fma_2(f, p, twice(0.6932609677314758f));
     p = fma_2(f, p, twice(0.9999280571937561f));
-    float a, b, ra, rb;
-    both(p, a, b);
+    float ra, rb;
     both(r, ra, rb);
-    return two(__uint_as_float(__float_as_uint(a) + (__float_as_uint(ra) << 23)), __uint_as_float(__float_as_uint(b) + (__float_as_uint(rb) << 23)));
+    return mul_2(p, two(__uint_as_float(0x3F800000u + (__float_as_uint(ra) << 23)), __uint_as_float(0x3F800000u + (__float_as_uint(rb) << 23))));
 }
 __device__ __forceinline__ float max_nan(float a, float b) {   // NaN if one is NaN
     float y;

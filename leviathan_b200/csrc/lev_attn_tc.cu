@@ -50,6 +50,7 @@ constexpr int TC_MAX_SPLITS = 8;           // CTAs of a cluster that share a uni
 constexpr unsigned TC_STAGE = 32768;       // 128 rows x 128 columns of 16 bits: two slabs of 64 columns
 constexpr int TC_MAX_STAGES = 6;
 constexpr float TC_LAZY = 8.0f;            // how far (log2) the maximum may run ahead of a row's reference
+constexpr float TC_EXACT = 1024.0f;        // references above this (in units of log 2) are subtracted before the scaling
 enum { TC_F32 = LEV_ELEM_F32, TC_F16 = LEV_ELEM_F16, TC_BF16 = LEV_ELEM_BF16 };
 
 struct TcArgs {
@@ -650,7 +651,15 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                         : "memory");
                 }
             }
-            const float neg = m == -INFINITY ? 0.f : -m * A.sl;
+            float neg = m == -INFINITY ? 0.f : -m * A.sl;
+            // One fused operation per pair of scores has the rounding of `neg` in every weight: 2^-14 at this bound, out of all range from
+            // 2^31 on.  Rows beyond it take the difference first, which no other row pays for.
+            if (__any_sync(0xffffffffu, fabsf(neg) > TC_EXACT)) {
+                const float sub = fabsf(neg) > TC_EXACT ? m : 0.f;
+                neg = fabsf(neg) > TC_EXACT ? 0.f : neg;
+#pragma unroll
+                for (int c = 0; c < 128; c++) s[c] = __float_as_uint(__uint_as_float(s[c]) - sub);
+            }
             const f32x2 neg2 = two(neg, neg);
             f32x2 part = two(0.f, 0.f);
 #pragma unroll
@@ -1368,7 +1377,8 @@ TcArgs tc_args(lev_ctx* ctx, int n_seqs, const int32_t* start, int64_t n_rows, i
     A.tpt = 128 / A.group;
     A.window = window;
     A.negate = scale < 0.f;   // maxima are taken of S: a negative scale goes into the queries
-    A.sl = (scale == 0.f ? 1e-30f : fabsf(scale)) * 1.4426950408889634f;   // a scale of zero: the same weights, and a replaced score stays -inf
+    // a scale of zero: the same weights for all finite scores, and a replaced score stays -inf
+    A.sl = scale == 0.f ? 1e-45f : fabsf(scale) * 1.4426950408889634f;
     A.status = ctx->d_status;
     return A;
 }

@@ -496,7 +496,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
     constexpr int O_COL = 256;                          // tensor memory: S slots at 0 and 128, then O
     extern __shared__ unsigned char smem_dyn[];
     __shared__ __align__(8) unsigned long long full[NS], empty[NS], s_full[2], p_full[2], pv_done[2], q_first, q_full, q_empty, v_last, v_clean;
-    __shared__ __align__(8) unsigned long long unit_full[2], unit_empty[2], answer_bar, told_bar[2];
+    __shared__ __align__(8) unsigned long long unit_full[2], unit_empty[2], known[2], answer_bar, told_bar[2];
     __shared__ __align__(16) unsigned answer_s[4];
     __shared__ unsigned tmem_base_s;
     __shared__ int abort_s, bad_s[2], told_s[2];
@@ -524,6 +524,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
             mbar_init(smem_u32(&pv_done[s]), 1);
             mbar_init(smem_u32(&unit_full[s]), 1);
             mbar_init(smem_u32(&unit_empty[s]), 4 * TILES + TC_LOAD_WARPS);   // softmax and MMA warps, the other loading warps
+            mbar_init(smem_u32(&known[s]), 1);
             mbar_init(smem_u32(&told_bar[s]), 1);
         }
         mbar_init(smem_u32(&q_full), A.q_boxes ? 1 : TC_LOAD_WARPS * CG);
@@ -703,6 +704,9 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         both(sum, l0, l1);
         float l = l0 + l1;
         const volatile TcUnit& V = unit_s[k & 1];   // (not held in registers over the steps)
+        // This CTA's loading warp has read the unit's part of the table long ago; its arrival is what makes bad_s visible.
+        tc_wait(smem_u32(&known[k & 1]), (k >> 1) & 1, abort_flag);
+        __syncwarp();
         const bool ok = V.ok, bad = !ok || bad_s[k & 1] == k + 1;   // an index outside the layout: the rows are NaN
         const bool live = tok < A.tpt && tile_tok + tok < V.tokens;
         const int kvh = V.kvh, row_first = V.row0 + V.t0;
@@ -1134,6 +1138,8 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 e_before = e_now;
                 e_now = e_next;
             }
+            // (each warp goes over all entries of this CTA's steps, and `entries` ends in a warp barrier)
+            if (w == 0 && lane == 0) mbar_arrive(smem_u32(&known[k & 1]));
             if (COPY && under_way) {
                 asm volatile("cp.async.wait_group 0;\n" ::: "memory");
                 while (under_way) hand_over();

@@ -20,7 +20,7 @@
 // Roles of a CTA: one (two) softmax warpgroup(s), one warp that issues MMAs, three that request TMA boxes or, where the cache cannot be
 // boxed (f32 pools, pages that are no whole groups of eight rows), copy rows.  A CTA keeps its tensor memory and barriers from unit to
 // unit: the hardware hands it the next one of the grid, longest first (24 sequences of mixed lengths: 207 us with a CTA per unit, 176 so).
-// Every wait is bounded (about 16 seconds, then LEV_TIMEOUT).
+// Every wait is bounded (a second in which nothing moves, then LEV_TIMEOUT).
 //
 // Places that a row does not attend to may hold anything, NaN included.  Scores there are replaced, but 0 * NaN is NaN in the product
 // with V.  Behind the last position of a unit V becomes zeros in shared memory (100 tokens of 8 sequences with NaN in the unfilled part
@@ -100,10 +100,31 @@ __device__ __forceinline__ void swap_pieces(uint4& a, uint4& b, int bit, int lan
     if (up) a = got;
     else b = got;
 }
-// Bounded, with patience: a tile whose rows meet NaN among the values they attend to goes over its positions again row by row (30 us
-// for each of them and 128 positions: a second at 33000 positions), and everybody else waits.
-__device__ __forceinline__ bool tc_wait(unsigned bar, unsigned parity, volatile int* abort_flag) {
-    return pk_try(bar, parity) || pk_wait_slow<16>(bar, parity, abort_flag);
+// Flags of a CTA: whether a wait ran out, and how far tc_row_again has come in this CTA and in the pair's other one.
+enum { TC_ABORT, TC_MOVES, TC_MOVES_OTHER, TC_FLAGS };
+// Bounded: about a second in which tc_row_again does not move either.  A tile whose rows meet NaN among the values they attend to goes over
+// its positions again row by row (60 to 110 us for each of them and 128 positions: a second at 10000 positions), and others wait.
+__device__ __noinline__ bool tc_wait_slow(unsigned bar, unsigned parity, volatile int* flags) {
+    long long t_start = 0;
+    int moves = 0;
+    for (unsigned i = 1;; i++) {
+        if (pk_try_suspended(bar, parity)) return true;
+        if ((i & 15u) == 0) {
+            if (flags[TC_ABORT]) return false;
+            const long long now = clock64();
+            const int moved = flags[TC_MOVES] + flags[TC_MOVES_OTHER];
+            if (t_start == 0 || moved != moves) {
+                t_start = now;
+                moves = moved;
+            } else if (now - t_start > kWaitCycles) {
+                flags[TC_ABORT] = 1;
+                return false;
+            }
+        }
+    }
+}
+__device__ __forceinline__ bool tc_wait(unsigned bar, unsigned parity, volatile int* flags) {
+    return pk_try(bar, parity) || tc_wait_slow(bar, parity, flags);
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
@@ -332,15 +353,21 @@ __device__ __forceinline__ void tc_store16(const TcArgs& A, int64_t at, float x)
 }
 
 // One row again, position by position over [lo, hi): for rows whose sums met a non-finite value where they do not attend.
-// 128 threads of the tile's warpgroup; ws: 128 floats.  Returns thread t's dims t (and t + 128) unnormalised.
+// 128 threads of the tile's warpgroup; ws: 128 floats.  Returns thread t's dims t (and t + 128) unnormalised.  `other`: cluster address of
+// the pair's other CTA's TC_MOVES_OTHER, or 0; who waits meanwhile is told of every 128 positions.
 template <int HD>
-__device__ void tc_row_again(const TcArgs& A, const TcUnit& U, int64_t q_at, int lo, int hi, int t, int bar, float* ws, float* o, float* m_out,
-                             float* l_out) {
+__device__ void tc_row_again(const TcArgs& A, const TcUnit& U, int64_t q_at, int lo, int hi, int t, int bar, float* ws, volatile int* flags, unsigned other, float* o,
+                             float* m_out, float* l_out) {
     float m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int i = 0; i < HD / 128; i++) o[i] = 0.f;
     for (int b = lo; b < hi; b += 128) {
         wg_sync(bar);   // the weights of the step before are read
+        if (t == 0) {
+            const int moves = flags[TC_MOVES] + 1;
+            flags[TC_MOVES] = moves;   // (of two tiles at once one may get lost)
+            if (other) asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(other), "r"(moves) : "memory");
+        }
         float s = -INFINITY;
         if (b + t < hi) {
             const unsigned char* row = tc_row(A, U, HD, b + t, false);
@@ -499,7 +526,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
     __shared__ __align__(8) unsigned long long unit_full[2], unit_empty[2], known[2], answer_bar, told_bar[2];
     __shared__ __align__(16) unsigned answer_s[4];
     __shared__ unsigned tmem_base_s;
-    __shared__ int abort_s, bad_s[2], told_s[2];
+    __shared__ int flags_s[TC_FLAGS], bad_s[2], told_s[2];
     __shared__ TcUnit unit_s[2];
     __shared__ unsigned again_s[TILES * 4];
     __shared__ float again_w[TILES][128];
@@ -512,7 +539,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
     const unsigned smem = (smem_u32(smem_dyn) + 1023u) & ~1023u;
     const unsigned ring = smem + TILES * D::kQTile;
     if (threadIdx.x == 0) {
-        abort_s = 0;
+        flags_s[TC_ABORT] = flags_s[TC_MOVES] = flags_s[TC_MOVES_OTHER] = 0;
         bad_s[0] = bad_s[1] = 0;
         for (int s = 0; s < NS; s++) {
             mbar_init(smem_u32(&full[s]), tc_full_count(COPY, CG));   // every warp that waits for `empty` (lev_attn_ring.h)
@@ -556,17 +583,17 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
     if (CG == 2) cluster_sync_all();
     tc_after();
     const unsigned tmem = tmem_base_s;
-    volatile int* abort_flag = &abort_s;
+    volatile int* flags = flags_s;
     // Unit k (from 0) of this CTA is in unit_s[k & 1].  Ends unit k and goes on to the next one; false: there is none.
     auto next_unit = [&](int k) {
         if (SPLIT) return false;   // a cluster that merges has one unit
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&unit_empty[k & 1]));
         k++;
-        tc_wait(smem_u32(&unit_full[k & 1]), ((k - 1) >> 1) & 1, abort_flag);
+        tc_wait(smem_u32(&unit_full[k & 1]), ((k - 1) >> 1) & 1, flags);
         __syncwarp();
         U = unit_s[k & 1];
-        return U.tokens > 0 && !*abort_flag;
+        return U.tokens > 0 && !*flags;
     };
     // Splits: the CTA of split z adds up rows z * share ... of a tile.  Every CTA stores its partial sums of a row, reference and sum of
     // weights straight into that CTA's shared memory, [tile][part][row of the share][HD] where the queries and stages were, when all
@@ -605,7 +632,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         for (int i = 0; i < n; i++, g++) {
             const int slot_i = TILES == 2 ? tile : g & 1, par = TILES == 2 ? g & 1 : (g >> 1) & 1;
             const unsigned s_addr = lane_base + (unsigned)slot_i * 128u;
-            tc_wait(smem_u32(&s_full[slot_i]), par, abort_flag);
+            tc_wait(smem_u32(&s_full[slot_i]), par, flags);
             __syncwarp();
             tc_after();
             unsigned s[128];
@@ -633,7 +660,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
             }
             if (i > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
                 const int prev = TILES == 2 ? tile : (g - 1) & 1, ppar = TILES == 2 ? (g - 1) & 1 : ((g - 1) >> 1) & 1;
-                tc_wait(smem_u32(&pv_done[prev]), ppar, abort_flag);
+                tc_wait(smem_u32(&pv_done[prev]), ppar, flags);
                 __syncwarp();
                 tc_after();
                 sum = fma_2(sum, two(corr, corr), two(0.f, 0.f));
@@ -696,7 +723,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         }
         if (n > 0) {
             const int last = TILES == 2 ? tile : (g - 1) & 1, lpar = TILES == 2 ? (g - 1) & 1 : ((g - 1) >> 1) & 1;
-            tc_wait(smem_u32(&pv_done[last]), lpar, abort_flag);
+            tc_wait(smem_u32(&pv_done[last]), lpar, flags);
             __syncwarp();
             tc_after();
         }
@@ -705,7 +732,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         float l = l0 + l1;
         const volatile TcUnit& V = unit_s[k & 1];   // (not held in registers over the steps)
         // This CTA's loading warp has read the unit's part of the table long ago; its arrival is what makes bad_s visible.
-        tc_wait(smem_u32(&known[k & 1]), (k >> 1) & 1, abort_flag);
+        tc_wait(smem_u32(&known[k & 1]), (k >> 1) & 1, flags);
         __syncwarp();
         const bool ok = V.ok, bad = !ok || bad_s[k & 1] == k + 1;   // an index outside the layout: the rows are NaN
         const bool live = tok < A.tpt && tile_tok + tok < V.tokens;
@@ -797,7 +824,8 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 lo = lo > jb * TC_KV ? lo : jb * TC_KV;
                 hi = hi < je * TC_KV ? hi : je * TC_KV;
                 float o[HD / 128], m2, l2;
-                tc_row_again<HD>(A, W, row * A.q_ld + rh * HD, lo, hi, t, 1 + tile, again_w[tile], o, &m2, &l2);
+                tc_row_again<HD>(A, W, row * A.q_ld + rh * HD, lo, hi, t, 1 + tile, again_w[tile], flags,
+                                 CG == 2 ? map_to_rank(smem_u32(&flags_s[TC_MOVES_OTHER]), lead + (rank ^ 1u)) : 0u, o, &m2, &l2);
 #pragma unroll
                 for (int q = 0; q < HD / 128; q++) {
                     const int d = t + 128 * q;
@@ -851,7 +879,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 Ring st = kr;
 #pragma unroll
                 for (int h = 0; h < KV_STAGES; h++) {
-                    tc_wait(smem_u32(&full[st.s]), st.ph, abort_flag);
+                    tc_wait(smem_u32(&full[st.s]), st.ph, flags);
                     tc_after();
                     const unsigned kb = ring + (unsigned)st.s * TC_STAGE;
                     constexpr int kSlabs = HD / 64 / KV_STAGES;
@@ -868,7 +896,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 Ring st = vr;
 #pragma unroll
                 for (int h = 0; h < KV_STAGES; h++) {
-                    tc_wait(smem_u32(&full[st.s]), st.ph, abort_flag);
+                    tc_wait(smem_u32(&full[st.s]), st.ph, flags);
                     tc_after();
                     const unsigned vb = ring + (unsigned)st.s * TC_STAGE;
                     const unsigned b_lo = ((vb >> 4) & 0x3FFFu) | ((vl.slab >> 4) << 16);
@@ -886,17 +914,17 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                     if (!dirty) return;
                     Ring at = vr;
                     for (int h = 0; h < KV_STAGES; h++) {
-                        tc_wait(smem_u32(&full[at.s]), at.ph, abort_flag);
+                        tc_wait(smem_u32(&full[at.s]), at.ph, flags);
                         at.step(1);
                     }
                     __syncwarp();
                     if (CG == 2 && lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&v_last), lead + 1));
                     zeros(g + 1, used);
-                    if (CG == 2) tc_wait(smem_u32(&v_clean), tails++ & 1, abort_flag);
+                    if (CG == 2) tc_wait(smem_u32(&v_clean), tails++ & 1, flags);
                 };
-                if (A.q_boxes) tc_wait(smem_u32(&q_full), k & 1, abort_flag);
-                else if (k == 0) tc_wait(smem_u32(&q_first), 0, abort_flag);
-                else tc_wait(smem_u32(&q_full), (k - 1) & 1, abort_flag);
+                if (A.q_boxes) tc_wait(smem_u32(&q_full), k & 1, flags);
+                else if (k == 0) tc_wait(smem_u32(&q_first), 0, flags);
+                else tc_wait(smem_u32(&q_full), (k - 1) & 1, flags);
                 tc_after();
                 if (TILES == 2) {
                     // stages: K0 V0 K1 V1 ...
@@ -912,7 +940,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
 #pragma unroll
                         for (int tile = 0; tile < 2; tile++) {
                             if (tile == 0 && i == n - 1) tail();
-                            tc_wait(smem_u32(&p_full[tile]), g & 1, abort_flag);
+                            tc_wait(smem_u32(&p_full[tile]), g & 1, flags);
                             tc_after();
                             pv(tile, tile, i == 0, tile == 1, i == n - 1 ? (used + 15) >> 4 : 8);
                             if (i + 1 < n) qk(tile, tile, tile == 1);
@@ -939,7 +967,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                         }
                         vr = st;
                         if (i == n - 1) tail();
-                        tc_wait(smem_u32(&p_full[g & 1]), (g >> 1) & 1, abort_flag);
+                        tc_wait(smem_u32(&p_full[g & 1]), (g >> 1) & 1, flags);
                         tc_after();
                         pv(0, g & 1, i == 0, true, i == n - 1 ? (used + 15) >> 4 : 8);
                         st.step(KV_STAGES);
@@ -952,7 +980,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 const int n = U.n, used = n > 0 ? U.last_used() : 0, dirty = used & 15 && cleaned(U) ? used : 0;
                 g += n;
                 if (dirty) {
-                    tc_wait(smem_u32(&v_last), tails++ & 1, abort_flag);
+                    tc_wait(smem_u32(&v_last), tails++ & 1, flags);
                     zeros(g, used);
                     if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&v_clean), lead));
                 }
@@ -1014,7 +1042,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 const unsigned row_bytes = (is_v ? kSlabsV : kSlabsK) * 128u;
 #pragma unroll
                 for (int h = 0; h < KV_STAGES; h++) {
-                    tc_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
+                    tc_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, flags);
                     const unsigned bar = full_c + 8u * (unsigned)st.s, dst = ring + (unsigned)st.s * TC_STAGE;
                     if (rank == 0 && w == 0) pk_expect(smem_u32(&full[st.s]), TC_STAGE * CG, elected);
                     const int x0 = CG == 2 ? (is_v ? (int)rank * 128 : 0) : h * 128;
@@ -1049,7 +1077,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 const int piece = lane & 15, sub = lane >> 4;   // two rows of 16 pieces (8 values each) per step of a warp
                 const char* pool = static_cast<const char*>(is_v ? A.v : A.k);
                 for (int h = 0; h < KV_STAGES; h++) {
-                    tc_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
+                    tc_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, flags);
                     const unsigned dst = ring + (unsigned)st.s * TC_STAGE + (unsigned)(piece >> 3) * 16384u;
                     auto row = [&](int r, int64_t* off) {
                         const int64_t v = (r >> 5) == 0 ? R.off[0] : (r >> 5) == 1 ? R.off[1] : (r >> 5) == 2 ? R.off[2] : R.off[3];
@@ -1111,7 +1139,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                 if (i == 0) {
                     // This unit's queries, when the last product that read the ones before is done.  The first K tile has been asked
                     // for: waiting any later could wait for a stage that only these queries would free.
-                    if (k > 0 && tc_waits_for_queries(A.q_boxes, w)) tc_wait(smem_u32(&q_empty), (k - 1) & 1, abort_flag);
+                    if (k > 0 && tc_waits_for_queries(A.q_boxes, w)) tc_wait(smem_u32(&q_empty), (k - 1) & 1, flags);
                     __syncwarp();
                     if (A.q_boxes) {   // one box of 64 columns: the group's heads of a tile's tokens
                         if (w == 0) {
@@ -1149,8 +1177,8 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
             if (w == 0) {
                 int x;
                 if (rank == 0) {
-                    tc_wait(smem_u32(&answer_bar), k & 1, abort_flag);
-                    x = *abort_flag ? -1 : tc_next_taken(smem_u32(answer_s));
+                    tc_wait(smem_u32(&answer_bar), k & 1, flags);
+                    x = *flags ? -1 : tc_next_taken(smem_u32(answer_s));
                     __syncwarp();
                     if (lane == 0) {
                         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");   // the answer has been read
@@ -1162,14 +1190,14 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                     }
                 } else {
                     if (lane == 0) mbar_expect(smem_u32(&told_bar[k & 1]), 4);
-                    tc_wait(smem_u32(&told_bar[k & 1]), (k >> 1) & 1, abort_flag);
+                    tc_wait(smem_u32(&told_bar[k & 1]), (k >> 1) & 1, flags);
                     __syncwarp();
-                    x = *abort_flag ? -1 : *(volatile int*)&told_s[k & 1];
+                    x = *flags ? -1 : *(volatile int*)&told_s[k & 1];
                 }
                 have = x >= 0 && tc_unit(A, x / cluster, per, split, lane, &U);
                 if (have && rank == 0 && lane == 0) tc_next_request(smem_u32(answer_s), smem_u32(&answer_bar));
                 // unit k + 1 goes where unit k - 1 was
-                if (k > 0) tc_wait(smem_u32(&unit_empty[(k + 1) & 1]), ((k - 1) >> 1) & 1, abort_flag);
+                if (k > 0) tc_wait(smem_u32(&unit_empty[(k + 1) & 1]), ((k - 1) >> 1) & 1, flags);
                 __syncwarp();
                 if (lane == 0) {
                     if (!have) U.tokens = 0;
@@ -1177,14 +1205,14 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
                     mbar_arrive(smem_u32(&unit_full[(k + 1) & 1]));
                 }
                 __syncwarp();
-                if (*abort_flag) have = false;
+                if (*flags) have = false;
             } else {
                 have = next_unit(k);
             }
         }
-        if (units && tc_waits_for_queries(A.q_boxes, w)) tc_wait(smem_u32(&q_empty), (units - 1) & 1, abort_flag);   // the tensor core's last releases have arrived
+        if (units && tc_waits_for_queries(A.q_boxes, w)) tc_wait(smem_u32(&q_empty), (units - 1) & 1, flags);   // the tensor core's last releases have arrived
         for (int s = 0; s < NS; s++) {
-            tc_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, abort_flag);
+            tc_wait(smem_u32(&empty[st.s]), st.ph ^ 1u, flags);
             st.step(1);
         }
     }
@@ -1193,7 +1221,7 @@ __global__ void __launch_bounds__(TcDims<HD, TILES>::kWarps * 32, 1)
         cluster_sync_all();   // the softmax warps' one
     }
     pdl_launch_dependents();   // what follows finds no room on an SM before (40 packed prompts: 73 us with the launch at the start, 71 here)
-    pk_finish(abort_flag, A.status, LEV_DEV_TIMEOUT);
+    pk_finish(flags, A.status, LEV_DEV_TIMEOUT);
     if constexpr (SPLIT) {
         // ---- the rows of this CTA's share: the parts in their order ----
         cluster_sync_all();   // all parts have arrived

@@ -43,8 +43,7 @@ __device__ __forceinline__ unsigned pk_try_suspended(unsigned bar, unsigned pari
         : "memory");
     return ok;
 }
-// bounded wait (about LIMIT seconds); false on timeout or when another thread of the CTA has already given up
-template <int LIMIT = 1>
+// bounded wait (about a second); false on timeout or when another thread of the CTA has already given up
 __device__ __noinline__ bool pk_wait_slow(unsigned bar, unsigned parity, volatile int* abort_flag) {
     long long t_start = 0;
     for (unsigned i = 1;; i++) {
@@ -53,7 +52,7 @@ __device__ __noinline__ bool pk_wait_slow(unsigned bar, unsigned parity, volatil
             if (*abort_flag) return false;
             const long long now = clock64();
             if (t_start == 0) t_start = now;
-            else if (now - t_start > LIMIT * kWaitCycles) {
+            else if (now - t_start > kWaitCycles) {
                 *abort_flag = 1;
                 return false;
             }
@@ -61,7 +60,7 @@ __device__ __noinline__ bool pk_wait_slow(unsigned bar, unsigned parity, volatil
     }
 }
 __device__ __forceinline__ bool pk_wait(unsigned bar, unsigned parity, volatile int* abort_flag) {
-    return pk_try(bar, parity) || pk_wait_slow<>(bar, parity, abort_flag);
+    return pk_try(bar, parity) || pk_wait_slow(bar, parity, abort_flag);
 }
 // A CTA's last steps after its roles.  A thread that knows of a wait that ran out lets copies in flight land; the status
 // is set behind the barrier, because the warp that gave up may be the last to get here.

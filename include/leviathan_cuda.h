@@ -269,7 +269,7 @@ enum { LEV_ELEM_F32 = 0, LEV_ELEM_F16 = 1, LEV_ELEM_BF16 = 2 };
  *   out = scale * (residual + alpha * gate * b)
  *   h = out * inv_rms(out) * pre  (h NULL: left out; pre NULL: no scale), h of type h_type
  * x, residual, out f32 [rows][n], any n.  gate f32 (NULL: 1): one row for all (gate_ld 0) or rows gate_ld elements apart.
- * out may be x or residual; h overlaps nothing.  Fastest on 16-byte boundaries with n % 4 == 0, up to 8192 elements. */
+ * out may be x or residual; otherwise out and h overlap nothing.  Fastest on 16-byte boundaries with n % 4 == 0, up to 8192 elements. */
 int lev_norm_residual(lev_ctx* ctx, const float* x, const float* residual, int64_t rows, int64_t n,
                       int norm_post, const float* post, const float* gate, int64_t gate_ld,
                       float alpha, float scale, const float* pre, float eps, float* out, void* h,

@@ -367,8 +367,11 @@ extern "C" int lev_norm_residual(lev_ctx* ctx, const float* x, const float* resi
     const size_t gate_bytes = gate ? ((size_t)(gate_ld ? (rows - 1) * gate_ld : 0) + n) * 4 : 0;
     if ((out != x && overlap(out, bytes, x, bytes)) || (out != residual && overlap(out, bytes, residual, bytes)))
         return lev_fail(ctx, LEV_BAD_ARGUMENT, "the output overlaps an input without being it");
-    if ((gate && overlap(out, bytes, gate, gate_bytes)) || (h && (overlap(h, h_bytes, x, bytes) || overlap(h, h_bytes, residual, bytes) || overlap(h, h_bytes, out, bytes) ||
-                                                                  (gate && overlap(h, h_bytes, gate, gate_bytes)))))
+    auto meets = [&](const void* p, size_t size) {   // an output: other CTAs store rows while one still reads
+        return p && (overlap(out, bytes, p, size) || (h && overlap(h, h_bytes, p, size)));
+    };
+    if ((h && (overlap(h, h_bytes, x, bytes) || overlap(h, h_bytes, residual, bytes) || overlap(h, h_bytes, out, bytes))) || meets(gate, gate_bytes) ||
+        meets(post, (size_t)n * 4) || meets(pre, (size_t)n * 4))
         return lev_fail(ctx, LEV_BAD_ARGUMENT, "an output overlaps another argument");
     LEV_CUDA(ctx, cudaSetDevice(ctx->device));
     MixArgs A = {x, residual, post, gate, pre, gate_ld, alpha, scale, eps, out, h, (int)n, norm_post != 0, h_type, rows};

@@ -131,3 +131,16 @@ def test_captured_replayed_and_on_another_stream(ctx, rows, n):
         a, b = ctx.norm_residual(x, res, post=w1, pre=w2, dtype=torch.bfloat16)
     torch.cuda.synchronize()
     assert torch.equal(a, out) and torch.equal(b, h)
+
+
+@pytest.mark.parametrize("rows,n", [(4, 64), (300, 9000)])
+def test_outputs_over_a_weight_are_refused(ctx, rows, n):
+    """other thread blocks read the weights while rows are written"""
+    x, res = torch.randn(rows, n, device=DEV), torch.randn(rows, n, device=DEV)
+    flat = torch.zeros((rows + 1) * n, device=DEV)
+    out, w, after = flat[:rows * n].view(rows, n), flat[(rows - 1) * n:rows * n], flat[rows * n:]
+    for kw in (dict(out=out, post=w), dict(out=out, pre=w), dict(h=out, post=w), dict(h=out, pre=w), dict(out=out, gate=w), dict(h=out, gate=w)):
+        with pytest.raises(lev.LevError, match="overlaps"):
+            ctx.norm_residual(x, res, **kw)
+    ctx.norm_residual(x, res, post=after, pre=after, out=out)   # right behind it is another matter
+    ctx.synchronize()

@@ -428,7 +428,7 @@ int lev_qkv_norm_rope_append_split(lev_ctx* ctx, float* q, float* k, float* v, i
  *   [start[0], start[n_chunks]) are not written.  n_rows: rows that q and out hold.
  *   q f32 (rounded to f16: magnitudes above 65504 are not served) or f16, out f16 or bf16 (what lev_gemm_prefill reads);
  *   rows q_ld and out_ld elements apart (whole 16-byte steps, 16-byte aligned), heads contiguous: q may be the leading part of
- *   each row of a fused projection output.  out must not overlap q.  f32 caches are rounded to f16 in the same way.
+ *   each row of a fused projection output.  The spans of out and of q, pools and table must not meet.  f32 caches are rounded to f16 in the same way.
  *   head_dim 128 or 256; up to 16 query heads per KV head; any page size (multiples of 8 are fastest).
  * A slot or position outside the layout, or a table entry outside the pool, is not followed: rows of that chunk are NaN (of an entry, those
  * that attend to its page, and others of the chunk may be); start entries that are no range leave their chunk out; both are reported by

@@ -1428,6 +1428,12 @@ extern "C" int lev_attn_chunk(lev_ctx* ctx, const lev_kv_layout* L, const void* 
     if (out_type != LEV_ELEM_F16 && out_type != LEV_ELEM_BF16) return lev_fail(ctx, LEV_UNSUPPORTED, "output element type %d (f16 or bf16)", out_type);
     LEV_TRY(tc_check(ctx, n_chunks, n_rows, q_heads, L->kv_heads, L->head_dim, q, q_type, q_ld, out, out_ld, window, scale));
     if ((((uintptr_t)k_pool | (uintptr_t)v_pool) & 15) != 0) return lev_fail(ctx, LEV_BAD_ARGUMENT, "cache pools are not 16-byte aligned");
+    const int64_t block_bytes = (int64_t)L->page * L->kv_heads * L->head_dim * (L->kv_type == LEV_KV_F32 ? 4 : 2), most = ((int64_t)1 << 50) / block_bytes + 1;
+    const int64_t pool_bytes = (L->blocks < most ? L->blocks : most) * block_bytes;   // (no layout is large enough to overflow)
+    const int64_t out_bytes = ((n_rows - 1) * out_ld + (int64_t)q_heads * L->head_dim) * 2;
+    if (ranges_meet(k_pool, pool_bytes, out, out_bytes) || ranges_meet(v_pool, pool_bytes, out, out_bytes) ||
+        ranges_meet(block_table, (int64_t)L->slots * L->max_blocks * 4, out, out_bytes))
+        return lev_fail(ctx, LEV_BAD_ARGUMENT, "the output overlaps the cache or its block table");
     EncodeTiledFn enc = encode_tiled();
     if (!enc) return lev_fail(ctx, LEV_UNSUPPORTED, "cuTensorMapEncodeTiled is not available");
     LEV_CUDA(ctx, cudaSetDevice(ctx->device));

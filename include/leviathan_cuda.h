@@ -310,7 +310,7 @@ int lev_softcap(lev_ctx* ctx, float* x, int64_t n, float cap);
  *     (-0 ties with 0, NaN comes last), with their log probabilities
  * The capped value is off by up to cap * 2^-21.  Without a cap logits of -inf have probability 0, and a row with +inf or with nothing
  * above -inf has no distribution; with one infinities count as -cap and cap.  A row with NaN has no distribution.  Where there is none the
- * log probabilities and the entropy are NaN and top_index is still in order.  No work buffers; repeat runs give the same bits. */
+ * log probabilities and the entropy are NaN and top_index is still in order.  Outputs overlap nothing.  No work buffers; repeat runs give the same bits. */
 #define LEV_NO_TOKEN (-1)
 int lev_logprobs(lev_ctx* ctx, const void* logits, int type, int64_t rows, int64_t n, int64_t ld,
                  float cap, const int32_t* tokens, int top, float* logprob, float* entropy,

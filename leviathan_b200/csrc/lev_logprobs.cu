@@ -545,6 +545,17 @@ extern "C" int lev_logprobs(lev_ctx* ctx, const void* logits, int type, int64_t 
     const size_t size = type == LEV_ELEM_F32 ? 4 : 2;
     if ((uintptr_t)logits % size != 0) return lev_fail(ctx, LEV_BAD_ARGUMENT, "logits are not aligned to their type");
     if (!logprob && !entropy && top == 0) return lev_fail(ctx, LEV_BAD_ARGUMENT, "nothing is asked for");
+    // outputs are stored while other rows are still read
+    const struct {
+        const void* p;
+        int64_t size;
+    } spans[6] = {{logprob, rows * 4},  {entropy, rows * 4}, {top ? top_index : nullptr, rows * top * 4}, {top ? top_logprob : nullptr, rows * top * 4},
+                  {logits, ((rows - 1) * ld + n) * (int64_t)size}, {logprob ? tokens : nullptr, rows * 4}};
+    for (int i = 0; i < 4; i++)
+        for (int j = i + 1; j < 6; j++)
+            if (spans[i].p && spans[j].p && (const char*)spans[i].p < (const char*)spans[j].p + spans[j].size &&
+                (const char*)spans[j].p < (const char*)spans[i].p + spans[i].size)
+                return lev_fail(ctx, LEV_BAD_ARGUMENT, "an output overlaps another argument");
     LEV_CUDA(ctx, cudaSetDevice(ctx->device));
     LpArgs A = {};
     A.x = logits;

@@ -73,9 +73,9 @@ _F32_F16, _ANY16, _ANY = (L.ELEM_F32, L.ELEM_F16), (L.ELEM_F16, L.ELEM_BF16), (L
 def _head_rows(t, what: str):
     """[rows][heads][head_dim] with heads and dims contiguous, as the parts of a fused projection output lie: shape and row stride."""
     shape, stride = t.shape, t.stride()
-    if len(shape) != 3 or stride[2] != 1 or stride[1] != shape[2]:
+    if len(shape) != 3 or stride[2] != 1 or (stride[1] != shape[2] and shape[1] != 1):   # of one row or one head the stride means nothing
         raise ValueError(f"{what}: [rows][heads][head_dim] with contiguous heads is wanted, got shape {tuple(shape)}, strides {stride}")
-    return shape, stride[0]
+    return shape, stride[0] if shape[0] > 1 else shape[1] * shape[2]
 
 
 def _i32(t, n: int, what: str):

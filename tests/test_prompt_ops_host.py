@@ -91,3 +91,15 @@ def test_row_calls_native_and_through_ctypes(lib, monkeypatch, tmp_path):
             assert L.STATUS[getattr(form, name)(*args)] == "badArgument", name
             with pytest.raises(TypeError):
                 getattr(form, name)(*args[:-1])
+
+
+def test_head_rows_of_one_row_or_one_head():
+    """strides of dimensions of size one mean nothing"""
+    api._torch()
+    x = torch.zeros(4, 128)
+    one_row = x[None].expand(1, 4, 128).as_strided((1, 4, 128), (0, 128, 1))
+    assert api._head_rows(one_row, "q") == (torch.Size([1, 4, 128]), 512)
+    assert api._head_rows(x[None].as_strided((1, 4, 128), (7, 128, 1)), "q")[1] == 512
+    one_head = x.as_strided((4, 1, 128), (128, 1, 1))
+    assert api._head_rows(one_head, "k") == (torch.Size([4, 1, 128]), 128)
+    assert api._head_rows(x[:1].as_strided((1, 1, 128), (0, 0, 1)), "k")[1] == 128

@@ -839,6 +839,8 @@ class PagedKV:
         kind = {torch.float16: L.KV_F16, torch.float32: L.KV_F32}.get(k.dtype)
         if kind is None:
             raise TypeError(f"cache pools of {k.dtype}: float16 or float32 is wanted")
+        if not k.device == v.device == table.device:
+            raise ValueError(f"pools on {k.device} and {v.device}, block table on {table.device}: one device is wanted")
         self = cls.__new__(cls)
         blocks, page, kv_heads, head_dim = k.shape
         self.layout = L.KVLayout(kind, page, kv_heads, head_dim, blocks, table.shape[1], table.shape[0])
@@ -847,10 +849,15 @@ class PagedKV:
         self.table_host, self.free, self.owned = None, [], None
         return self
 
+    def _own_blocks(self):
+        if self.owned is None:
+            raise ValueError("the caller hands out this cache's blocks")
+
     def ensure(self, slot: int, pos: int) -> int:
         """Make sequence `slot` own the block of `pos`; returns the flat pool position."""
         import torch
 
+        self._own_blocks()
         need = pos // self.page + 1
         if need > self.max_blocks:
             raise IndexError("beyond context")
@@ -869,6 +876,7 @@ class PagedKV:
     def release(self, slot: int):
         import torch
 
+        self._own_blocks()
         while self.owned[slot]:
             self.free.append(self.owned[slot].pop())
         self.table_host[slot] = 0

@@ -103,3 +103,19 @@ def test_head_rows_of_one_row_or_one_head():
     one_head = x.as_strided((4, 1, 128), (128, 1, 1))
     assert api._head_rows(one_head, "k") == (torch.Size([4, 1, 128]), 128)
     assert api._head_rows(x[:1].as_strided((1, 1, 128), (0, 0, 1)), "k")[1] == 128
+
+
+@pytest.mark.parametrize("where", ["v", "table"])
+def test_cache_over_pools_of_two_devices_is_refused(where):
+    """a kernel would follow the other device's address"""
+    t = dict(k=torch.zeros(4, 16, 2, 128, dtype=torch.float16), v=torch.zeros(4, 16, 2, 128, dtype=torch.float16), table=torch.zeros(2, 3, dtype=torch.int32))
+    t[where] = t[where].to("meta")
+    with pytest.raises(ValueError, match="one device"):
+        api.PagedKV.over(t["k"], t["v"], t["table"])
+
+
+def test_blocks_of_a_cache_over_pools_are_the_callers():
+    c = api.PagedKV.over(torch.zeros(4, 16, 2, 128, dtype=torch.float16), torch.zeros(4, 16, 2, 128, dtype=torch.float16), torch.zeros(2, 3, dtype=torch.int32))
+    for call in (lambda: c.ensure(0, 5), lambda: c.release(0)):
+        with pytest.raises(ValueError, match="hands out"):
+            call()

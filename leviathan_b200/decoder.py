@@ -135,7 +135,8 @@ class SyntheticDecoder:
                 for w in (wq, wk, wv) if prompts else (wq, wk, wv, wo):
                     w.release_gguf()   # only the decode kernels read these: one resident copy instead of two
             moe = self._experts(l)
-            cache = PagedKV(batch * blocks_per_seq + 1, cfg.page, KVH, HD, slots=batch, max_blocks=blocks_per_seq, dtype="f16", device=device)
+            # one slot more for prompts: its entries stay at the scratch block, where rows that belong to no chunk go
+            cache = PagedKV(batch * blocks_per_seq + 1, cfg.page, KVH, HD, slots=batch + prompts, max_blocks=blocks_per_seq, dtype="f16", device=device)
             for s in range(batch):
                 cache.ensure(s, cfg.positions - 1)
             self._fill(cache.k, f"blk.{l}.cache_k")
@@ -288,16 +289,19 @@ class SyntheticDecoder:
 
     # ---- prompts ----
     def _rows_of(self, start, n: int):
-        """for each of n rows: its chunk and its number inside the chunk"""
+        """for each of n rows: its chunk, its number inside the chunk, and whether it has one (rows in front of start[0] and behind
+        start[-1], the padding of a batch of fixed size, do not)"""
         import torch
 
         row = torch.arange(n, device=self.dev)
-        chunk = torch.bucketize(row, start[1:].long(), right=True)
-        return chunk, (row - start.long()[chunk]).to(torch.int32)
+        chunk = torch.bucketize(row, start[1:].long(), right=True).clamp_(max=start.numel() - 2)
+        inside = (row >= start[0]) & (row < start[-1])
+        return chunk, torch.where(inside, row - start.long()[chunk], 0).to(torch.int32), inside
 
     def _layers_of_prompt(self, tokens, attend):
         """Embedding rows, all layers and the final norm over rows of tokens -> bf16 [rows][hidden].  `attend(layer, qkv)` gives a
-        layer's attention output, bf16 [rows][q_heads][head_dim], from the fused projection's f32 rows."""
+        layer's attention output, bf16 [rows][q_heads][head_dim], from the fused projection's f32 rows, in the buffer that it is given
+        (zeros where no chunk has rows)."""
         import torch
 
         c, ctx, n = self.cfg, self.ctx, tokens.numel()
@@ -306,9 +310,10 @@ class SyntheticDecoder:
         bf16 = torch.bfloat16
         x = ctx.embed_rows(self.head, tokens, math.sqrt(c.hidden))
         h = ctx.act_bf16(ctx.rmsnorm(x, self.layers[0].attn_norm, c.eps))
+        a = torch.zeros((n, c.q_heads, c.head_dim), dtype=bf16, device=self.dev)
         nexts = [L.attn_norm for L in self.layers[1:]] + [self.out_norm]
         for L, norm in zip(self.layers, nexts):
-            a = attend(L, ctx.gemm_prefill(L.wqkv, h))
+            attend(L, ctx.gemm_prefill(L.wqkv, h), a)
             o = ctx.gemm_prefill(L.wo, a.view(n, c.q_heads * c.head_dim))
             x, f = ctx.norm_residual(o, x, pre=L.ffn_norm, eps=c.eps, out=x)
             o = ctx.moe_layer(L.moe, f, c.top_k)
@@ -317,40 +322,45 @@ class SyntheticDecoder:
 
     def prefill(self, tokens, start, slot, pos):
         """Takes new tokens into the caches: rows start[i] ... start[i + 1] - 1 of `tokens` (int32) continue sequence slot[i] at position
-        pos[i] (int32 device tensors; at least one token each).  Returns (next tokens int32 [chunks], softcapped logits [chunks][vocab]) behind
-        each chunk's last token: what the Rust runtime's prefill_advance leaves (rust/crates/lev-model/src/gpu.rs:1346)."""
+        pos[i] (int32 device tensors; at least one token each, what an empty chunk returns means nothing).  Tokens in front of start[0] and
+        behind start[-1] are padding: they may be anything and reach no sequence.  Returns (next tokens int32 [chunks], softcapped logits
+        [chunks][vocab]) behind each chunk's last token: what the Rust runtime's prefill_advance leaves (rust/crates/lev-model/src/gpu.rs:1346)."""
         import torch
 
         c, ctx = self.cfg, self.ctx
-        chunk, within = self._rows_of(start, tokens.numel())
-        row_slot, row_pos = slot[chunk].contiguous(), pos[chunk] + within
+        chunk, within, inside = self._rows_of(start, tokens.numel())
+        slot = torch.where(slot < self.batch, slot, -1)   # the scratch slot is no sequence: reported like any other bad one
+        row_slot = torch.where(inside, slot[chunk], self.batch)
+        row_pos = torch.where(inside, pos[chunk] + within, 0)
 
-        def attend(L, qkv):
+        def attend(L, qkv, out):
             ctx.qkv_norm_rope_append(qkv, c.q_heads, L.cache, row_slot, row_pos, L.q_norm, L.k_norm, c.eps, self.inv_freq)
             q = qkv.view(-1, c.q_heads + 2 * c.kv_heads, c.head_dim)[:, :c.q_heads]
-            return ctx.attn_chunk(L.cache, start, slot, pos, q, 0, c.attn_scale)
+            ctx.attn_chunk(L.cache, start, slot, pos, q, 0, c.attn_scale, out=out)
 
-        h = self._layers_of_prompt(tokens, attend)
-        logits = ctx.softcap(ctx.gemm_prefill(self.head, h.index_select(0, start[1:].long() - 1)), c.softcap)
+        h = self._layers_of_prompt(torch.where(inside, tokens, 0), attend)
+        last = (start[1:].long() - 1).clamp_(0, tokens.numel() - 1)
+        logits = ctx.softcap(ctx.gemm_prefill(self.head, h.index_select(0, last)), c.softcap)
         return ctx.argmax(logits), logits
 
     def score(self, tokens, start, top: int = 0, rows: int = 512):
         """Whole prompts packed behind one another, no cache: for every row the log probability of the next token of its prompt (0 behind a
-        prompt's last token), the entropy of the prediction and its `top` alternatives (see Context.logprobs).  Logits are made `rows` rows at a time."""
+        prompt's last token), the entropy of the prediction and its `top` alternatives (see Context.logprobs).  Logits are made `rows` rows at a time.
+        Tokens in front of start[0] and behind start[-1] are padding and may be anything; their log probability is 0, the rest means nothing."""
         import torch
 
         c, ctx, n = self.cfg, self.ctx, tokens.numel()
-        _, within = self._rows_of(start, n)
+        chunk, within, inside = self._rows_of(start, n)
 
-        def attend(L, qkv):
+        def attend(L, qkv, out):
             ctx.qkv_norm_rope(qkv, c.q_heads, c.kv_heads, c.head_dim, L.q_norm, L.k_norm, c.eps, self.inv_freq, within)
             b = ctx.act_bf16(qkv).view(n, c.q_heads + 2 * c.kv_heads, c.head_dim)
-            return ctx.attn_prompt(b[:, :c.q_heads], b[:, c.q_heads:c.q_heads + c.kv_heads], b[:, c.q_heads + c.kv_heads:], start, 0, c.attn_scale)
+            ctx.attn_prompt(b[:, :c.q_heads], b[:, c.q_heads:c.q_heads + c.kv_heads], b[:, c.q_heads + c.kv_heads:], start, 0, c.attn_scale, out=out)
 
-        h = self._layers_of_prompt(tokens, attend)
-        given = torch.full_like(tokens, -1)
-        given[:-1] = tokens[1:]
-        given[start[1:].long() - 1] = -1   # nothing follows a prompt's last token
+        h = self._layers_of_prompt(torch.where(inside, tokens, 0), attend)
+        # nothing follows a prompt's last token
+        row = torch.arange(n, device=self.dev)
+        given = torch.where(inside & (row + 1 < start[1:][chunk]), tokens.roll(-1), -1)
         parts = [ctx.logprobs(ctx.gemm_prefill(self.head, h[a:a + rows]), given[a:a + rows], top=top, softcap=c.softcap) for a in range(0, n, rows)]
         return tuple(None if p[0] is None else torch.cat(p) for p in zip(*parts))
 

@@ -210,3 +210,54 @@ def test_prompts_are_refused_without_their_tensors(ctx):
     with pytest.raises(ValueError, match="prompts=True"):
         dec.prefill(one, torch.tensor([0, 1], dtype=torch.int32, device="cuda"), one, one)
     dec.free()
+
+
+def test_padding_of_a_prompt_batch_reaches_no_sequence(ctx):
+    """a batch of fixed size: tokens in front of the first chunk and behind the last one are junk, and the caches keep what they held"""
+    cfg = DecoderConfig(**PROMPT)
+    dec = SyntheticDecoder(ctx, cfg, batch=3, prompts=True)
+    i32 = lambda v: torch.tensor(np.asarray(v), dtype=torch.int32, device="cuda")  # noqa: E731
+    rng = np.random.default_rng(5)
+    toks = rng.integers(0, cfg.vocab, 30)
+    slot, pos = i32([2, 0]), i32([40, 7])
+    pools = [t.clone() for L in dec.layers for t in (L.cache.k, L.cache.v)]
+    want, logits = dec.prefill(i32(toks), i32([0, 11, 30]), slot, pos)
+    ctx.synchronize()
+    filled = [t.clone() for L in dec.layers for t in (L.cache.k, L.cache.v)]
+    for t, p in zip((t for L in dec.layers for t in (L.cache.k, L.cache.v)), pools):
+        t.copy_(p)
+    padded = np.concatenate([[-1, 5, cfg.vocab, 1 << 30, 3], toks, [-7] * 9, rng.integers(0, cfg.vocab, 40)])
+    got, padded_logits = dec.prefill(i32(padded), i32([5, 16, 35]), slot, pos)
+    ctx.synchronize()
+    _near(padded_logits.cpu().numpy(), logits.cpu().numpy())
+    mine = {0: range(7, 26), 2: range(40, 51)}
+    held = torch.ones(dec.layers[0].cache.k.shape[:2], dtype=torch.bool, device="cuda")
+    held[0] = False   # the scratch block
+    for s, positions in mine.items():
+        for p in positions:
+            held[dec.layers[0].cache.owned[s][p // cfg.page], p % cfg.page] = False
+    for t, before, after in zip((t for L in dec.layers for t in (L.cache.k, L.cache.v)), pools, filled):
+        assert torch.equal(t[held], before[held])
+        _near(t[~held].float().cpu().numpy()[cfg.page:], after[~held].float().cpu().numpy()[cfg.page:])
+    # a slot that is no sequence's is reported
+    dec.prefill(i32(toks), i32([0, 11, 30]), i32([3, 0]), pos)
+    with pytest.raises(lev.LevError, match="badDimensions"):
+        ctx.synchronize()
+    dec.free()
+
+
+def test_padding_of_scored_prompts(ctx):
+    cfg = DecoderConfig(**PROMPT)
+    dec = SyntheticDecoder(ctx, cfg, batch=1, prompts=True)
+    i32 = lambda v: torch.tensor(np.asarray(v), dtype=torch.int32, device="cuda")  # noqa: E731
+    rng = np.random.default_rng(6)
+    toks = rng.integers(0, cfg.vocab, 40)
+    lp, ent, ids, lps = dec.score(i32(toks), i32([0, 0, 15, 15, 40]), top=3)
+    padded = np.concatenate([[-5, cfg.vocab], toks, [1 << 29] * 7])
+    plp, pent, pids, plps = dec.score(i32(padded), i32([2, 2, 17, 17, 42]), top=3)
+    ctx.synchronize()
+    assert lp[14] == 0 and lp[39] == 0 and (lp[:14] < 0).all() and (lp[15:39] < 0).all()
+    assert (plp[:2] == 0).all() and (plp[42:] == 0).all()
+    for a, b in ((plp, lp), (pent, ent), (plps, lps)):
+        _near(a[2:42].cpu().numpy(), b.cpu().numpy())
+    dec.free()

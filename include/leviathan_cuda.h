@@ -433,7 +433,8 @@ int lev_qkv_norm_rope_append_split(lev_ctx* ctx, float* q, float* k, float* v, i
  * A slot or position outside the layout, or a table entry outside the pool, is not followed: rows of that chunk are NaN (of an entry, those
  * that attend to its page, and others of the chunk may be); start entries that are no range leave their chunk out; both are reported by
  * the next status read.  Cached values that a row does not attend to may
- * be anything, NaN included (in front of a window or among the new tokens they cost a second, slow pass over the rows concerned).  No work buffers: captured graphs and streams share nothing.  Repeat runs give the same bits. */
+ * be anything, NaN included (in front of a window or among the new tokens they cost a second, slow pass over the rows concerned: seconds behind
+ * 10000 positions and more).  No work buffers: captured graphs and streams share nothing.  Repeat runs give the same bits. */
 int lev_attn_chunk(lev_ctx* ctx, const lev_kv_layout* layout, const void* k_pool, const void* v_pool,
                    const int32_t* block_table, int n_chunks, const int32_t* start, const int32_t* slot,
                    const int32_t* pos, int64_t n_rows, int q_heads, const void* q, int q_type,

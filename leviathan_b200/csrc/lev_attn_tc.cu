@@ -15,7 +15,8 @@
 // The reference m of a row follows its running maximum only when that has moved by more than 2^8 (the weights stay
 // below 256, exact in 16 bits to the same relative error), so that O is rescaled in a handful of steps and not in every
 // one.  Sums of weights are f32, O is f32 in tensor memory.  Rounded to 16 bits: q where it comes as f32 (the cache is
-// f16, and both operands of an MMA have one type), P (11 bits for f16, 8 for bf16 prompts), the output.
+// f16, and both operands of an MMA have one type), K and V of f32 pools, P (11 bits for f16, 8 for bf16 prompts; what f16 loses below 2^-24
+// of the reference is still in the sum, at most 2^-25 per position), the output.
 //
 // Roles of a CTA: one (two) softmax warpgroup(s), one warp that issues MMAs, three that request TMA boxes or, where the cache cannot be
 // boxed (f32 pools, pages that are no whole groups of eight rows), copy rows.  A CTA keeps its tensor memory and barriers from unit to
@@ -28,10 +29,11 @@
 // is computed once more, position by position, over the places that it does attend to (tc_row_again; slow, and never taken where all
 // values are finite).
 //
-// What bounds it: for 16 heads of 256 on 8, a prompt of 4096 takes 104 us = 1.32 PFLOP/s (0.80 of a library product's burst rate; the
-// tensor pipe is active 70 % of the cycles, the rest is the diagonal's half steps and the softmax between two products).  For 32 heads of
-// 128 (two tiles) the warps that make the weights bound it: 24 chunks of mixed lengths 176 us = 0.74 PFLOP/s, the tensor pipe active 45 %;
-// an exponential costs as much as 8 of a tile's multiply-adds there.  Few tokens on a long cache: 5 tokens behind 4091
+// What bounds it: for 16 heads of 256 on 8, a prompt of 4096 takes 106 us = 1.30 PFLOP/s (0.78 of a library product's burst rate; over
+// seconds, under the power cap, 125 us = 0.80 of its sustained rate; the tensor pipe is active 70 % of the cycles, the rest is the
+// diagonal's half steps and the softmax between two products).  For 32 heads of 128 (two tiles) the warps that make the weights bound it:
+// 24 chunks of mixed lengths 177 us = 0.73 PFLOP/s (over seconds 207), the tensor pipe active 45 %; an exponential costs as much as 8 of a
+// tile's multiply-adds there.  Few tokens on a long cache: 5 tokens behind 4091
 // positions, 33.6 MB, 20 us = 1.7 TB/s, a chain of latencies (start, table, K, scores, weights, V, merge) of which the bytes take 5.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -20,8 +20,8 @@
 // A row belongs to a cluster of up to eight thread blocks, whose partial results the first one joins through distributed
 // shared memory: no work buffer, no second launch.
 //
-// What bounds it: 512 rows of 262144 f32 logits with a softcap and 20 alternatives (537 MB) take 116 us = 4.6 TB/s (0.71 of the copy
-// peak), without alternatives 99 us.  With a cap a value costs an exponential twice and a quarter of a reciprocal: the special
+// What bounds it: 512 rows of 262144 f32 logits with a softcap and 20 alternatives (537 MB) take 120 us = 4.5 TB/s (0.68 of the copy
+// peak), without alternatives 101 us.  With a cap a value costs an exponential twice and a quarter of a reciprocal: the special
 // function units alone need about 67 us, issue slots are at 66 %; the alternatives add the sorting at the end of each row, which the
 // other blocks of the SM cover in part.
 #include <cuda_bf16.h>
